@@ -100,6 +100,88 @@ int sepia_gpu_moe_prefill(const SepiaMoeLayerDesc *layer, int64_t n_tokens, Sepi
 int sepia_gpu_expert_ffn(const SepiaExpertTensor *gate, const SepiaExpertTensor *up, const SepiaExpertTensor *down,
                          int n_experts, int expert, int64_t hidden, int64_t inter, SepiaGpuBuf *x, SepiaGpuBuf *y);
 
+/* ---- Serving: a paged 8-bit key/value cache and sampling -----------------
+ * No counterpart in the reference, whose cache is one sequence's f32 rows
+ * (src/sepia.c:1203-1247) and whose next token is the host's arg-max. */
+
+/* A layer's cache for n_seqs sequences. The pool holds n_pages pages of
+ * `page` tokens (16, 32 or 64); page p is 2 * n_kv_heads * page * head_dim
+ * bytes of codes at codes_off + p times that: K int8 [kv head][token][dim],
+ * then V int8 [kv head][dim][token] (a dim's tokens side by side), and f32
+ * scales [p][K, V][kv head] at scales_off: a cached value is code * scale.
+ * Row s of the table (int32 [n_seqs][max_pages] at table_off) holds the pages
+ * of sequence s in order; entries behind its last token are not read. A page
+ * may stand in several rows (a shared prefix) as long as no call appends to
+ * it. head_dim: a multiple of 16 up to 128. codes_off a multiple of 16, the
+ * others of 4; max_pages * page at most 2^31 - 1. */
+typedef struct {
+    int64_t n_pages, max_pages;
+    int n_seqs, n_kv_heads, head_dim, page;
+    SepiaGpuBuf *codes, *scales, *table;
+    size_t codes_off, scales_off, table_off;
+} SepiaKv8Cache;
+
+/* The rows of a call belong to the cache's sequences back to back: lens
+ * (int32 [n_seqs]) holds the tokens that sequence s has in the cache before
+ * the call, and its new rows are starts[s] .. starts[s + 1] - 1 (int32
+ * [n_seqs + 1], rising) at positions lens[s], lens[s] + 1, ... A sequence may
+ * have none. n_tokens rows are there (at most 2^24); rows outside all
+ * sequences are left as they are. lens, starts and the table are read on the
+ * device when the launch runs, so a captured call follows what they hold at
+ * its replay. A page outside the pool, or lengths and rows that do not fit
+ * the call or the table, make the batch fail at sepia_gpu_end (device errors
+ * 6 and 7) and touch nothing outside the buffers.
+ *
+ * append: rows k, v (f32 [n_tokens][n_kv_heads * head_dim]) into the pages.
+ * With k_norm (f32 [head_dim]; NULL: none) a key x of a head becomes
+ * x * k_norm / sqrt(mean(x^2) + eps) first. The scale of a (page, K or V,
+ * head) covers the page's tokens so far: it grows to the largest new
+ * magnitude / 127 (in f32, times 1 / 127) where that is larger, and the codes
+ * that are there are rounded anew; a page's first token starts it afresh. A value that is not
+ * finite makes that scale NaN, and with it what the page's head stands for.
+ * Two sequences of one call may not append to the same page. */
+int sepia_hip_kv8_append(const SepiaKv8Cache *cache, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n_tokens,
+                         SepiaGpuBuf *k, SepiaGpuBuf *v, SepiaGpuBuf *k_norm, float eps);
+
+/* Cached rows as f32: k, v [n_tokens][n_kv_heads * head_dim]; row i of
+ * sequence s is position first[s] + i (first in the place of lens). */
+int sepia_hip_kv8_read(const SepiaKv8Cache *cache, SepiaGpuBuf *first, SepiaGpuBuf *starts, int64_t n_tokens,
+                       SepiaGpuBuf *k, SepiaGpuBuf *v);
+
+/* Attention of the call's rows over the cache (their own keys and values
+ * appended before): row t at position p of its sequence sees the positions
+ * [max(0, p - window + 1), p] (window 0: [0, p]). As in sepia_gpu_banded_attn:
+ * scores q . k * inv_head_dim + (p - j < rel_extent ? rel_logits[t][head]
+ * [p - j] * tau[t] : 0), softmax, weighted v. q, out: f32 [n_tokens][n_heads]
+ * [head_dim] (out may be q); rel_logits f32 [n_tokens][n_heads][rel_extent],
+ * NULL with rel_extent 0: no such term; tau f32 [n_tokens], NULL: 1. n_heads
+ * is a multiple of n_kv_heads, up to 16 times. A row whose scores are all -inf
+ * is NaN. */
+int sepia_hip_kv8_attn(const SepiaKv8Cache *cache, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n_tokens,
+                       SepiaGpuBuf *q, SepiaGpuBuf *rel_logits, SepiaGpuBuf *tau, SepiaGpuBuf *out,
+                       int64_t n_heads, int64_t rel_extent, int64_t window, float inv_head_dim);
+
+/* What each row asks of sepia_hip_sample; one value a row. */
+typedef struct {
+    SepiaGpuBuf *u;             /* f32, a uniform random number in [0, 1) */
+    SepiaGpuBuf *temperature;   /* f32, NULL: 1; 0 or less (or NaN): the row's first token of the order */
+    SepiaGpuBuf *top_p;         /* f32, NULL, 1 or more, or NaN: off */
+    SepiaGpuBuf *min_p;         /* f32, NULL, 0 or less, or NaN: off; more than 1 counts as 1 */
+    SepiaGpuBuf *top_k;         /* int32, NULL or 0 or less: off */
+} SepiaSampleDesc;
+
+/* The next token of each row of logits (f32, up to 2^20 rows, row r at element
+ * r * stride, vocab values of it, 1 to 2^20). A token's weight is exp((logit - largest) /
+ * temperature); -inf and NaN have none. In the order of falling logits, equal
+ * ones by index: the first top_k tokens are kept, of these the shortest
+ * beginning with at least top_p of their weight, of these the ones of weight
+ * min_p or more. tokens[r] (int32) is the first whose cumulative weight
+ * exceeds u times the kept weight, -1 for a row without any finite or +inf
+ * logit; prob[r] (f32, NULL: not wanted) its share of the kept weight. Sums of
+ * weights are exact in units of 2^-44 of the largest weight. */
+int sepia_hip_sample(const SepiaSampleDesc *desc, SepiaGpuBuf *logits, int64_t rows, int64_t vocab, int64_t stride,
+                     SepiaGpuBuf *tokens, SepiaGpuBuf *prob);
+
 /* Launch timing: between start and stop every launch is bracketed by a pair
  * of HIP events on the stream it runs on; stop waits for the stream and adds
  * each launch's duration to its kernel's total. query reads the totals of a
@@ -149,7 +231,9 @@ uint64_t sepia_hip_uploaded_bytes(void);
 
 /* The first device error a kernel recorded since the last call, 0 if none,
  * and clears it. A kernel records one when a bounded spin wait expires (code
- * 5): its launch's outputs are then invalid. sepia_gpu_end checks and
+ * 5), a cache's table names a page outside its pool (6) or a sequence's
+ * length or rows do not fit the call (7): its launch's outputs are then
+ * invalid. sepia_gpu_end checks and
  * clears it itself and fails the batch (logging the code); callers that run
  * the library's launches without ending a batch (a captured graph replayed
  * on the library's stream) call this after synchronizing. No counterpart in

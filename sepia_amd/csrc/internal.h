@@ -1,5 +1,5 @@
-/* internal.h -- what the other host files of libsepia_hip.so (store.c) use
- * of sepia_hip.c. Not exported. */
+/* internal.h -- what the other host files of libsepia_hip.so (store.c,
+ * serve.c) use of sepia_hip.c. Not exported. */
 #ifndef SEPIA_INTERNAL_H
 #define SEPIA_INTERNAL_H
 
@@ -28,6 +28,23 @@ SEPIA_HIDDEN size_t sepia_buf_len(const SepiaGpuBuf *b);
 SEPIA_HIDDEN int64_t sepia_row_bytes(int ggml_type, int64_t n);
 /* Count one device or pinned-host allocation (sepia_hip_alloc_count). */
 SEPIA_HIDDEN void sepia_count_alloc(void);
+/* An op's checks and preparations (serve.c), as sepia_hip.c's own ops make
+ * them: an open batch; [off, off + n) inside a buffer; an input's host-written
+ * parts of a range uploaded; an output's device copy current, and downloaded
+ * at sepia_gpu_end. Each logs and returns 0 on failure. */
+SEPIA_HIDDEN int sepia_need_batch(const char *op);
+SEPIA_HIDDEN int sepia_chk(const SepiaGpuBuf *b, size_t off, size_t n, const char *op, const char *what);
+SEPIA_HIDDEN int sepia_prep_in(SepiaGpuBuf *b, size_t off, size_t n, const char *op);
+SEPIA_HIDDEN int sepia_prep_out(SepiaGpuBuf *b, const char *op);
+/* The scratch's data region of at least `need` bytes (NULL: logged). */
+SEPIA_HIDDEN void *sepia_scratch(size_t need, const char *op);
+
+/* Kernels of the second code object (kernels/sepia_serve.hip), and a launch
+ * of one on the library's stream, timed when the profiler is on. */
+enum { SK_KV8_APPEND, SK_KV8_READ, SK_KV8_ATTN, SK_SAMPLE, SK_COUNT };
+SEPIA_HIDDEN int sepia_serve_launch(int k, unsigned gx, unsigned gy, unsigned gz, unsigned block, void **args,
+                                    const char *op);
+
 /* Release store.c's pinned staging buffers (sepia_gpu_shutdown calls it). */
 SEPIA_HIDDEN void sepia_store_shutdown(void);
 

@@ -104,6 +104,14 @@ static const char *const k_names[K_COUNT] = {
 };
 #undef FFN_NAMES
 
+/* Kernels of the second code object, sepia_serve.hsaco (the SK_* of
+ * internal.h); their ids follow the first's. */
+static const char *const serve_names[SK_COUNT] = {
+    "sepia_kv8_append", "sepia_kv8_read", "sepia_kv8_attn", "sepia_sample",
+};
+#define K_ALL (K_COUNT + SK_COUNT)
+static const char *k_name(int k) { return k < K_COUNT ? k_names[k] : serve_names[k - K_COUNT]; }
+
 /* GGUF block geometry (reference src/quants.c:28-56; tools/gguf_inspect.py:109-117). */
 typedef struct {
     int type;
@@ -203,9 +211,9 @@ static int g_cus = 0;               /* compute units, from the device at init */
 static int g_have_iq2xxs;
 static int g_noalloc_ok;            /* the allocation-free entry's device array is set up */
 static char g_device_name[256];
-static hipModule_t g_module;
+static hipModule_t g_module, g_serve_module;
 static hipStream_t g_stream;
-static hipFunction_t g_fn[K_COUNT];
+static hipFunction_t g_fn[K_ALL];
 static int g_batch_open;
 
 static const TypeInfo *type_info(int t) {
@@ -639,11 +647,11 @@ uint64_t sepia_hip_uploaded_bytes(void) { return g_uploaded; }
 /* ------------------------------------------------------------ lifecycle - */
 int sepia_gpu_available(void) { return g_available; }
 
-/* dir/sepia_kernels.hsaco if that file exists, else the code object beside
+/* dir/`file` if that file exists, else the code object of that name beside
  * this shared library. 0 if neither path fits in `path`. */
-static int kernel_path(const char *dir, char *path, size_t cap) {
+static int kernel_path(const char *dir, const char *file, char *path, size_t cap) {
     if (dir && dir[0]) {
-        if ((size_t)snprintf(path, cap, "%s/sepia_kernels.hsaco", dir) >= cap) return 0;
+        if ((size_t)snprintf(path, cap, "%s/%s", dir, file) >= cap) return 0;
         if (access(path, R_OK) == 0) return 1;
     }
     Dl_info info;
@@ -651,10 +659,10 @@ static int kernel_path(const char *dir, char *path, size_t cap) {
         const char *slash = strrchr(info.dli_fname, '/');
         const int len = slash ? (int)(slash - info.dli_fname) : 1;
         const char *base = slash ? info.dli_fname : ".";
-        if ((size_t)snprintf(path, cap, "%.*s/sepia_kernels.hsaco", len, base) >= cap) return 0;
+        if ((size_t)snprintf(path, cap, "%.*s/%s", len, base, file) >= cap) return 0;
         if (access(path, R_OK) == 0) return 1;
     }
-    if (dir && dir[0]) snprintf(path, cap, "%s/sepia_kernels.hsaco", dir);  /* report the caller's path */
+    if (dir && dir[0]) snprintf(path, cap, "%s/%s", dir, file);  /* report the caller's path */
     return 1;
 }
 
@@ -702,6 +710,9 @@ static int err_word_setup(void) {
     void *dp = NULL;
     e = hipHostGetDevicePointer(&dp, (void *)g_err_host, 0);
     if (e == hipSuccess) e = hipMemcpyHtoD(gp, &dp, sizeof dp);
+    if (e == hipSuccess) e = hipModuleGetGlobal(&gp, &gsz, g_serve_module, "sepia_err_word");
+    if (e == hipSuccess && gsz != sizeof(void *)) e = hipErrorInvalidSymbol;
+    if (e == hipSuccess) e = hipMemcpyHtoD(gp, &dp, sizeof dp);
     if (e != hipSuccess) {
         LOG("init: publishing the device error word failed: %s", hipGetErrorString(e));
         return 0;
@@ -716,6 +727,43 @@ unsigned sepia_hip_take_device_error(void) {
     const unsigned code = *g_err_host;
     if (code) *g_err_host = 0;
     return code;
+}
+
+static void unload_kernels(void) {
+    if (g_module) hipModuleUnload(g_module);
+    if (g_serve_module) hipModuleUnload(g_serve_module);
+    g_module = g_serve_module = NULL;
+}
+
+/* Both code objects, each from kernel_dir or from beside the library, and
+ * every kernel in them. */
+static int load_kernels(const char *kernel_dir) {
+    static const struct {
+        const char *file;
+        hipModule_t *module;
+        int k0, k1;
+    } objects[] = { { "sepia_kernels.hsaco", &g_module, 0, K_COUNT },
+                    { "sepia_serve.hsaco", &g_serve_module, K_COUNT, K_ALL } };
+    for (size_t i = 0; i < sizeof objects / sizeof objects[0]; i++) {
+        char path[4096];
+        if (!kernel_path(kernel_dir, objects[i].file, path, sizeof path)) {
+            LOG("init: kernel directory path too long");
+            return 0;
+        }
+        hipError_t e = hipModuleLoad(objects[i].module, path);
+        if (e != hipSuccess) {
+            *objects[i].module = NULL;
+            LOG("cannot load %s: %s", path, hipGetErrorString(e));
+            return 0;
+        }
+        for (int k = objects[i].k0; k < objects[i].k1; k++) {
+            if ((e = hipModuleGetFunction(&g_fn[k], *objects[i].module, k_name(k))) != hipSuccess) {
+                LOG("kernel \"%s\" not found in %s: %s", k_name(k), path, hipGetErrorString(e));
+                return 0;
+            }
+        }
+    }
+    return 1;
 }
 
 int sepia_gpu_init(const char *kernel_dir) {
@@ -741,30 +789,12 @@ int sepia_gpu_init(const char *kernel_dir) {
     }
     g_lds_max = prop.sharedMemPerBlock ? prop.sharedMemPerBlock : 65536;
     g_cus = prop.multiProcessorCount;
-    char path[4096];
-    if (!kernel_path(kernel_dir, path, sizeof path)) {
-        LOG("init: kernel directory path too long");
-        return 0;
-    }
     if ((e = hipStreamCreate(&g_stream)) != hipSuccess) {
         LOG("failed to create a stream: %s", hipGetErrorString(e));
         return 0;
     }
-    if ((e = hipModuleLoad(&g_module, path)) != hipSuccess) {
-        LOG("cannot load %s: %s", path, hipGetErrorString(e));
-        hipStreamDestroy(g_stream);
-        return 0;
-    }
-    for (int k = 0; k < K_COUNT; k++) {
-        if ((e = hipModuleGetFunction(&g_fn[k], g_module, k_names[k])) != hipSuccess) {
-            LOG("kernel \"%s\" not found in %s: %s", k_names[k], path, hipGetErrorString(e));
-            hipModuleUnload(g_module);
-            hipStreamDestroy(g_stream);
-            return 0;
-        }
-    }
-    if (!err_word_setup()) {
-        hipModuleUnload(g_module);
+    if (!load_kernels(kernel_dir) || !err_word_setup()) {
+        unload_kernels();
         hipStreamDestroy(g_stream);
         return 0;
     }
@@ -790,7 +820,7 @@ void sepia_gpu_shutdown(void) {
     if (g_scratch) hipFree(g_scratch);
     g_scratch = NULL;
     g_scratch_len = 0;
-    hipModuleUnload(g_module);
+    unload_kernels();
     hipStreamDestroy(g_stream);
     g_available = 0;
     g_batch_open = 0;
@@ -824,6 +854,13 @@ int sepia_gpu_flush(void) {
     return 1;
 }
 
+/* What a device error's code stands for. */
+static const char *device_error(unsigned code) {
+    if (code == 6) return "a page of a cache's table lies outside its pool";
+    if (code == 7) return "a sequence's length or rows do not fit the call";
+    return "a kernel's bounded wait expired";
+}
+
 int sepia_gpu_end(void) {
     if (!need_init("end")) return 0;
     if (!g_batch_open) {
@@ -845,7 +882,7 @@ int sepia_gpu_end(void) {
     }
     const unsigned code = sepia_hip_take_device_error();
     if (code) {
-        LOG("end: a kernel's bounded wait expired (device error %u); the batch's outputs are invalid", code);
+        LOG("end: %s (device error %u); the batch's outputs are invalid", device_error(code), code);
         return 0;
     }
     return 1;
@@ -860,8 +897,8 @@ static int g_prof_overflow;
 static hipEvent_t g_prof_ev[PROF_MAX][2];
 static int g_prof_kid[PROF_MAX];
 static int g_prof_ev_made;
-static double g_prof_ms[K_COUNT];
-static int64_t g_prof_cnt[K_COUNT];
+static double g_prof_ms[K_ALL];
+static int64_t g_prof_cnt[K_ALL];
 
 /* AMD's launch extension (declared in the C++-only hip/hip_ext.h): the
  * start/stop events are attached to the dispatch itself, so their interval
@@ -888,10 +925,22 @@ static int launch3(int k, unsigned gx, unsigned gy, unsigned gz, unsigned block,
         e = hipModuleLaunchKernel(g_fn[k], gx, gy, gz, block, 1, 1, (unsigned)lds, g_stream, args, NULL);
     }
     if (e != hipSuccess) {
-        LOG("%s: launch of %s failed: %s", op, k_names[k], hipGetErrorString(e));
+        LOG("%s: launch of %s failed: %s", op, k_name(k), hipGetErrorString(e));
         return 0;
     }
     return 1;
+}
+
+/* ---- more hooks for the other host files (internal.h) ---- */
+int sepia_need_batch(const char *op) { return need_batch(op); }
+int sepia_chk(const SepiaGpuBuf *b, size_t off, size_t n, const char *op, const char *what) {
+    return chk(b, off, n, op, what);
+}
+int sepia_prep_in(SepiaGpuBuf *b, size_t off, size_t n, const char *op) { return prep_in_r(b, off, n, op); }
+int sepia_prep_out(SepiaGpuBuf *b, const char *op) { return prep_out(b, op); }
+void *sepia_scratch(size_t need, const char *op) { return scratch(need, op); }
+int sepia_serve_launch(int k, unsigned gx, unsigned gy, unsigned gz, unsigned block, void **args, const char *op) {
+    return launch3(K_COUNT + k, gx, gy, gz, block, 0, args, op);
 }
 
 static int launch2(int k, unsigned gx, unsigned gy, unsigned block, size_t lds, void **args, const char *op) {
@@ -954,8 +1003,8 @@ int sepia_hip_profile_stop(void) {
 }
 
 int sepia_hip_profile_query(const char *kernel, int64_t *launches, double *total_ms) {
-    for (int k = 0; k < K_COUNT; k++) {
-        if (!kernel || strcmp(kernel, k_names[k]) != 0) continue;
+    for (int k = 0; k < K_ALL; k++) {
+        if (!kernel || strcmp(kernel, k_name(k)) != 0) continue;
         if (launches) *launches = g_prof_cnt[k];
         if (total_ms) *total_ms = g_prof_ms[k];
         return 1;

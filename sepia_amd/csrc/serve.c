@@ -1,0 +1,256 @@
+/* serve.c -- the serving operators of include/sepia_hip_ext.h: the paged
+ * 8-bit key/value cache (kernels/kv8.h) and sampling (kernels/sample.h). Host
+ * checks and launches; what only the device knows (lengths, rows, the page
+ * table) the kernels check. */
+#include "internal.h"
+
+#include <string.h>
+
+#include "../../include/sepia_hip_ext.h"
+
+#define LOG(...) sepia_log(__VA_ARGS__)
+#define MAX_ROWS ((int64_t)1 << 24)     /* rows of a call: grids of fewer than 2^32 threads */
+#define MAX_SAMPLES ((int64_t)1 << 20)
+
+/* struct Kv8Args of kernels/kv8.h */
+typedef struct {
+    uint8_t *codes;
+    float *scales;
+    const int32_t *table, *lens, *starts;
+    int64_t n_pages;
+    int32_t n_seqs, max_pages, Hkv, Dh, lg, n;
+} Kv8Args;
+
+/* Checks a cache and a call's rows, and fills the kernels' arguments; `write`:
+ * the call writes to the pages. */
+static int kv8_args(const char *op, const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n,
+                    int write, Kv8Args *a) {
+    if (!c || c->n_pages < 1 || c->max_pages < 1 || c->n_seqs < 1 || c->n_seqs > 65536 || c->n_kv_heads < 1 ||
+        c->n_kv_heads > 65535 || n < 0 || n > MAX_ROWS || c->n_pages > 0x7FFFFFFF) {
+        LOG("%s: invalid arguments", op);
+        return 0;
+    }
+    if (c->page != 16 && c->page != 32 && c->page != 64) {
+        LOG("%s: pages of %d tokens not supported (16, 32 or 64)", op, c->page);
+        return 0;
+    }
+    if (c->head_dim < 16 || c->head_dim > 128 || c->head_dim % 16) {
+        LOG("%s: head dim %d not supported (a multiple of 16 up to 128)", op, c->head_dim);
+        return 0;
+    }
+    if (c->max_pages > 0x7FFFFFFF / c->page) {
+        LOG("%s: %lld pages of %d tokens a sequence pass 2^31 - 1 positions", op, (long long)c->max_pages, c->page);
+        return 0;
+    }
+    if (c->codes_off % 16 || c->scales_off % 4 || c->table_off % 4) {
+        LOG("%s: the cache's offsets are not multiples of 16 (codes) and 4 bytes", op);
+        return 0;
+    }
+    const size_t page = 2 * (size_t)c->n_kv_heads * (size_t)c->page * (size_t)c->head_dim;
+    if ((size_t)c->n_pages > SIZE_MAX / page) {
+        LOG("%s: invalid arguments", op);
+        return 0;
+    }
+    const size_t cb = (size_t)c->n_pages * page, sb = (size_t)c->n_pages * 2 * (size_t)c->n_kv_heads * 4;
+    const size_t tb = (size_t)c->n_seqs * (size_t)c->max_pages * 4, lb = (size_t)c->n_seqs * 4;
+    if (!sepia_chk(c->codes, c->codes_off, cb, op, "codes") || !sepia_chk(c->scales, c->scales_off, sb, op, "scales") ||
+        !sepia_chk(c->table, c->table_off, tb, op, "table") || !sepia_chk(lens, 0, lb, op, "lens") ||
+        !sepia_chk(starts, 0, lb + 4, op, "starts"))
+        return 0;
+    if (!sepia_need_batch(op) || !sepia_prep_in(c->table, c->table_off, tb, op) || !sepia_prep_in(lens, 0, lb, op) ||
+        !sepia_prep_in(starts, 0, lb + 4, op))
+        return 0;
+    if (write ? !sepia_prep_out(c->codes, op) || !sepia_prep_out(c->scales, op)
+              : !sepia_prep_in(c->codes, c->codes_off, cb, op) || !sepia_prep_in(c->scales, c->scales_off, sb, op))
+        return 0;
+    memset(a, 0, sizeof *a);
+    a->codes = sepia_buf_dev(c->codes) + c->codes_off;
+    a->scales = (float *)(sepia_buf_dev(c->scales) + c->scales_off);
+    a->table = (const int32_t *)(sepia_buf_dev(c->table) + c->table_off);
+    a->lens = (const int32_t *)sepia_buf_dev(lens);
+    a->starts = (const int32_t *)sepia_buf_dev(starts);
+    a->n_pages = c->n_pages;
+    a->n_seqs = c->n_seqs;
+    a->max_pages = (int32_t)c->max_pages;
+    a->Hkv = c->n_kv_heads;
+    a->Dh = c->head_dim;
+    a->lg = c->page == 16 ? 4 : c->page == 32 ? 5 : 6;
+    a->n = (int32_t)n;
+    return 1;
+}
+
+/* `out` is written while the inputs are read: it may be none of the cache's
+ * buffers, nor one of the call's tables. */
+static int kv8_apart(const char *op, const SepiaKv8Cache *c, const SepiaGpuBuf *lens, const SepiaGpuBuf *starts,
+                     const SepiaGpuBuf *out, const char *what) {
+    if (out != c->codes && out != c->scales && out != c->table && out != lens && out != starts) return 1;
+    LOG("%s: %s is also an input", op, what);
+    return 0;
+}
+
+/* Units of pages (kv8_map.h: a sequence of r rows touches at most r / page +
+ * 2), kv heads, K and V; a wave for each 16 tokens of a page. */
+static int kv8_pages(int k, const SepiaKv8Cache *c, int64_t n, void **args, const char *op) {
+    return sepia_serve_launch(k, (unsigned)(n / c->page + 2 * (int64_t)c->n_seqs), (unsigned)c->n_kv_heads, 2,
+                              (unsigned)c->page * 4, args, op);
+}
+
+int sepia_hip_kv8_append(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n, SepiaGpuBuf *k,
+                         SepiaGpuBuf *v, SepiaGpuBuf *k_norm, float eps) {
+    const char *op = "kv8_append";
+    Kv8Args a;
+    if (!c || !lens || !starts || !k || !v) {
+        LOG("%s: invalid arguments", op);
+        return 0;
+    }
+    const size_t rows = n < 0 || n > MAX_ROWS ? 0 : (size_t)n * (size_t)c->n_kv_heads * (size_t)c->head_dim * 4;
+    const size_t nb = (size_t)c->head_dim * 4;
+    if (k_norm && !(eps >= 0.0f)) {
+        LOG("%s: eps is negative or NaN", op);
+        return 0;
+    }
+    if (c->n_kv_heads < 1 || c->head_dim < 1 || !sepia_chk(k, 0, rows, op, "k") || !sepia_chk(v, 0, rows, op, "v") ||
+        (k_norm && !sepia_chk(k_norm, 0, nb, op, "k_norm"))) {
+        if (c->n_kv_heads < 1 || c->head_dim < 1) LOG("%s: invalid arguments", op);
+        return 0;
+    }
+    if (!kv8_apart(op, c, lens, starts, k, "k") || !kv8_apart(op, c, lens, starts, v, "v") ||
+        (k_norm && !kv8_apart(op, c, lens, starts, k_norm, "k_norm")))
+        return 0;
+    if (!kv8_args(op, c, lens, starts, n, 1, &a) || !sepia_prep_in(k, 0, rows, op) || !sepia_prep_in(v, 0, rows, op) ||
+        (k_norm && !sepia_prep_in(k_norm, 0, nb, op)))
+        return 0;
+    if (n == 0) return 1;
+    const float *kp = (const float *)sepia_buf_dev(k), *vp = (const float *)sepia_buf_dev(v);
+    const float *np = (const float *)sepia_buf_dev(k_norm);
+    void *args[] = { &a, &kp, &vp, &np, &eps };
+    return kv8_pages(SK_KV8_APPEND, c, n, args, op);
+}
+
+int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *starts, int64_t n, SepiaGpuBuf *k,
+                       SepiaGpuBuf *v) {
+    const char *op = "kv8_read";
+    Kv8Args a;
+    if (!c || !first || !starts || !k || !v || k == v || c->n_kv_heads < 1 || c->head_dim < 1) {
+        LOG("%s: invalid arguments", op);
+        return 0;
+    }
+    const size_t rows = n < 0 || n > MAX_ROWS ? 0 : (size_t)n * (size_t)c->n_kv_heads * (size_t)c->head_dim * 4;
+    if (!sepia_chk(k, 0, rows, op, "k") || !sepia_chk(v, 0, rows, op, "v") ||
+        !kv8_apart(op, c, first, starts, k, "k") || !kv8_apart(op, c, first, starts, v, "v"))
+        return 0;
+    if (!kv8_args(op, c, first, starts, n, 0, &a) || !sepia_prep_out(k, op) || !sepia_prep_out(v, op)) return 0;
+    if (n == 0) return 1;
+    float *kp = (float *)sepia_buf_dev(k), *vp = (float *)sepia_buf_dev(v);
+    void *args[] = { &a, &kp, &vp };
+    return kv8_pages(SK_KV8_READ, c, n, args, op);
+}
+
+/* struct Kv8Attn of kernels/kv8.h */
+typedef struct {
+    const float *q, *rel, *tau;
+    float *out;
+    int32_t H, R, window;
+    float c;
+} Kv8Attn;
+
+int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n, SepiaGpuBuf *q,
+                       SepiaGpuBuf *rel_logits, SepiaGpuBuf *tau, SepiaGpuBuf *out, int64_t n_heads,
+                       int64_t rel_extent, int64_t window, float inv_head_dim) {
+    const char *op = "kv8_attn";
+    Kv8Args a;
+    Kv8Attn b;
+    if (!c || !lens || !starts || !q || !out || c->n_kv_heads < 1 || c->head_dim < 1 || n_heads < 1 ||
+        n_heads > 65535 || n_heads % c->n_kv_heads || n_heads / c->n_kv_heads > 16 || window < 0 ||
+        rel_extent < 0 || rel_extent > 0x7FFFFFFF || (rel_extent > 0) != (rel_logits != NULL) ||
+        (rel_extent > 0 && n > 0 && n > INT64_MAX / 4 / n_heads / rel_extent)) {
+        LOG("%s: invalid arguments", op);
+        return 0;
+    }
+    const size_t rows = n < 0 || n > MAX_ROWS ? 0 : (size_t)n;
+    const size_t qb = rows * (size_t)n_heads * (size_t)c->head_dim * 4, rb = rows * (size_t)n_heads * (size_t)rel_extent * 4;
+    if (!sepia_chk(q, 0, qb, op, "q") || !sepia_chk(out, 0, qb, op, "out") ||
+        (rel_logits && !sepia_chk(rel_logits, 0, rb, op, "rel_logits")) || (tau && !sepia_chk(tau, 0, rows * 4, op, "tau")) ||
+        !kv8_apart(op, c, lens, starts, out, "out"))
+        return 0;
+    if (out == rel_logits || out == tau) {
+        LOG("%s: out is also an input", op);
+        return 0;
+    }
+    if (!kv8_args(op, c, lens, starts, n, 0, &a) || !sepia_prep_in(q, 0, qb, op) ||
+        (rel_logits && !sepia_prep_in(rel_logits, 0, rb, op)) || (tau && !sepia_prep_in(tau, 0, rows * 4, op)) ||
+        !sepia_prep_out(out, op))
+        return 0;
+    if (n == 0) return 1;
+    memset(&b, 0, sizeof b);
+    b.q = (const float *)sepia_buf_dev(q);
+    b.rel = (const float *)sepia_buf_dev(rel_logits);
+    b.tau = (const float *)sepia_buf_dev(tau);
+    b.out = (float *)sepia_buf_dev(out);
+    b.H = (int32_t)n_heads;
+    b.R = (int32_t)rel_extent;
+    b.window = window > 0x7FFFFFFF ? 0 : (int32_t)window;
+    b.c = inv_head_dim;
+    void *args[] = { &a, &b };
+    return sepia_serve_launch(SK_KV8_ATTN, (unsigned)n, (unsigned)n_heads, 1, 64, args, op);
+}
+
+/* struct SampleArgs of kernels/sample.h */
+typedef struct {
+    const float *logits, *u, *temperature, *top_p, *min_p;
+    const int32_t *top_k;
+    int32_t *token;
+    float *prob;
+    int64_t stride;
+    int32_t vocab;
+} SampleArgs;
+
+int sepia_hip_sample(const SepiaSampleDesc *d, SepiaGpuBuf *logits, int64_t rows, int64_t vocab, int64_t stride,
+                     SepiaGpuBuf *tokens, SepiaGpuBuf *prob) {
+    const char *op = "sample";
+    if (!d || !d->u || !logits || !tokens || rows < 0 || rows > MAX_SAMPLES || vocab < 1 || stride < vocab ||
+        (rows > 0 && stride > INT64_MAX / 4 / rows)) {
+        LOG("%s: invalid arguments", op);
+        return 0;
+    }
+    if (vocab > (1 << 20)) {
+        LOG("%s: %lld logits a row not supported (up to 2^20)", op, (long long)vocab);
+        return 0;
+    }
+    const size_t lb = rows ? ((size_t)(rows - 1) * (size_t)stride + (size_t)vocab) * 4 : 0, rb = (size_t)rows * 4;
+    SepiaGpuBuf *const in[] = { d->u, d->temperature, d->top_p, d->min_p, d->top_k };
+    static const char *const names[] = { "u", "temperature", "top_p", "min_p", "top_k" };
+    if (!sepia_chk(logits, 0, lb, op, "logits") || !sepia_chk(tokens, 0, rb, op, "tokens") ||
+        (prob && !sepia_chk(prob, 0, rb, op, "prob")))
+        return 0;
+    for (int i = 0; i < 5; i++) {
+        if (in[i] && !sepia_chk(in[i], 0, rb, op, names[i])) return 0;
+        if (in[i] && (in[i] == tokens || in[i] == prob)) {
+            LOG("%s: %s is also an output", op, names[i]);
+            return 0;
+        }
+    }
+    if (tokens == prob || logits == tokens || logits == prob) {
+        LOG("%s: logits, tokens and prob are not three buffers", op);
+        return 0;
+    }
+    if (!sepia_need_batch(op) || !sepia_prep_in(logits, 0, lb, op)) return 0;
+    for (int i = 0; i < 5; i++)
+        if (in[i] && !sepia_prep_in(in[i], 0, rb, op)) return 0;
+    if (!sepia_prep_out(tokens, op) || (prob && !sepia_prep_out(prob, op))) return 0;
+    if (rows == 0) return 1;
+    SampleArgs a;
+    memset(&a, 0, sizeof a);
+    a.logits = (const float *)sepia_buf_dev(logits);
+    a.u = (const float *)sepia_buf_dev(d->u);
+    a.temperature = (const float *)sepia_buf_dev(d->temperature);
+    a.top_p = (const float *)sepia_buf_dev(d->top_p);
+    a.min_p = (const float *)sepia_buf_dev(d->min_p);
+    a.top_k = (const int32_t *)sepia_buf_dev(d->top_k);
+    a.token = (int32_t *)sepia_buf_dev(tokens);
+    a.prob = (float *)sepia_buf_dev(prob);
+    a.stride = stride;
+    a.vocab = (int32_t)vocab;
+    void *args[] = { &a };
+    return sepia_serve_launch(SK_SAMPLE, (unsigned)rows, 1, 1, 1024, args, op);
+}

@@ -16,6 +16,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libsepia_hip.so")
 HSACO_PATH = os.path.join(LIB_DIR, "sepia_kernels.hsaco")
+SERVE_HSACO_PATH = os.path.join(LIB_DIR, "sepia_serve.hsaco")
 INCLUDE_DIR = os.path.join(os.path.dirname(PKG), "include")
 
 
@@ -46,6 +47,18 @@ class ResidentTensor(ctypes.Structure):
 class ExpertSlot(ctypes.Structure):
     _fields_ = [("part_idx", ctypes.c_int), ("abs_offset", ctypes.c_int64), ("nbytes", ctypes.c_int64),
                 ("ggml_type", ctypes.c_int)]
+
+
+class Kv8Cache(ctypes.Structure):
+    _fields_ = [("n_pages", ctypes.c_int64), ("max_pages", ctypes.c_int64), ("n_seqs", ctypes.c_int),
+                ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("page", ctypes.c_int),
+                ("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("codes_off", ctypes.c_size_t), ("scales_off", ctypes.c_size_t), ("table_off", ctypes.c_size_t)]
+
+
+class SampleDesc(ctypes.Structure):
+    _fields_ = [("u", ctypes.c_void_p), ("temperature", ctypes.c_void_p), ("top_p", ctypes.c_void_p),
+                ("min_p", ctypes.c_void_p), ("top_k", ctypes.c_void_p)]
 
 
 _P, _SZ, _I64, _F, _I = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int64, ctypes.c_float, ctypes.c_int
@@ -88,6 +101,11 @@ PROTOTYPES = {
     "sepia_hip_moe_decode_noalloc": (_I, [ctypes.POINTER(MoeLayerDesc), _P, _P, _P]),
     "sepia_gpu_expert_ffn": (_I, [ctypes.POINTER(ExpertTensor), ctypes.POINTER(ExpertTensor),
                                   ctypes.POINTER(ExpertTensor), _I, _I, _I64, _I64, _P, _P]),
+    # serving: the paged 8-bit key/value cache and sampling (serve.c)
+    "sepia_hip_kv8_append": (_I, [ctypes.POINTER(Kv8Cache), _P, _P, _I64, _P, _P, _P, _F]),
+    "sepia_hip_kv8_read": (_I, [ctypes.POINTER(Kv8Cache), _P, _P, _I64, _P, _P]),
+    "sepia_hip_kv8_attn": (_I, [ctypes.POINTER(Kv8Cache), _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _F]),
+    "sepia_hip_sample": (_I, [ctypes.POINTER(SampleDesc), _P, _I64, _I64, _I64, _P, _P]),
     "sepia_hip_profile_start": (_I, []),
     "sepia_hip_profile_stop": (_I, []),
     "sepia_hip_profile_query": (_I, [ctypes.c_char_p, ctypes.POINTER(_I64), ctypes.POINTER(ctypes.c_double)]),
@@ -129,8 +147,8 @@ def load():
     """Load libsepia_hip.so (raises if it was not built)."""
     global _lib
     if _lib is None:
-        if not os.path.exists(LIB_PATH) or not os.path.exists(HSACO_PATH):
-            raise SepiaHipError("libsepia_hip.so / sepia_kernels.hsaco not built under %s "
+        if not all(os.path.exists(p) for p in (LIB_PATH, HSACO_PATH, SERVE_HSACO_PATH)):
+            raise SepiaHipError("libsepia_hip.so / sepia_kernels.hsaco / sepia_serve.hsaco not built under %s "
                                 "(run __graft_entry__.build())" % LIB_DIR)
         L = ctypes.CDLL(LIB_PATH)
         for name, (res, args) in PROTOTYPES.items():
