@@ -36,12 +36,15 @@ SEPIA_HIDDEN int sepia_need_batch(const char *op);
 SEPIA_HIDDEN int sepia_chk(const SepiaGpuBuf *b, size_t off, size_t n, const char *op, const char *what);
 SEPIA_HIDDEN int sepia_prep_in(SepiaGpuBuf *b, size_t off, size_t n, const char *op);
 SEPIA_HIDDEN int sepia_prep_out(SepiaGpuBuf *b, const char *op);
-/* The scratch's data region of at least `need` bytes (NULL: logged). */
+/* The scratch's data region of at least `need` bytes (NULL: logged), and how
+ * many a call may ask for: what there is while the stream is being captured,
+ * else any number. */
 SEPIA_HIDDEN void *sepia_scratch(size_t need, const char *op);
+SEPIA_HIDDEN size_t sepia_scratch_limit(void);
 
 /* Kernels of the second code object (kernels/sepia_serve.hip), and a launch
  * of one on the library's stream, timed when the profiler is on. */
-enum { SK_KV8_APPEND, SK_KV8_READ, SK_KV8_ATTN, SK_SAMPLE, SK_COUNT };
+enum { SK_KV8_APPEND, SK_KV8_READ, SK_KV8_ATTN, SK_KV8_ATTN_D, SK_KV8_FOLD, SK_SAMPLE, SK_COUNT };
 SEPIA_HIDDEN int sepia_serve_launch(int k, unsigned gx, unsigned gy, unsigned gz, unsigned block, void **args,
                                     const char *op);
 

@@ -1,4 +1,5 @@
-// kv8.h -- a paged key/value cache held in 8 bits, and attention over it.
+// kv8.h -- a paged key/value cache held in 8 bits: its layout, appending to it
+// and reading it back (attention over it: kv8_attn.h).
 //
 // Page p of the pool holds P tokens (16, 32 or 64) of every kv head: K codes
 // int8 [head][token][dim], then V codes int8 [head][dim][token], and a scale
@@ -284,72 +285,4 @@ extern "C" __global__ __launch_bounds__(256) void sepia_kv8_read(Kv8Args a, floa
         *(float2 *)(out + (int64_t)(u.row + slot - u.s0) * ld + d) = make_float2(
             (float)(int8_t)(we[i / 4] >> (8 * (i % 4))) * sc, (float)(int8_t)(wf[i / 4] >> (8 * (i % 4))) * sc);
     }
-}
-
-// ----------------------------------------------------------- attention -----
-// Row t of sequence s at position pos sees the columns [max(0, pos - window +
-// 1), pos]: score (q . k) c + [pos - col < R] rel[t][h][pos - col] tau[t],
-// softmax, weighted v. One wave a (row, head): a lane a column of 64 for the
-// scores, two dims of the head for the weighted v.
-struct Kv8Attn {
-    const float *q, *rel, *tau;
-    float *out;
-    int32_t H, R, window;
-    float c;
-};
-extern "C" __global__ __launch_bounds__(64) void sepia_kv8_attn(Kv8Args a, Kv8Attn b) {
-    __shared__ float qs[128], ps[64];
-    const int lane = (int)threadIdx.x, t = (int)blockIdx.x, h = (int)blockIdx.y, hk = h / (b.H / a.Hkv);
-    kv8_check(a);
-    const int s = kv8_find(a, t, 1, 0);
-    int32_t len, r0, r1;
-    if (s < 0 || !kv8_seq(a, s, len, r0, r1) || t >= r1) return;
-    const int pos = len + (t - r0), lo = b.window > 0 && pos >= b.window ? pos - b.window + 1 : 0;
-    const float *q = b.q + ((int64_t)t * b.H + h) * a.Dh;
-    for (int d = lane; d < a.Dh; d += 64) qs[d] = q[d];
-    __syncthreads();
-    const float tau = b.tau ? b.tau[t] : 1.0f;
-    float m = -INFINITY, l = 0.0f, acc0 = 0.0f, acc1 = 0.0f;
-    for (int c0 = lo & ~63; c0 <= pos; c0 += 64) {
-        const int col = c0 + lane;
-        const bool in = col >= lo && col <= pos;
-        const int64_t page = kv8_page(a, s, (in ? col : pos) >> a.lg);
-        if (__ballot(page < 0)) {
-            sepia_report_error(nullptr, KV8_ERR_PAGE, lane);
-            return;
-        }
-        float sc = -INFINITY, vs = 0.0f;
-        if (in) {
-            const int8_t *kc = a.k_codes(page, hk) + (col & (a.P() - 1)) * a.Dh;
-            float dot = 0.0f;
-            for (int d = 0; d < a.Dh; d++) dot = __builtin_fmaf(qs[d], (float)kc[d], dot);
-            sc = dot * (*a.scale(page, 0, hk) * b.c);
-            if (b.rel && pos - col < b.R) sc += b.rel[((int64_t)t * b.H + h) * b.R + (pos - col)] * tau;
-            vs = *a.scale(page, 1, hk);
-        }
-        float mn = sc;
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) mn = fmaxf(mn, __shfl_xor(mn, o, 64));
-        mn = fmaxf(m, mn);
-        const float ref = mn == -INFINITY ? 0.0f : mn;
-        const float al = m == mn ? 1.0f : expf(m - ref), p = in ? expf(sc - ref) : 0.0f;
-        m = mn;
-        l = l * al + wave_sum(p);
-        acc0 *= al;
-        acc1 *= al;
-        ps[lane] = in ? p * vs : 0.0f;
-        __syncthreads();
-        for (int i = 0; i < 64; i++) {
-            const int ci = c0 + i;
-            if (ci < lo || ci > pos || 2 * lane >= a.Dh) continue;
-            const int8_t *vc = a.v_codes(kv8_page(a, s, ci >> a.lg), hk) + (ci & (a.P() - 1));
-            acc0 = __builtin_fmaf(ps[i], (float)vc[(int64_t)(2 * lane) << a.lg], acc0);
-            acc1 = __builtin_fmaf(ps[i], (float)vc[(int64_t)(2 * lane + 1) << a.lg], acc1);
-        }
-        __syncthreads();
-    }
-    if (2 * lane >= a.Dh) return;
-    float *o = b.out + ((int64_t)t * b.H + h) * a.Dh + 2 * lane;
-    o[0] = acc0 / l;
-    o[1] = acc1 / l;
 }

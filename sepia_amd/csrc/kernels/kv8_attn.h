@@ -1,0 +1,416 @@
+// kv8_attn.h -- attention over the paged 8-bit cache (kv8.h) on the int8
+// matrix cores.
+//
+// Row t of sequence s at position pos sees the columns [max(0, pos - window +
+// 1), pos]: score (q . k) c + [pos - col < R] rel[t][h][pos - col] tau[t],
+// softmax, weighted v. The codes are operands as they lie in the cache; what
+// meets them is split into three signed base-256 digits, 24 bits in all, whose
+// products with codes are exact integers:
+//   q    relative to the row's largest |q|;
+//   p v  each weight times its page's V scale, relative to the largest power
+//        of two below the row's largest such product among the step's 64
+//        columns (products below 2^-100 are multiples of 2^-122).
+// A wave owns 16 rows, each a (token, query head) pair of one kv head, and
+// walks the columns in steps of 64:
+//   S^T = K q^T   v_mfma_i32_16x16x64_i8, four tiles of 16 columns; row 4 g + i
+//         of tile t is column 16 g + 4 t + i of the step, so that lane (n, g)
+//         = (lane & 15, lane >> 4) gets columns 16 g .. + 15 of row n: the
+//         scales of one page, one run of rel_logits, and the row's softmax
+//         in two exchanges between lane groups;
+//   O^T = V^T P^T with k = column in the same order, so that the weights'
+//         digits are an operand where they are made (no LDS, no exchange) and
+//         a dim's 16 columns of a page, side by side in V's layout, the other.
+// O stays in registers, f32, per row n: dims 16 ct + 4 g + i.
+#pragma once
+#include "kv8.h"
+
+#define KV8_NW 4             // waves of a workgroup: they take a unit's steps in turn
+#define KV8_C 8355711.0f     // 0x7F7F7F: the largest magnitude of three digits
+#define KV8_CP 4177855.0f    // half of it: a weight's place relative to a power of two
+#define KV8_L2E 1.44269504f
+
+struct Kv8Attn {
+    const float *q, *rel, *tau;
+    float *out;
+    float *part, *ml;        // per split: O [16][Dh]; maxima [16], sums [16]
+    int32_t H, R, window, TT, budget;   // TT: tokens of a row tile
+    float c;
+};
+
+typedef int32_t kv8_i4 __attribute__((ext_vector_type(4)));
+typedef float kv8_f4 __attribute__((ext_vector_type(4)));
+
+// Over the four lane groups (lanes n, n + 16, n + 32, n + 48).
+__device__ __forceinline__ float kv8_max_g(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float kv8_sum_g(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+// How a call's work is cut: sequence s has rt row tiles of TT tokens and at
+// most `steps` steps of 64 columns in each; a unit (row tile, kv head) is cut
+// into `splits` runs of about `chunk` steps, so that the runs of all units are
+// about `budget`. Every workgroup works this out for itself from the lengths.
+struct Kv8Plan {
+    int s, k, hk, x, splits, slot, len, r0, r1;   // slot: of split 0 of the unit (splits > 1); + Hkv a split
+};
+__device__ __forceinline__ void kv8_cost(const Kv8Args &a, const Kv8Attn &b, int s, int &rt, int &steps) {
+    rt = steps = 0;
+    int32_t len, r0, r1;
+    if (s >= a.n_seqs || !kv8_seq(a, s, len, r0, r1) || r1 == r0) return;
+    const int end = len + (r1 - r0);
+    rt = (r1 - r0 + b.TT - 1) / b.TT;
+    steps = (end + 63) / 64;
+    if (b.window > 0) steps = min(steps, (int)(((int64_t)b.window + b.TT + 61) / 64) + 1);
+}
+// The id-th run (combine: the id-th unit that is cut) in the order sequence,
+// row tile, split, kv head; 0 past the last.
+template <bool COMBINE>
+__device__ __forceinline__ int kv8_plan(const Kv8Args &a, const Kv8Attn &b, int id, Kv8Plan &p) {
+    const int lane = (int)(threadIdx.x & 63);
+    float total = 0.0f;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+        int rt, steps;
+        kv8_cost(a, b, s0 + lane, rt, steps);
+        total += wave_sum((float)rt * (float)steps);
+    }
+    const int chunk = b.budget > 0 ? max(KV8_NW, (int)ceilf(fminf(total * (float)a.Hkv / (float)b.budget, 1e9f))) : 0x7FFFFFFF;
+    p.hk = id % a.Hkv;
+    const int at = id / a.Hkv;
+    int base = 0, slots = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+        int rt, steps;
+        kv8_cost(a, b, s0 + lane, rt, steps);
+        const int splits = (int)(((int64_t)steps + chunk - 1) / chunk);
+        const int mine = COMBINE ? (splits > 1 ? rt : 0) : rt * splits;
+        const int cut = splits > 1 ? rt * splits : 0;
+        int sum = mine, csum = cut;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(sum, o, 64), v = __shfl_up(csum, o, 64);
+            if (lane >= o) sum += u, csum += v;
+        }
+        const uint64_t hit = __ballot(at >= base + sum - mine && at < base + sum);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            p.s = s0 + l;
+            p.splits = __builtin_amdgcn_readlane(splits, l);
+            const int i = at - base - __builtin_amdgcn_readlane(sum - mine, l);
+            p.k = COMBINE ? i : i / p.splits;
+            p.x = COMBINE ? 0 : i - p.k * p.splits;
+            p.slot = (slots + __builtin_amdgcn_readlane(csum - cut, l) + p.k * p.splits) * a.Hkv + p.hk;
+            kv8_seq(a, p.s, p.len, p.r0, p.r1);
+            return 1;
+        }
+        base += __builtin_amdgcn_readlane(sum, 63);
+        slots += __builtin_amdgcn_readlane(csum, 63);
+    }
+    return 0;
+}
+
+// A row tile's tokens and its steps of 64 columns.
+struct Kv8Tile {
+    int t0, nt, pos0, lo, last, step0, steps;   // lo, last: the first and last column any row sees
+};
+__device__ __forceinline__ Kv8Tile kv8_tile(const Kv8Attn &b, const Kv8Plan &p) {
+    Kv8Tile t;
+    t.t0 = p.r0 + p.k * b.TT;
+    t.nt = min(b.TT, p.r1 - t.t0);
+    t.pos0 = p.len + p.k * b.TT;
+    t.last = t.pos0 + t.nt - 1;
+    t.lo = b.window > 0 ? max(0, t.pos0 - b.window + 1) : 0;
+    t.step0 = t.lo >> 6;
+    t.steps = (t.last >> 6) - t.step0 + 1;
+    return t;
+}
+
+// Three digit planes of four 24-bit places in the three low bytes of u0..u3
+// (the lower two digits offset by 128): planes 0 (low) to 2.
+__device__ __forceinline__ void kv8_planes(const uint32_t *u, int32_t &p0, int32_t &p1, int32_t &p2) {
+    const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x05010400), b = __builtin_amdgcn_perm(u[3], u[2], 0x05010400);
+    const uint32_t c = __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0602), d = __builtin_amdgcn_perm(u[3], u[2], 0x06020C0C);
+    p0 = (int32_t)(__builtin_amdgcn_perm(b, a, 0x05040100) ^ 0x80808080u);
+    p1 = (int32_t)(__builtin_amdgcn_perm(b, a, 0x07060302) ^ 0x80808080u);
+    p2 = (int32_t)(c | d);
+}
+// hi 65536 + mid 256 + lo of exact sums (|sum| <= 2^20): mid 256 + lo is exact.
+__device__ __forceinline__ float kv8_join(int32_t hi, int32_t mid, int32_t lo) {
+    return __builtin_fmaf((float)hi, 65536.0f, (float)(int32_t)(((uint32_t)mid << 8) + (uint32_t)lo));
+}
+
+// One wave's 16 rows. NK: K operands a row (64 dims each), NC: tiles of 16
+// dims; both cover Dh (FULL: Dh is 128).
+template <bool FULL>
+struct Kv8Wave {
+    kv8_i4 qd[3][2];        // q's digits: lane (n, g) dims 64 ks + 16 g .. + 15 of row n
+    kv8_f4 O[8];
+    float m, l, qs, tau;    // row n's maximum; this lane's part of its sum; q's scale times c
+    int32_t lo, pos;        // row n's columns (inactive: none)
+    const float *rel;       // row n's rel_logits at distance pos, so that column col's is rel[-col]
+    int32_t lo_max, pos_min;   // over the active rows
+
+    __device__ __forceinline__ void init(const Kv8Args &a, const Kv8Attn &b, const Kv8Tile &t, int row0, int hk) {
+        const int lane = (int)(threadIdx.x & 63), n = lane & 15, g = lane >> 4, G = b.H / a.Hkv;
+        const int ti = (row0 + n) / G, h = hk * G + (row0 + n - ti * G);
+        const bool on = ti < t.nt;
+        const int64_t th = (int64_t)(t.t0 + (on ? ti : 0)) * b.H + (on ? h : hk * G);
+        const float *q = b.q + th * a.Dh;
+        float v[2][16], most = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+            const int d = 64 * ks + 16 * g;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                kv8_f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (on && (FULL || d < a.Dh)) x = *(const kv8_f4 *)(q + d + 4 * i);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    v[ks][4 * i + e] = x[e];
+                    most = fmaxf(most, fabsf(x[e]));
+                    bad |= !(fabsf(x[e]) < INFINITY);
+                }
+            }
+        }
+        most = kv8_max_g(bad ? INFINITY : most);
+        const float inv = most > 0.0f && most < INFINITY ? KV8_C / most : 0.0f;
+        qs = most < INFINITY ? most * (b.c / KV8_C) : NAN;
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t u[4];
+                int32_t p0, p1, p2;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    u[e] = (uint32_t)(int32_t)__builtin_rintf(fmaxf(-KV8_C, fminf(KV8_C, v[ks][4 * i + e] * inv))) + 0x8080u;
+                kv8_planes(u, p0, p1, p2);
+                qd[0][ks][i] = p0;
+                qd[1][ks][i] = p1;
+                qd[2][ks][i] = p2;
+            }
+        pos = on ? t.pos0 + ti : -1;
+        lo = on ? (b.window > 0 ? max(0, pos - b.window + 1) : 0) : 0x7FFFFFFF;
+        tau = b.tau ? b.tau[t.t0 + (on ? ti : 0)] : 1.0f;
+        rel = b.rel ? b.rel + th * b.R + (on ? pos : t.pos0) : nullptr;
+        lo_max = b.window > 0 ? max(0, t.last - b.window + 1) : 0;
+        pos_min = t.pos0;
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) O[i] = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // The pages of a step: of this lane's K row and of its columns 16 g .. .
+    // Columns outside [lo, last] of the tile take the nearest page inside.
+    static __device__ __forceinline__ void pages(const Kv8Args &a, const Kv8Plan &p, const Kv8Tile &t, int step, int64_t &pk,
+                                                 int64_t &pv) {
+        const int lane = (int)(threadIdx.x & 63), first = t.lo >> a.lg, end = t.last >> a.lg;
+        const int ik = (64 * step + 16 * ((lane & 15) >> 2)) >> a.lg, iv = (64 * step + 16 * (lane >> 4)) >> a.lg;
+        pk = kv8_page(a, p.s, max(first, min(end, ik)));
+        pv = kv8_page(a, p.s, max(first, min(end, iv)));
+        if (__ballot(pk < 0 || pv < 0)) sepia_report_error(nullptr, KV8_ERR_PAGE, lane);
+        pk = max(pk, (int64_t)0);
+        pv = max(pv, (int64_t)0);
+    }
+    // K operand [t][ks]: column 16 (n >> 2) + 4 t + (n & 3), dims 64 ks + 16 g.
+    static __device__ __forceinline__ void load_k(const Kv8Args &a, int64_t page, int hk, int step, kv8_i4 (&K)[4][2]) {
+        const int lane = (int)(threadIdx.x & 63), n = lane & 15, g = lane >> 4;
+        const int slot = (64 * step + 16 * (n >> 2) + (n & 3)) & (a.P() - 1);
+        const int8_t *k = a.k_codes(page, hk) + slot * a.Dh + (FULL || 16 * g < a.Dh ? 16 * g : 0);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            K[t][0] = *(const kv8_i4 *)(k + 4 * t * a.Dh);
+            K[t][1] = *(const kv8_i4 *)(k + 4 * t * a.Dh + (FULL || 64 + 16 * g < a.Dh ? 64 : 0));
+        }
+    }
+    // V operand [ct]: dim 16 ct + n, columns 16 g .. + 15.
+    static __device__ __forceinline__ void load_v(const Kv8Args &a, int64_t page, int hk, int step, kv8_i4 (&V)[8]) {
+        const int lane = (int)(threadIdx.x & 63), n = lane & 15, g = lane >> 4;
+        const int8_t *v = a.v_codes(page, hk) + ((int64_t)n << a.lg) + ((64 * step + 16 * g) & (a.P() - 1));
+#pragma unroll
+        for (int ct = 0; ct < 8; ct++) V[ct] = *(const kv8_i4 *)(v + ((int64_t)(FULL || 16 * ct < a.Dh ? 16 * ct : 0) << a.lg));
+    }
+    // Scores' digit sums of a step.
+    __device__ __forceinline__ void dots(const kv8_i4 (&K)[4][2], float (&s)[16]) const {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            kv8_i4 d[3];
+#pragma unroll
+            for (int p = 0; p < 3; p++) {
+                d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(K[t][0], qd[p][0], kv8_i4{0, 0, 0, 0}, 0, 0, 0);
+                d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(K[t][1], qd[p][1], d[p], 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[4 * t + i] = kv8_join(d[2][i], d[1][i], d[0][i]);
+        }
+    }
+    // The step's softmax and weighted v; ks, vs: the scales of the page of
+    // columns 16 g .. .
+    __device__ __forceinline__ void step(const Kv8Args &a, const Kv8Attn &b, int step, float (&s)[16], float ks, float vs,
+                                         const kv8_i4 (&V)[8]) {
+        const int g = (int)(threadIdx.x & 63) >> 4, c0 = 64 * step + 16 * g;
+        const float sc = qs * ks;
+#pragma unroll
+        for (int j = 0; j < 16; j++) s[j] *= sc;
+        if (b.rel && pos_min - (64 * step + 63) < b.R) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const int d = pos - c0 - j;
+                if (d >= 0 && d < b.R) s[j] = __builtin_fmaf(rel[-(int64_t)(c0 + j)], tau, s[j]);
+            }
+        }
+        bool any = true;
+        if (64 * step < lo_max || 64 * step + 63 > pos_min) {
+            any = c0 <= pos && c0 + 15 >= lo;
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[j] = c0 + j >= lo && c0 + j <= pos ? s[j] : -INFINITY;
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int j = 1; j < 16; j++) mx = fmaxf(mx, s[j]);
+        const float mn = fmaxf(m, kv8_max_g(mx));
+        const float ref = mn == -INFINITY ? 0.0f : mn;
+        if (__ballot(mn != m)) {
+            const float al = __builtin_amdgcn_exp2f((m - ref) * KV8_L2E);   // 1 where the maximum stays
+            l *= al;
+#pragma unroll
+            for (int ct = 0; ct < 8; ct++) O[ct] *= al;
+            m = mn;
+        }
+        vs = any ? vs : 0.0f;
+        // the row's largest product, as the power of two below it
+        const float wm = kv8_max_g(__builtin_amdgcn_exp2f((mx - ref) * KV8_L2E) * vs);
+        const uint32_t e = max(__builtin_bit_cast(uint32_t, wm) & 0x7F800000u, 27u << 23);
+        const float place = fminf(vs * (KV8_CP * __builtin_bit_cast(float, (254u << 23) - e)), 3e38f);
+        const float back = __builtin_bit_cast(float, e) * (1.0f / KV8_CP);
+        kv8_i4 pd[3];
+        float sum = vs * 0.0f;   // a NaN or infinite scale of V makes the row NaN
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t u[4];
+            int32_t p0, p1, p2;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float p = __builtin_amdgcn_exp2f((s[4 * i + j] - ref) * KV8_L2E);
+                sum += p;
+                // 2^23 + 0x8080 + the place: its low bytes are the digits
+                u[j] = __builtin_bit_cast(uint32_t, __builtin_fmaf(p, place, 8421504.0f));
+            }
+            kv8_planes(u, p0, p1, p2);
+            pd[0][i] = p0;
+            pd[1][i] = p1;
+            pd[2][i] = p2;
+        }
+        l += sum;
+#pragma unroll
+        for (int ct = 0; ct < 8; ct++) {
+            if (!FULL && 16 * ct >= a.Dh) break;
+            kv8_i4 d[3];
+#pragma unroll
+            for (int p = 0; p < 3; p++) d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(V[ct], pd[p], kv8_i4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) O[ct][i] = __builtin_fmaf(kv8_join(d[2][i], d[1][i], d[0][i]), back, O[ct][i]);
+        }
+    }
+    // Steps s0, s0 + stride, .. below s1 (of the tile's steps).
+    __device__ __forceinline__ void walk(const Kv8Args &a, const Kv8Attn &b, const Kv8Plan &p, const Kv8Tile &t, int s0, int s1,
+                                         int stride) {
+        if (s0 >= s1) return;
+        kv8_i4 K[4][2], V[8];
+        int64_t pk, pv, nk, nv;
+        pages(a, p, t, t.step0 + s0, pk, pv);
+        load_k(a, pk, p.hk, t.step0 + s0, K);
+        for (int i = s0; i < s1; i += stride) {
+            const int step_i = t.step0 + i;
+            const float ks = *a.scale(pv, 0, p.hk), vs = *a.scale(pv, 1, p.hk);
+            load_v(a, pv, p.hk, step_i, V);
+            const bool more = i + stride < s1;
+            if (more) pages(a, p, t, step_i + stride, nk, nv);
+            float s[16];
+            dots(K, s);
+            if (more) load_k(a, nk, p.hk, step_i + stride, K);
+            step(a, b, step_i, s, ks, vs, V);
+            pv = nv;
+        }
+    }
+};
+
+// Grid: the plan's runs, KV8_NW waves each.
+template <bool FULL>
+__device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b) {
+    __shared__ kv8_f4 so[KV8_NW][8][64];
+    __shared__ float sm[KV8_NW][16], sl[KV8_NW][16];
+    kv8_check(a);
+    Kv8Plan p;
+    if (!kv8_plan<false>(a, b, (int)blockIdx.x, p)) return;
+    const Kv8Tile t = kv8_tile(b, p);
+    const int span = (t.steps + p.splits - 1) / p.splits, s0 = p.x * span, s1 = min(t.steps, s0 + span);
+    const int w = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4, G = b.H / a.Hkv;
+    Kv8Wave<FULL> W;
+    W.init(a, b, t, 0, p.hk);
+    W.walk(a, b, p, t, s0 + w, s1, KV8_NW);
+    const float l = kv8_sum_g(W.l);
+    if (g == 0) {
+        sm[w][n] = W.m;
+        sl[w][n] = l;
+    }
+#pragma unroll
+    for (int ct = 0; ct < 8; ct++) so[w][ct][lane] = W.O[ct];
+    __syncthreads();
+    // fold the waves: wave w takes dims 16 ct .. of ct = w, w + NW
+    float M = -INFINITY, f[KV8_NW], L = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KV8_NW; i++) M = fmaxf(M, sm[i][n]);
+    const float ref = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (int i = 0; i < KV8_NW; i++) {
+        f[i] = __builtin_amdgcn_exp2f((sm[i][n] - ref) * KV8_L2E);
+        L += sl[i][n] * f[i];
+    }
+    const int ti = n / G;
+    if (ti >= t.nt) return;
+    const int64_t th = (int64_t)(t.t0 + ti) * b.H + p.hk * G + (n - ti * G);
+    const int64_t slot = p.slot + (int64_t)p.x * a.Hkv;
+    for (int ct = w; 16 * ct < a.Dh; ct += KV8_NW) {
+        kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < KV8_NW; i++) o += so[i][ct][lane] * f[i];
+        if (p.splits > 1) *(kv8_f4 *)(b.part + (slot * 16 + n) * a.Dh + 16 * ct + 4 * g) = o;
+        else *(kv8_f4 *)(b.out + th * a.Dh + 16 * ct + 4 * g) = o / L;
+    }
+    if (p.splits > 1 && w == 0 && g == 0) {
+        b.ml[slot * 32 + n] = M;
+        b.ml[slot * 32 + 16 + n] = L;
+    }
+}
+extern "C" __global__ __launch_bounds__(64 * KV8_NW, 2) void sepia_kv8_attn(Kv8Args a, Kv8Attn b) { kv8_attn_run<true>(a, b); }
+extern "C" __global__ __launch_bounds__(64 * KV8_NW, 2) void sepia_kv8_attn_d(Kv8Args a, Kv8Attn b) { kv8_attn_run<false>(a, b); }
+
+// Folds the runs of every unit that was cut. Grid: as many workgroups as
+// units that may be, a thread for 4 dims of a row at a time.
+extern "C" __global__ __launch_bounds__(256) void sepia_kv8_fold(Kv8Args a, Kv8Attn b) {
+    Kv8Plan p;
+    if (!kv8_plan<true>(a, b, (int)blockIdx.x, p)) return;
+    const Kv8Tile t = kv8_tile(b, p);
+    const int span = (t.steps + p.splits - 1) / p.splits, ns = (t.steps + span - 1) / span, G = b.H / a.Hkv;
+    const int per = a.Dh / 4;
+    for (int i = (int)threadIdx.x; i < 16 * per; i += 256) {
+        const int n = i / per, d = 4 * (i - n * per), ti = n / G;
+        if (ti >= t.nt) continue;
+        float M = -INFINITY, L = 0.0f;
+        for (int x = 0; x < ns; x++) M = fmaxf(M, b.ml[((int64_t)p.slot + (int64_t)x * a.Hkv) * 32 + n]);
+        const float ref = M == -INFINITY ? 0.0f : M;
+        kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int x = 0; x < ns; x++) {
+            const int64_t slot = (int64_t)p.slot + (int64_t)x * a.Hkv;
+            const float f = __builtin_amdgcn_exp2f((b.ml[slot * 32 + n] - ref) * KV8_L2E);
+            L += b.ml[slot * 32 + 16 + n] * f;
+            o += *(const kv8_f4 *)(b.part + (slot * 16 + n) * a.Dh + d) * f;
+        }
+        *(kv8_f4 *)(b.out + ((int64_t)(t.t0 + ti) * b.H + p.hk * G + (n - ti * G)) * a.Dh + d) = o / L;
+    }
+}

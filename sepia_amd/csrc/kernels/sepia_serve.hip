@@ -3,6 +3,7 @@
 // keep their places: some of those measured differently when moved.
 #include "common.h"
 #include "kv8.h"
+#include "kv8_attn.h"
 #include "sample.h"
 
 // The device error word's address (common.h); the host writes it right after

@@ -107,7 +107,7 @@ static const char *const k_names[K_COUNT] = {
 /* Kernels of the second code object, sepia_serve.hsaco (the SK_* of
  * internal.h); their ids follow the first's. */
 static const char *const serve_names[SK_COUNT] = {
-    "sepia_kv8_append", "sepia_kv8_read", "sepia_kv8_attn", "sepia_sample",
+    "sepia_kv8_append", "sepia_kv8_read", "sepia_kv8_attn", "sepia_kv8_attn_d", "sepia_kv8_fold", "sepia_sample",
 };
 #define K_ALL (K_COUNT + SK_COUNT)
 static const char *k_name(int k) { return k < K_COUNT ? k_names[k] : serve_names[k - K_COUNT]; }
@@ -1331,6 +1331,8 @@ static size_t scratch_limit(void) {
     if (hipStreamIsCapturing(g_stream, &cs) == hipSuccess && cs == hipStreamCaptureStatusNone) return SIZE_MAX;
     return g_scratch ? g_scratch_len - CNT_BYTES : 0;
 }
+
+size_t sepia_scratch_limit(void) { return scratch_limit(); }
 
 /* Tokens t0 .. t0 + T - 1 (T <= ATT_TMAX) of a call whose arguments are
  * checked. fold: through partials and the fold launch even without a split

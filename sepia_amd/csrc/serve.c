@@ -146,11 +146,13 @@ int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *
     return kv8_pages(SK_KV8_READ, c, n, args, op);
 }
 
-/* struct Kv8Attn of kernels/kv8.h */
+/* struct Kv8Attn of kernels/kv8_attn.h */
+#define KV8_BUDGET 512      /* runs of a call whose units alone leave the chip idle: two workgroups a CU */
 typedef struct {
     const float *q, *rel, *tau;
     float *out;
-    int32_t H, R, window;
+    float *part, *ml;
+    int32_t H, R, window, TT, budget;
     float c;
 } Kv8Attn;
 
@@ -191,8 +193,30 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
     b.R = (int32_t)rel_extent;
     b.window = window > 0x7FFFFFFF ? 0 : (int32_t)window;
     b.c = inv_head_dim;
+    /* 16 rows a wave; units (row tile, kv head) are cut into runs of steps
+     * where they are few, and the runs folded */
+    b.TT = (int32_t)(16 / (n_heads / c->n_kv_heads));
+    const int64_t ids = n / b.TT + c->n_seqs, few = n / b.TT > c->n_seqs ? n / b.TT : n < c->n_seqs ? n : c->n_seqs;
+    const size_t per = 16 * (size_t)c->head_dim * 4, limit = sepia_scratch_limit();
+    int64_t budget = few * c->n_kv_heads < 2 * KV8_BUDGET ? KV8_BUDGET : 0, slots = 2 * budget + 64;
+    while (budget && (size_t)slots * (per + 128) > limit) {
+        budget /= 2;
+        slots = 2 * budget + 64;
+    }
+    if (budget) {
+        uint8_t *s = (uint8_t *)sepia_scratch((size_t)slots * (per + 128), op);
+        if (!s) return 0;
+        b.part = (float *)s;
+        b.ml = (float *)(s + (size_t)slots * per);
+    }
+    b.budget = (int32_t)budget;
     void *args[] = { &a, &b };
-    return sepia_serve_launch(SK_KV8_ATTN, (unsigned)n, (unsigned)n_heads, 1, 64, args, op);
+    if (!sepia_serve_launch(c->head_dim == 128 ? SK_KV8_ATTN : SK_KV8_ATTN_D, (unsigned)(budget + ids * c->n_kv_heads), 1, 1,
+                            256, args, op))
+        return 0;
+    if (!budget) return 1;
+    const int64_t cut = ids * c->n_kv_heads < budget ? ids * c->n_kv_heads : budget;
+    return sepia_serve_launch(SK_KV8_FOLD, (unsigned)cut, 1, 1, 256, args, op);
 }
 
 /* struct SampleArgs of kernels/sample.h */
