@@ -170,7 +170,7 @@ typedef struct {
     SepiaGpuBuf *top_k;         /* int32, NULL or 0 or less: off */
 } SepiaSampleDesc;
 
-/* The next token of each row of logits (f32, up to 2^20 rows, row r at element
+/* The next token of each row of logits (f32, up to 65535 rows, row r at element
  * r * stride, vocab values of it, 1 to 2^20). A token's weight is exp((logit - largest) /
  * temperature); -inf and NaN have none. In the order of falling logits, equal
  * ones by index: the first top_k tokens are kept, of these the shortest
@@ -178,7 +178,7 @@ typedef struct {
  * min_p or more. tokens[r] (int32) is the first whose cumulative weight
  * exceeds u times the kept weight, -1 for a row without any finite or +inf
  * logit; prob[r] (f32, NULL: not wanted) its share of the kept weight. Sums of
- * weights are exact in units of 2^-44 of the largest weight. */
+ * weights are exact in units of 2^-43 of the largest weight. */
 int sepia_hip_sample(const SepiaSampleDesc *desc, SepiaGpuBuf *logits, int64_t rows, int64_t vocab, int64_t stride,
                      SepiaGpuBuf *tokens, SepiaGpuBuf *prob);
 

@@ -9,174 +9,547 @@
 // each time. The draw is the first token whose cumulative weight exceeds u
 // times the kept weight. T <= 0: the first token of the order.
 //
-// Weights are summed as integers in units of 2^-44 of the largest, so that
+// Weights are summed as integers in units of 2^-43 of the largest, so that
 // every sum is exact and does not depend on its order: a row of up to 2^20
-// tokens sums to less than 2^64, and a weight is within 2^-45 of its value
-// (over n tokens the sums err by about sqrt(n) 2^-46, 10^-11 at most).
+// tokens sums to at most 2^63, and a weight is within 2^-44 of its value
+// (over n tokens the sums err by about sqrt(n) 2^-45, 3e-11 at most).
+//
+// Nothing is sorted but the few tokens next to a decision. One pass over the
+// row counts and sums the tokens by their weight's logarithm (1024 bins, 32 to
+// the octave). The bins' prefix sums then bound where the k-th token, the
+// top-p border and the draw fall: each decision's bound gives the next one's,
+// a bin or a few in all. A second pass gathers the tokens of those bins, whose
+// exact order gives the three in turn. Where they are too many (flat rows,
+// long runs of equal logits) each decision is found by its digits instead.
+//
+// A row is cut into chunks where the rows are fewer than the chip's places,
+// and the passes become launches: each chunk's first token of the order (the
+// row's maximum), each chunk's bins, and the gathering: every workgroup of it
+// sums the row's bins and finds the bins to gather for itself, and the last of
+// a row to arrive with its chunk's tokens decides. (Bins added up by atomics
+// took 73 us at 48 rows of 10 chunks: 64-bit device-scope atomics are carried
+// out at the memory's side.)
 #pragma once
 #include "common.h"
 
-#define SAMPLE_ONE 17592186044416.0   // 2^44: the largest weight
+#define SAMPLE_ONE 8796093022208.0    // 2^43: the largest weight
+#define SAMPLE_NT 1024
+#define SAMPLE_BINS 1024              // one a thread
+#define SAMPLE_CAP 4096               // gathered tokens: four a thread
 
+// In scratch where a row has several chunks: a chunk's bins, and what the
+// row's workgroups gather.
+struct SampleChunk {
+    unsigned long long mass[SAMPLE_BINS], over_min, best;
+    uint32_t count[SAMPLE_BINS];
+};
+struct SampleRow {
+    unsigned long long list[SAMPLE_CAP];
+    uint32_t n, arrived;
+};
 struct SampleArgs {
     const float *logits, *u, *temperature, *top_p, *min_p;
     const int32_t *top_k;
     int32_t *token;
     float *prob;
+    SampleRow *rows;
+    SampleChunk *bins;   // [row][chunk]
     int64_t stride;
-    int32_t vocab;
+    int32_t vocab, chunk, chunks;
 };
 
 // Keys fall as logits rise: 0 is the largest. -0 and +0 are equal.
 __device__ __forceinline__ uint32_t sample_key(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
-    return (int32_t)b < 0 ? b : ~(b | 0x80000000u) & 0x7FFFFFFFu;
+    return (int32_t)b < 0 ? b : ~b & 0x7FFFFFFFu;
 }
 __device__ __forceinline__ float sample_logit(uint32_t key) {
     return __builtin_bit_cast(float, (int32_t)key < 0 ? key : ~key & 0x7FFFFFFFu);
 }
-__device__ __forceinline__ bool sample_on(float x) { return x > -INFINITY; }   // neither -inf nor NaN
-__device__ __forceinline__ double sample_weight(float x, float m, double t) {
-    return x == m ? 1.0 : exp(((double)x - (double)m) / t);
-}
-__device__ __forceinline__ uint64_t sample_mass(float x, float m, double t) {
-    return (uint64_t)__builtin_rint(sample_weight(x, m, t) * SAMPLE_ONE);
+// Place in the order: key, then index. Tokens without weight: the last.
+__device__ __forceinline__ float sample_token(unsigned long long place) { return sample_logit((uint32_t)(place >> 20)); }
+#define SAMPLE_NONE 0xFFFFFFFFFFFFFFFFull
+__device__ __forceinline__ unsigned long long sample_place(float x, int i) {
+    return x > -INFINITY ? ((unsigned long long)sample_key(x) << 20) | (uint32_t)i : SAMPLE_NONE;
 }
 
-#define SAMPLE_NT 1024
-#define SAMPLE_BINS 2048
+// 2^(j / 256), filled by the workgroup: a product of the powers that j's bits
+// stand for, within 8 roundings of 2^-53.
+struct SamplePow {
+    double t[256];
+    __device__ __forceinline__ void fill() {
+        const double p[8] = {0x1.00b1afa5abcbfp+0, 0x1.0163da9fb3335p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0,
+                             0x1.0b5586cf9890fp+0, 0x1.172b83c7d517bp+0, 0x1.306fe0a31b715p+0, 0x1.6a09e667f3bcdp+0};
+        const int j = (int)threadIdx.x;
+        if (j >= 256) return;
+        double e = 1.0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) e *= j >> i & 1 ? p[i] : 1.0;
+        t[j] = e;
+    }
+};
+// The weight's logarithm, base 2: (x - m) log2(e) / T.
+__device__ __forceinline__ double sample_log(float x, float m, double scale) {
+    return x == m ? 0.0 : ((double)x - (double)m) * scale;
+}
+__device__ __forceinline__ int sample_bin(double z) {
+    return z > -32.0 ? (int)(z * -32.0) : SAMPLE_BINS - 1;   // a NaN: the last
+}
+// 2^z: the nearest multiple of 1/256 from the table, the rest, at most
+// ln 2 / 512 = 1.4e-3 in e^r, by its series to the fourth power (4e-17 off).
+__device__ __forceinline__ double sample_pow(double z, const SamplePow &P) {
+    const double big = 6755399441055744.0;
+    const double t = __builtin_fma(z, 256.0, big);
+    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
+    const double r = __builtin_fma(z, 256.0, big - t) * (0.69314718055994530942 / 256.0);
+    double e = __builtin_fma(r, 1.0 / 24.0, 1.0 / 6.0);
+    e = __builtin_fma(e, r, 0.5);
+    e = __builtin_fma(e, r, 1.0);
+    e = __builtin_fma(e, r, 1.0);
+    return __builtin_ldexp(e * P.t[n & 255], n >> 8);
+}
+__device__ __forceinline__ unsigned long long sample_mass(double z, const SamplePow &P) {
+    if (!(z > -45.0)) return 0;
+    return __builtin_bit_cast(unsigned long long, sample_pow(z, P) * SAMPLE_ONE + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+}
+
 struct SampleLds {
-    unsigned long long mass[SAMPLE_BINS];
-    uint32_t count[SAMPLE_BINS];
-    unsigned long long red[16];
-    uint32_t redc[16];
-    int32_t bin;
-    unsigned long long below;
+    unsigned long long mass[SAMPLE_BINS], upto[SAMPLE_BINS + 1];   // sums by bin; of the bins before
+    uint32_t count[SAMPLE_BINS], cupto[SAMPLE_BINS + 1];
+    unsigned long long list[SAMPLE_CAP], base[SAMPLE_BINS];
+    unsigned long long wave[16], set[SAMPLE_BINS / 64], found[3];
+    uint32_t wavec[16], n;
+    SamplePow pow;
 };
 
-__device__ __forceinline__ unsigned long long sample_sum(unsigned long long v, SampleLds &L) {
+// f(value, index) for the row's tokens i0 .. i1 - 1, SAMPLE_LOADS loads of a
+// thread in flight at a time (one at a time, a pass over 100003 logits by one
+// workgroup took 40 us, a loaded memory round trip an iteration).
+#define SAMPLE_LOADS 8
+template <class F>
+__device__ __forceinline__ void sample_walk(const float *__restrict__ x, int i0, int i1, F f) {
+    for (int i = i0 + (int)threadIdx.x; i < i1; i += SAMPLE_LOADS * SAMPLE_NT) {
+        float v[SAMPLE_LOADS];
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+        for (int j = 0; j < SAMPLE_LOADS; j++) v[j] = x[min(i + j * SAMPLE_NT, i1 - 1)];
+#pragma unroll
+        for (int j = 0; j < SAMPLE_LOADS; j++)
+            if (i + j * SAMPLE_NT < i1 && v[j] > -INFINITY) f(v[j], i + j * SAMPLE_NT);
+    }
+}
+
+// Exclusive prefix sums over the workgroup's threads; the total too.
+__device__ __forceinline__ unsigned long long sample_scan(unsigned long long v, unsigned long long *wave,
+                                                          unsigned long long &total) {
+    const int lane = (int)threadIdx.x & 63, w = (int)threadIdx.x >> 6;
+    unsigned long long s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned long long u = __shfl_up(s, o, 64);
+        if (lane >= o) s += u;
+    }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) L.red[threadIdx.x >> 6] = v;
+    if (lane == 63) wave[w] = s;
     __syncthreads();
-    v = 0;
-    for (int i = 0; i < SAMPLE_NT / 64; i++) v += L.red[i];
+    unsigned long long before = 0;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const unsigned long long t = wave[i];
+        if (i < w) before += t;
+        total += t;
+    }
+    return before + s - v;
+}
+__device__ __forceinline__ unsigned long long sample_min(unsigned long long v, unsigned long long *wave) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        const unsigned long long u = __shfl_xor(v, o, 64);
+        v = u < v ? u : v;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; i++) v = wave[i] < v ? wave[i] : v;
     return v;
 }
 
-// The first token of the order whose cumulative weight (by_count: place from
-// 1) exceeds `over`; its key and index, and the cumulative weight up to and
-// with it. There is one. A pass over the row settles 11, 11 and 10 bits of
-// the key, then, among equal logits, 10 and 10 of the index.
-struct SampleAt {
-    uint32_t key;
-    int32_t index;
-    unsigned long long cum;
-};
-__device__ SampleAt sample_find(const SampleArgs &a, const float *x, float m, double t, bool by_count,
-                                unsigned long long over, SampleLds &L) {
-    SampleAt r;
-    uint64_t prefix = 0;          // the settled bits of key << 20 | index
-    int settled = 0;
-    unsigned long long done = 0, mass = 0;   // what lies before the prefix: by the measure, and weight
-    const int bits[5] = {11, 11, 10, 10, 10};
-    for (int level = 0; level < 5; level++) {
-        const int left = 52 - settled - bits[level];
-        for (int i = threadIdx.x; i < SAMPLE_BINS; i += SAMPLE_NT) L.mass[i] = 0, L.count[i] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < a.vocab; i += SAMPLE_NT) {
-            const uint64_t c = ((uint64_t)sample_key(x[i]) << 20) | (uint32_t)i;
-            if (!sample_on(x[i]) || (settled && c >> (52 - settled) != prefix)) continue;
-            const int b = (int)(c >> left) & ((1 << bits[level]) - 1);
-            atomicAdd(&L.count[b], 1u);
-            atomicAdd(&L.mass[b], (unsigned long long)sample_mass(x[i], m, t));
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            int b = 0;
-            while (b < SAMPLE_BINS - 1) {
-                const unsigned long long n = by_count ? L.count[b] : L.mass[b];
-                if (done + n > over) break;
-                done += n;
-                mass += L.mass[b];
-                b++;
-            }
-            L.bin = b;
-            L.below = done;
-            L.red[0] = mass;
-        }
-        __syncthreads();
-        done = L.below;
-        mass = L.red[0];
-        prefix = (prefix << bits[level]) | (uint32_t)L.bin;
-        settled += bits[level];
-        __syncthreads();
-    }
-    r.key = (uint32_t)(prefix >> 20);
-    r.index = (int32_t)(prefix & 0xFFFFF);
-    r.cum = mass + sample_mass(x[r.index], m, t);
-    return r;
+// Bins' prefix sums from L.mass and L.count.
+__device__ __forceinline__ void sample_prefix(SampleLds &L) {
+    const int b = (int)threadIdx.x;
+    unsigned long long total;
+    __syncthreads();
+    const unsigned long long m = sample_scan(L.mass[b], L.wave, total);
+    L.upto[b] = m;
+    if (b == 0) L.upto[SAMPLE_BINS] = total;
+    const unsigned long long c = sample_scan(L.count[b], L.wave, total);
+    L.cupto[b] = (uint32_t)c;
+    if (b == 0) L.cupto[SAMPLE_BINS] = (uint32_t)total;
+    __syncthreads();
+}
+// The bin with upto[b] <= over < upto[b + 1] (cupto with by_count), by every
+// wave for itself: 64 bins apart, then 16 of them.
+__device__ __forceinline__ int sample_seek(const SampleLds &L, bool by_count, unsigned long long over) {
+    const int lane = (int)threadIdx.x & 63;
+    const uint64_t far = __ballot((by_count ? L.cupto[16 * lane] : L.upto[16 * lane]) <= over);
+    const int b = 16 * (63 - __builtin_clzll(far)) + (lane & 15);
+    const uint64_t near = __ballot((by_count ? L.cupto[b] : L.upto[b]) <= over) & 0xFFFF;
+    return 16 * (63 - __builtin_clzll(far)) + 31 - __builtin_clz((uint32_t)near);
 }
 
+// The first token of the order whose cumulative weight (by_count: place from
+// 1) exceeds `over`, and the weight up to and with it, by the order's digits:
+// a pass over the row settles ten bits of the place.
+struct SampleAt {
+    unsigned long long place, cum;
+};
+__device__ __forceinline__ SampleAt sample_find(const float *x, int vocab, float m, double scale, bool by_count,
+                                                unsigned long long over, SampleLds &L) {
+    unsigned long long prefix = 0, mass = 0, last = 0;
+    for (int left = 50; left >= 0; left -= 10) {   // 62 bits hold the 52 of a place
+        L.mass[threadIdx.x] = 0;
+        L.count[threadIdx.x] = 0;
+        __syncthreads();
+        sample_walk(x, 0, vocab, [&](float v, int i) {
+            const unsigned long long at = sample_place(v, i);
+            if (at >> left >> 10 != prefix) return;
+            const int b = (int)(at >> left) & 1023;
+            atomicAdd(&L.count[b], 1u);
+            atomicAdd(&L.mass[b], sample_mass(sample_log(v, m, scale), L.pow));
+        });
+        sample_prefix(L);
+        const int b = sample_seek(L, by_count, over);
+        over -= by_count ? L.cupto[b] : L.upto[b];
+        mass += L.upto[b];
+        last = L.mass[b];
+        prefix = prefix << 10 | (unsigned)b;
+        __syncthreads();
+    }
+    return SampleAt{prefix, mass + last};
+}
+
+// What a row asks for, as its workgroups need it.
+struct SampleAsk {
+    const float *x;
+    float m, p, u;
+    int vocab, k;
+    double scale;
+    unsigned long long over_min;   // the weight of its tokens of w >= min-p
+    bool by_k, by_p;
+    int bk;                        // the bin of its k-th token
+};
+__device__ __forceinline__ unsigned long long sample_share(float f, unsigned long long total) {
+    return (unsigned long long)((double)f * (double)total);
+}
+// The least cumulative weight that is at least p of the total.
+__device__ __forceinline__ unsigned long long sample_want(float p, unsigned long long total) {
+    const double w = __builtin_ceil((double)fmaxf(p, 0.0f) * (double)total);
+    return w >= 1.0 ? (unsigned long long)w : 1;
+}
+__device__ __forceinline__ unsigned long long sample_over(float u, unsigned long long kept) {
+    const unsigned long long over = u > 0.0f ? sample_share(fminf(u, 1.0f), kept) : 0;
+    return over >= kept ? kept ? kept - 1 : 0 : over;
+}
+// From the row's bins in L.mass (and L.count, if its k may cut): their prefix
+// sums, and in L.set the bins that decide. Returns the least logit of those.
+__device__ __forceinline__ float sample_bounds(SampleAsk &q, SampleLds &L) {
+    const int tid = (int)threadIdx.x;
+    sample_prefix(L);
+    const unsigned long long all = L.upto[SAMPLE_BINS];
+    q.by_k = q.k > 0 && (uint32_t)q.k < L.cupto[SAMPLE_BINS];
+    q.by_p = q.p < 1.0f;
+    q.bk = -1;
+    // each decision's bin, or the range of bins that the one before leaves it
+    unsigned long long lo = all, hi = all;   // the weight kept so far is in [lo, hi]
+    int p0 = 0, p1 = -1;
+    if (q.by_k) {
+        q.bk = sample_seek(L, true, (unsigned long long)q.k - 1);
+        lo = L.upto[q.bk];
+        hi = L.upto[q.bk + 1];
+    }
+    if (q.by_p) {
+        const unsigned long long w0 = sample_want(q.p, lo), w1 = sample_want(q.p, hi);
+        p0 = sample_seek(L, false, w0 - 1);
+        p1 = w0 == w1 ? p0 : sample_seek(L, false, w1 - 1);
+        lo = w0;
+        hi = L.upto[p1 + 1];
+    }
+    lo = lo < q.over_min ? lo : q.over_min;
+    hi = hi < q.over_min ? hi : q.over_min;
+    const int d0 = sample_seek(L, false, sample_over(q.u, lo));
+    const int d1 = lo == hi ? d0 : sample_seek(L, false, sample_over(q.u, hi));
+    const bool in = tid == q.bk || (tid >= p0 && tid <= p1) || (tid >= d0 && tid <= d1);
+    const unsigned long long word = __ballot(in);
+    if ((tid & 63) == 0) L.set[tid >> 6] = word;
+    const int last = max(max(q.bk, p1), d1);
+    if (tid == 0) L.n = 0;
+    __syncthreads();
+    if (last == SAMPLE_BINS - 1) return -INFINITY;
+    if (q.m == INFINITY) return q.m;   // all other tokens are in the last bin
+    const double least = (double)q.m - (double)(last + 1) / 32.0 / q.scale;
+    return (float)(least - (fabs(least) + fabs((double)q.m)) * 0x1p-20);   // rounded down, surely
+}
+// The chosen bins' tokens among the row's i0 .. i1 - 1 into L.list; L.n counts
+// them, also where they are more than the list holds.
+__device__ __forceinline__ void sample_gather(const SampleAsk &q, float least, int i0, int i1, SampleLds &L) {
+    sample_walk(q.x, i0, i1, [&](float v, int i) {
+        if (!(v >= least)) return;
+        const int b = sample_bin(sample_log(v, q.m, q.scale));
+        if (!(L.set[b >> 6] >> (b & 63) & 1)) return;
+        const uint32_t at = atomicAdd(&L.n, 1u);
+        if (at < SAMPLE_CAP) L.list[at] = sample_place(v, i);
+    });
+    __syncthreads();
+}
+// The decision from the n gathered tokens in L.list.
+__device__ __forceinline__ void sample_finish(const SampleArgs &a, int row, const SampleAsk &q, uint32_t n, SampleLds &L) {
+    const int tid = (int)threadIdx.x;
+    unsigned long long kept = L.upto[SAMPLE_BINS], place;
+    if (n <= SAMPLE_CAP) {
+        int size = 2;
+        while (size < (int)n) size <<= 1;
+        for (int i = (int)n + tid; i < size; i += SAMPLE_NT) L.list[i] = SAMPLE_NONE;
+        for (int k = 2; k <= size; k <<= 1)
+            for (int j = k >> 1; j; j >>= 1) {
+                __syncthreads();
+                for (int h = tid; h < size / 2; h += SAMPLE_NT) {
+                    const int i = 2 * h - (h & (j - 1)), o = i + j;
+                    const unsigned long long s = L.list[i], t = L.list[o];
+                    if ((s > t) == !(i & k)) {
+                        L.list[i] = t;
+                        L.list[o] = s;
+                    }
+                }
+            }
+        __syncthreads();
+        // four tokens a thread, in order: weights, and the weight before each,
+        // of the bins before its own and then within it
+        unsigned long long p[4], w[4], before, total, sum = 0;
+        int b[4];
+        bool first[4];
+        int prev = tid > 0 && 4 * tid < (int)n ? sample_bin(sample_log(sample_token(L.list[4 * tid - 1]), q.m, q.scale)) : -1;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const bool on = 4 * tid + e < (int)n;
+            p[e] = on ? L.list[4 * tid + e] : SAMPLE_NONE;
+            const double z = on ? sample_log(sample_token(p[e]), q.m, q.scale) : 0.0;
+            b[e] = on ? sample_bin(z) : -1;
+            w[e] = on ? sample_mass(z, L.pow) : 0;
+            first[e] = on && b[e] != prev;
+            prev = b[e];
+            sum += w[e];
+        }
+        before = sample_scan(sum, L.wave, total);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (first[e]) {
+                L.base[b[e]] = before;
+                L.count[b[e]] = (uint32_t)(4 * tid + e);   // the counts are in cupto
+            }
+            before += w[e];
+        }
+        __syncthreads();
+        before -= sum;
+        unsigned long long cum[4];   // up to and with it
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            before += w[e];
+            cum[e] = b[e] >= 0 ? L.upto[b[e]] + before - L.base[b[e]] : 0;
+        }
+        if (q.by_k) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (b[e] == q.bk && L.cupto[b[e]] + (4 * tid + e - L.count[b[e]]) + 1 == (uint32_t)q.k) L.found[0] = cum[e];
+            __syncthreads();
+            kept = L.found[0];
+        }
+        if (q.by_p) {
+            const unsigned long long want = sample_want(q.p, kept);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (cum[e] - w[e] < want && want <= cum[e]) L.found[1] = cum[e];
+            __syncthreads();
+            kept = L.found[1];
+        }
+        kept = kept < q.over_min ? kept : q.over_min;
+        const unsigned long long over = sample_over(q.u, kept);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (cum[e] - w[e] <= over && over < cum[e]) L.found[2] = p[e];
+        __syncthreads();
+        place = L.found[2];
+    } else {
+        for (int step = q.by_k ? 0 : q.by_p ? 1 : 2;; step = step == 0 && q.by_p ? 1 : 2) {   // top-k, top-p, the draw
+            if (step == 2 && kept > q.over_min) kept = q.over_min;
+            const unsigned long long over = step == 0 ? (unsigned long long)q.k - 1
+                                            : step == 1 ? sample_want(q.p, kept) - 1 : sample_over(q.u, kept);
+            const SampleAt r = sample_find(q.x, q.vocab, q.m, q.scale, step == 0, over, L);
+            place = r.place;
+            if (step == 2) break;
+            kept = r.cum;
+        }
+    }
+    if (tid == 0) {
+        a.token[row] = (int32_t)(place & 0xFFFFF);
+        if (a.prob)
+            a.prob[row] = (float)(sample_pow(sample_log(sample_token(place), q.m, q.scale), L.pow) * SAMPLE_ONE /
+                                  (double)kept);
+    }
+}
+
+// A row's first token of the order among i0 .. i1 - 1.
+__device__ __forceinline__ unsigned long long sample_best(const float *x, int i0, int i1, unsigned long long *wave) {
+    unsigned long long best = SAMPLE_NONE;
+    sample_walk(x, i0, i1, [&](float v, int i) {
+        const unsigned long long p = sample_place(v, i);
+        best = p < best ? p : best;
+    });
+    return sample_min(best, wave);
+}
+// A row's first token from its chunks'.
+__device__ __forceinline__ unsigned long long sample_first(const SampleArgs &a, int row, unsigned long long *wave) {
+    unsigned long long best = SAMPLE_NONE;
+    if ((int)threadIdx.x < a.chunks) best = a.bins[(int64_t)row * a.chunks + (int)threadIdx.x].best;
+    return sample_min(best, wave);
+}
+// Whether the row's first token is all there is to decide; the workgroup of
+// `write` says so.
+__device__ __forceinline__ bool sample_done(const SampleArgs &a, int row, unsigned long long best, bool write) {
+    const float temperature = a.temperature ? a.temperature[row] : 1.0f;
+    if (best != SAMPLE_NONE && temperature > 0.0f && !(a.top_k && a.top_k[row] == 1)) return false;
+    if (write && threadIdx.x == 0) {
+        a.token[row] = best == SAMPLE_NONE ? -1 : (int32_t)(best & 0xFFFFF);
+        if (a.prob) a.prob[row] = best == SAMPLE_NONE ? 0.0f : 1.0f;
+    }
+    return true;
+}
+__device__ __forceinline__ SampleAsk sample_ask(const SampleArgs &a, int row, unsigned long long best) {
+    SampleAsk q;
+    q.x = a.logits + (int64_t)row * a.stride;
+    q.m = sample_logit((uint32_t)(best >> 20));
+    q.vocab = a.vocab;
+    q.k = a.top_k ? a.top_k[row] : 0;
+    q.p = a.top_p ? a.top_p[row] : 1.0f;
+    q.u = a.u[row];
+    q.scale = 1.4426950408889634074 / (double)(a.temperature ? a.temperature[row] : 1.0f);
+    q.over_min = 0;
+    return q;
+}
+// The bins of the row's tokens i0 .. i1 - 1 in L.mass and, where its k may
+// cut, L.count; q.over_min.
+__device__ __forceinline__ void sample_bins(const SampleArgs &a, int row, SampleAsk &q, int i0, int i1, SampleLds &L) {
+    const int tid = (int)threadIdx.x;
+    const float min_p = a.min_p && a.min_p[row] > 0.0f ? fminf(a.min_p[row], 1.0f) : 0.0f;
+    const unsigned long long floor_mass = min_p > 0.0f ? (unsigned long long)__builtin_ceil((double)min_p * SAMPLE_ONE) : 0;
+    L.mass[tid] = 0;
+    L.count[tid] = 0;
+    L.pow.fill();
+    __syncthreads();
+    unsigned long long tail = 0, over_min = 0, tails, ntails;
+    uint32_t ntail = 0;
+    const bool counted = q.k > 0;
+    sample_walk(q.x, i0, i1, [&](float v, int) {
+        const double z = sample_log(v, q.m, q.scale);
+        const int b = sample_bin(z);
+        const unsigned long long w = sample_mass(z, L.pow);
+        if (w >= floor_mass) over_min += w;
+        if (b == SAMPLE_BINS - 1) {   // many of a row's tokens: not one by one to the same bin
+            tail += w;
+            ntail++;
+        } else {
+            atomicAdd(&L.mass[b], w);
+            if (counted) atomicAdd(&L.count[b], 1u);
+        }
+    });
+    sample_scan(tail, L.wave, tails);
+    sample_scan(ntail, L.wave, ntails);
+    sample_scan(over_min, L.wave, q.over_min);
+    if (tid == SAMPLE_BINS - 1) {
+        L.mass[tid] = tails;
+        L.count[tid] = (uint32_t)ntails;
+    }
+    __syncthreads();
+}
+
+// Grid (chunks, rows): the chunk's first token of the order; the row's counters
+// cleared.
+extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_max(SampleArgs a) {
+    __shared__ unsigned long long wave[16];
+    const int c = (int)blockIdx.x, row = (int)blockIdx.y;
+    const unsigned long long best =
+        sample_best(a.logits + (int64_t)row * a.stride, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), wave);
+    if (threadIdx.x) return;
+    a.bins[(int64_t)row * a.chunks + c].best = best;
+    if (c == 0) a.rows[row].n = a.rows[row].arrived = 0;
+}
+
+// Grid (chunks, rows): the chunk's bins.
+extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_bins(SampleArgs a) {
+    __shared__ SampleLds L;
+    const int c = (int)blockIdx.x, row = (int)blockIdx.y, tid = (int)threadIdx.x;
+    const unsigned long long best = sample_first(a, row, L.wave);
+    if (sample_done(a, row, best, c == 0)) return;
+    SampleAsk q = sample_ask(a, row, best);
+    sample_bins(a, row, q, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), L);
+    SampleChunk *o = a.bins + (int64_t)row * a.chunks + c;
+    o->mass[tid] = L.mass[tid];
+    if (q.k > 0) o->count[tid] = L.count[tid];
+    if (tid == 0) o->over_min = q.over_min;
+}
+
+// Grid (chunks, rows): the decision, over the chunks' bins.
+extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_pick(SampleArgs a) {
+    __shared__ SampleLds L;
+    const int c = (int)blockIdx.x, row = (int)blockIdx.y, tid = (int)threadIdx.x;
+    const unsigned long long best = sample_first(a, row, L.wave);
+    if (sample_done(a, row, best, false)) return;
+    SampleAsk q = sample_ask(a, row, best);
+    const SampleChunk *o = a.bins + (int64_t)row * a.chunks;
+    unsigned long long mass = 0;
+    uint32_t count = 0;
+    for (int i = 0; i < a.chunks; i++) {
+        mass += o[i].mass[tid];
+        if (q.k > 0) count += o[i].count[tid];
+        q.over_min += o[i].over_min;
+    }
+    L.mass[tid] = mass;
+    L.count[tid] = count;
+    L.pow.fill();
+    const float least = sample_bounds(q, L);
+    sample_gather(q, least, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), L);
+    // The gathered tokens cross workgroups as relaxed agent-scope atomics: the
+    // wait and the barrier order them before the arrival, the last arriver's
+    // loads come after its own (a fence would write back the whole L2).
+    SampleRow *r = a.rows + row;
+    const uint32_t n = L.n;
+    __shared__ uint32_t at;
+    if (tid == 0) at = __hip_atomic_fetch_add(&r->n, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (at + n <= SAMPLE_CAP)
+        for (int i = tid; i < (int)n; i += SAMPLE_NT)
+            __hip_atomic_store(&r->list[at + i], L.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) at = __hip_atomic_fetch_add(&r->arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (at + 1 != (uint32_t)a.chunks) return;
+    const uint32_t total = __hip_atomic_load(&r->n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (total <= SAMPLE_CAP)
+        for (int i = tid; i < (int)total; i += SAMPLE_NT)
+            L.list[i] = __hip_atomic_load(&r->list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sample_finish(a, row, q, total, L);
+}
+
+// Grid (1, rows): a row by one workgroup.
 extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample(SampleArgs a) {
     __shared__ SampleLds L;
-    const int row = (int)blockIdx.x;
-    const float *x = a.logits + (int64_t)row * a.stride;
-    float m = -INFINITY;
-    unsigned long long n = 0;
-    for (int i = threadIdx.x; i < a.vocab; i += SAMPLE_NT) {
-        m = fmaxf(m, x[i]);
-        n += sample_on(x[i]);
-    }
-    n = sample_sum(n, L);
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) L.redc[threadIdx.x >> 6] = __builtin_bit_cast(uint32_t, m);
-    __syncthreads();
-    for (int i = 0; i < SAMPLE_NT / 64; i++) m = fmaxf(m, __builtin_bit_cast(float, L.redc[i]));
-    if (n == 0) {
-        if (threadIdx.x == 0) {
-            a.token[row] = -1;
-            if (a.prob) a.prob[row] = 0.0f;
-        }
-        return;
-    }
-    const float temperature = a.temperature ? a.temperature[row] : 1.0f;
-    const float top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p && a.min_p[row] > 0.0f ? fminf(a.min_p[row], 1.0f) : 0.0f;
-    const int32_t k = a.top_k ? a.top_k[row] : 0;
-    if (!(temperature > 0.0f)) {
-        const SampleAt r = sample_find(a, x, m, 1.0, true, 0, L);
-        if (threadIdx.x == 0) {
-            a.token[row] = r.index;
-            if (a.prob) a.prob[row] = 1.0f;
-        }
-        return;
-    }
-    const double t = (double)temperature;
-    const unsigned long long floor_mass = min_p > 0.0f ? (unsigned long long)__builtin_ceil((double)min_p * SAMPLE_ONE) : 0;
-    unsigned long long all = 0, over_min = 0;
-    for (int i = threadIdx.x; i < a.vocab; i += SAMPLE_NT) {
-        const unsigned long long w = sample_on(x[i]) ? sample_mass(x[i], m, t) : 0;
-        all += w;
-        over_min += w >= floor_mass ? w : 0;
-    }
-    unsigned long long kept = sample_sum(all, L);
-    over_min = sample_sum(over_min, L);
-    if (k > 0 && (unsigned long long)k < n) kept = sample_find(a, x, m, t, true, (unsigned long long)k - 1, L).cum;
-    if (top_p < 1.0f) {
-        // the last kept token is the first with cumulative weight >= p times the total
-        const double want = __builtin_ceil((double)fmaxf(top_p, 0.0f) * (double)kept);
-        kept = sample_find(a, x, m, t, false, want >= 1.0 ? (unsigned long long)want - 1 : 0, L).cum;
-    }
-    if (over_min < kept) kept = over_min;
-    const float u = a.u[row];
-    unsigned long long over = u > 0.0f ? (unsigned long long)((double)fminf(u, 1.0f) * (double)kept) : 0;
-    if (over >= kept) over = kept - 1;
-    const SampleAt r = sample_find(a, x, m, t, false, over, L);
-    if (threadIdx.x == 0) {
-        a.token[row] = r.index;
-        if (a.prob) a.prob[row] = (float)(sample_weight(x[r.index], m, t) * SAMPLE_ONE / (double)kept);
-    }
+    const int row = (int)blockIdx.y;
+    const unsigned long long best = sample_best(a.logits + (int64_t)row * a.stride, 0, a.vocab, L.wave);
+    if (sample_done(a, row, best, true)) return;
+    SampleAsk q = sample_ask(a, row, best);
+    sample_bins(a, row, q, 0, a.vocab, L);
+    const float least = sample_bounds(q, L);
+    sample_gather(q, least, 0, a.vocab, L);
+    sample_finish(a, row, q, L.n, L);
 }

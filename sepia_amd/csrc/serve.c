@@ -10,7 +10,7 @@
 
 #define LOG(...) sepia_log(__VA_ARGS__)
 #define MAX_ROWS ((int64_t)1 << 24)     /* rows of a call: grids of fewer than 2^32 threads */
-#define MAX_SAMPLES ((int64_t)1 << 20)
+#define MAX_SAMPLES 65535              /* and of a sample call: the grid's second dimension */
 
 /* struct Kv8Args of kernels/kv8.h */
 typedef struct {
@@ -219,14 +219,21 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
     return sepia_serve_launch(SK_KV8_FOLD, (unsigned)cut, 1, 1, 256, args, op);
 }
 
-/* struct SampleArgs of kernels/sample.h */
+/* struct SampleArgs of kernels/sample.h, and the bytes of its SampleRow and
+ * SampleChunk */
+#define SAMPLE_ROW_BYTES (4096 * 8 + 8)
+#define SAMPLE_CHUNK_BYTES (1024 * 12 + 16)
+#define SAMPLE_CHUNKS 16    /* chunks of a row at most */
+#define SAMPLE_CHUNK 8192   /* logits of a chunk at least */
+#define SAMPLE_PLACES 512   /* workgroups that the chip holds, two a CU */
 typedef struct {
     const float *logits, *u, *temperature, *top_p, *min_p;
     const int32_t *top_k;
     int32_t *token;
     float *prob;
+    uint8_t *rows, *bins;
     int64_t stride;
-    int32_t vocab;
+    int32_t vocab, chunk, chunks;
 } SampleArgs;
 
 int sepia_hip_sample(const SepiaSampleDesc *d, SepiaGpuBuf *logits, int64_t rows, int64_t vocab, int64_t stride,
@@ -275,6 +282,20 @@ int sepia_hip_sample(const SepiaSampleDesc *d, SepiaGpuBuf *logits, int64_t rows
     a.prob = (float *)sepia_buf_dev(prob);
     a.stride = stride;
     a.vocab = (int32_t)vocab;
+    /* chunks of a row: as many as the rows leave places for */
+    int64_t chunks = (vocab + SAMPLE_CHUNK - 1) / SAMPLE_CHUNK;
+    if (chunks > SAMPLE_PLACES / rows) chunks = SAMPLE_PLACES / rows;
+    if (chunks > SAMPLE_CHUNKS) chunks = SAMPLE_CHUNKS;
+    const size_t per = SAMPLE_ROW_BYTES + SAMPLE_CHUNK_BYTES * (size_t)(chunks > 0 ? chunks : 1);
+    if (chunks < 2 || (size_t)rows * per > sepia_scratch_limit()) chunks = 1;
+    a.chunks = (int32_t)chunks;
+    a.chunk = (int32_t)((vocab + chunks - 1) / chunks);
     void *args[] = { &a };
-    return sepia_serve_launch(SK_SAMPLE, (unsigned)rows, 1, 1, 1024, args, op);
+    if (chunks == 1) return sepia_serve_launch(SK_SAMPLE, 1, (unsigned)rows, 1, 1024, args, op);
+    a.rows = (uint8_t *)sepia_scratch((size_t)rows * per, op);
+    if (!a.rows) return 0;
+    a.bins = a.rows + (size_t)rows * SAMPLE_ROW_BYTES;
+    for (int k = SK_SAMPLE_MAX; k <= SK_SAMPLE_PICK; k++)
+        if (!sepia_serve_launch(k, (unsigned)chunks, (unsigned)rows, 1, 1024, args, op)) return 0;
+    return 1;
 }

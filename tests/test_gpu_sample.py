@@ -2,8 +2,8 @@
 vocabularies from one token to 2^20, equal logits, empty rows, and every filter alone and together.
 
 A decision may differ where a cumulative weight lies nearer to what it is compared with than the sums' own rounding:
-2^-45 of the largest weight a token on this side, and less in numpy's. The tests' inputs are checked to be further
-off than that (`near`), so tokens have to be equal; the share is rounded to f32 (2^-24) from sums within vocab * 2^-45
+2^-44 of the largest weight a token on this side, and less in numpy's. The tests' inputs are checked to be further
+off than that (`near`), so tokens have to be equal; the share is rounded to f32 (2^-24) from sums within vocab * 2^-44
 of a kept weight of at least 1, the largest."""
 import ctypes
 
@@ -77,7 +77,7 @@ def test_mixed_rows(dev, rows, vocab):
           top_k=rng.choice([0, 1, 5, 64, 1000], rows).astype(np.int32))
 
 
-@pytest.mark.parametrize("vocab", [8, 1024, 65536, 100003])
+@pytest.mark.parametrize("vocab", [8, 1024, 65536, 100003, 1 << 20])
 def test_equal_logits(dev, vocab):
     """All weights are 1: every sum is exact, and ties go to the lowest index."""
     x = np.full((6, vocab), 2.5, np.float32)
