@@ -33,9 +33,11 @@
 #include "common.h"
 
 #define SAMPLE_ONE 8796093022208.0    // 2^43: the largest weight
-#define SAMPLE_NT 1024
-#define SAMPLE_BINS 1024              // one a thread
-#define SAMPLE_CAP 4096               // gathered tokens: four a thread
+#define SAMPLE_NT 512                 // two workgroups a CU (of 1024 threads one: 36 against 26 us at 48 rows)
+#define SAMPLE_WAVES (SAMPLE_NT / 64)
+#define SAMPLE_BINS 1024              // two a thread
+#define SAMPLE_CAP 4096               // gathered tokens: eight a thread
+#define SAMPLE_OWN (SAMPLE_CAP / SAMPLE_NT)
 
 // In scratch where a row has several chunks: a chunk's bins, and what the
 // row's workgroups gather.
@@ -88,37 +90,38 @@ struct SamplePow {
         t[j] = e;
     }
 };
-// The weight's logarithm, base 2: (x - m) log2(e) / T.
+// The weight's logarithm in units of 1/256 octave, (x - m) 256 log2(e) / T,
+// at least -15360 (2^-60). The minimum also makes 0 of infinity - infinity.
 __device__ __forceinline__ double sample_log(float x, float m, double scale) {
-    return x == m ? 0.0 : ((double)x - (double)m) * scale;
+    return __builtin_fmax(__builtin_fmin(((double)x - (double)m) * scale, 0.0), -15360.0);
 }
-__device__ __forceinline__ int sample_bin(double z) {
-    return z > -32.0 ? (int)(z * -32.0) : SAMPLE_BINS - 1;   // a NaN: the last
-}
-// 2^z: the nearest multiple of 1/256 from the table, the rest, at most
-// ln 2 / 512 = 1.4e-3 in e^r, by its series to the fourth power (4e-17 off).
-__device__ __forceinline__ double sample_pow(double z, const SamplePow &P) {
-    const double big = 6755399441055744.0;
-    const double t = __builtin_fma(z, 256.0, big);
-    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
-    const double r = __builtin_fma(z, 256.0, big - t) * (0.69314718055994530942 / 256.0);
-    double e = __builtin_fma(r, 1.0 / 24.0, 1.0 / 6.0);
-    e = __builtin_fma(e, r, 0.5);
+// Its nearest integer (1.5 * 2^52 leaves it in the sum's low word), and the
+// bin of eight of those.
+#define SAMPLE_BIG 6755399441055744.0
+__device__ __forceinline__ int sample_low(double t) { return (int)(uint32_t)__builtin_bit_cast(uint64_t, t); }
+__device__ __forceinline__ int sample_bin(double z) { return min(-sample_low(z + SAMPLE_BIG) >> 3, SAMPLE_BINS - 1); }
+// 2^(z / 256 + shift): the nearest integer by the table, the rest, at most 1/2,
+// by the fourth power of the series of 2^(r / 256) (4e-17 off).
+__device__ __forceinline__ double sample_pow(double z, const SamplePow &P, int shift) {
+    const double c = 0.69314718055994530942 / 256.0, t = z + SAMPLE_BIG, r = z - (t - SAMPLE_BIG);
+    const int n = sample_low(t);
+    double e = __builtin_fma(r, c * c * c * c / 24.0, c * c * c / 6.0);
+    e = __builtin_fma(e, r, c * c / 2.0);
+    e = __builtin_fma(e, r, c);
     e = __builtin_fma(e, r, 1.0);
-    e = __builtin_fma(e, r, 1.0);
-    return __builtin_ldexp(e * P.t[n & 255], n >> 8);
+    return __builtin_ldexp(e * P.t[n & 255], (n >> 8) + shift);
 }
+// The weight in units of 2^-43 (2^52 leaves it in the sum's low 52 bits).
 __device__ __forceinline__ unsigned long long sample_mass(double z, const SamplePow &P) {
-    if (!(z > -45.0)) return 0;
-    return __builtin_bit_cast(unsigned long long, sample_pow(z, P) * SAMPLE_ONE + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+    return __builtin_bit_cast(unsigned long long, sample_pow(z, P, 43) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
 }
 
 struct SampleLds {
     unsigned long long mass[SAMPLE_BINS], upto[SAMPLE_BINS + 1];   // sums by bin; of the bins before
     uint32_t count[SAMPLE_BINS], cupto[SAMPLE_BINS + 1];
     unsigned long long list[SAMPLE_CAP], base[SAMPLE_BINS];
-    unsigned long long wave[16], set[SAMPLE_BINS / 64], found[3];
-    uint32_t wavec[16], n;
+    unsigned long long wave[SAMPLE_WAVES], set[SAMPLE_BINS / 64], found[3];
+    uint32_t n;
     SamplePow pow;
 };
 
@@ -154,7 +157,7 @@ __device__ __forceinline__ unsigned long long sample_scan(unsigned long long v, 
     unsigned long long before = 0;
     total = 0;
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
+    for (int i = 0; i < SAMPLE_WAVES; i++) {
         const unsigned long long t = wave[i];
         if (i < w) before += t;
         total += t;
@@ -171,20 +174,26 @@ __device__ __forceinline__ unsigned long long sample_min(unsigned long long v, u
     if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = v;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 16; i++) v = wave[i] < v ? wave[i] : v;
+    for (int i = 0; i < SAMPLE_WAVES; i++) v = wave[i] < v ? wave[i] : v;
     return v;
 }
 
+__device__ __forceinline__ void sample_clear(SampleLds &L) {
+    for (int i = (int)threadIdx.x; i < SAMPLE_BINS; i += SAMPLE_NT) L.mass[i] = 0, L.count[i] = 0;
+    __syncthreads();
+}
 // Bins' prefix sums from L.mass and L.count.
 __device__ __forceinline__ void sample_prefix(SampleLds &L) {
-    const int b = (int)threadIdx.x;
+    const int b = 2 * (int)threadIdx.x;
     unsigned long long total;
     __syncthreads();
-    const unsigned long long m = sample_scan(L.mass[b], L.wave, total);
+    const unsigned long long m = sample_scan(L.mass[b] + L.mass[b + 1], L.wave, total);
     L.upto[b] = m;
+    L.upto[b + 1] = m + L.mass[b];
     if (b == 0) L.upto[SAMPLE_BINS] = total;
-    const unsigned long long c = sample_scan(L.count[b], L.wave, total);
+    const unsigned long long c = sample_scan((unsigned long long)L.count[b] + L.count[b + 1], L.wave, total);
     L.cupto[b] = (uint32_t)c;
+    L.cupto[b + 1] = (uint32_t)c + L.count[b];
     if (b == 0) L.cupto[SAMPLE_BINS] = (uint32_t)total;
     __syncthreads();
 }
@@ -208,9 +217,7 @@ __device__ __forceinline__ SampleAt sample_find(const float *x, int vocab, float
                                                 unsigned long long over, SampleLds &L) {
     unsigned long long prefix = 0, mass = 0, last = 0;
     for (int left = 50; left >= 0; left -= 10) {   // 62 bits hold the 52 of a place
-        L.mass[threadIdx.x] = 0;
-        L.count[threadIdx.x] = 0;
-        __syncthreads();
+        sample_clear(L);
         sample_walk(x, 0, vocab, [&](float v, int i) {
             const unsigned long long at = sample_place(v, i);
             if (at >> left >> 10 != prefix) return;
@@ -235,7 +242,7 @@ struct SampleAsk {
     float m, p, u;
     int vocab, k;
     double scale;
-    unsigned long long over_min;   // the weight of its tokens of w >= min-p
+    unsigned long long over_min;   // the weight of its tokens of w >= min-p (no min-p: the largest number)
     bool by_k, by_p;
     int bk;                        // the bin of its k-th token
 };
@@ -279,15 +286,16 @@ __device__ __forceinline__ float sample_bounds(SampleAsk &q, SampleLds &L) {
     hi = hi < q.over_min ? hi : q.over_min;
     const int d0 = sample_seek(L, false, sample_over(q.u, lo));
     const int d1 = lo == hi ? d0 : sample_seek(L, false, sample_over(q.u, hi));
-    const bool in = tid == q.bk || (tid >= p0 && tid <= p1) || (tid >= d0 && tid <= d1);
-    const unsigned long long word = __ballot(in);
-    if ((tid & 63) == 0) L.set[tid >> 6] = word;
+    for (int b = tid; b < SAMPLE_BINS; b += SAMPLE_NT) {
+        const unsigned long long word = __ballot(b == q.bk || (b >= p0 && b <= p1) || (b >= d0 && b <= d1));
+        if ((tid & 63) == 0) L.set[b >> 6] = word;
+    }
     const int last = max(max(q.bk, p1), d1);
     if (tid == 0) L.n = 0;
     __syncthreads();
     if (last == SAMPLE_BINS - 1) return -INFINITY;
     if (q.m == INFINITY) return q.m;   // all other tokens are in the last bin
-    const double least = (double)q.m - (double)(last + 1) / 32.0 / q.scale;
+    const double least = (double)q.m - (double)(8 * last + 9) / q.scale;
     return (float)(least - (fabs(least) + fabs((double)q.m)) * 0x1p-20);   // rounded down, surely
 }
 // The chosen bins' tokens among the row's i0 .. i1 - 1 into L.list; L.n counts
@@ -323,16 +331,16 @@ __device__ __forceinline__ void sample_finish(const SampleArgs &a, int row, cons
                 }
             }
         __syncthreads();
-        // four tokens a thread, in order: weights, and the weight before each,
+        // some tokens a thread, in order: weights, and the weight before each,
         // of the bins before its own and then within it
-        unsigned long long p[4], w[4], before, total, sum = 0;
-        int b[4];
-        bool first[4];
-        int prev = tid > 0 && 4 * tid < (int)n ? sample_bin(sample_log(sample_token(L.list[4 * tid - 1]), q.m, q.scale)) : -1;
+        unsigned long long p[SAMPLE_OWN], w[SAMPLE_OWN], before, total, sum = 0;
+        int b[SAMPLE_OWN];
+        bool first[SAMPLE_OWN];
+        int prev = tid > 0 && SAMPLE_OWN * tid < (int)n ? sample_bin(sample_log(sample_token(L.list[SAMPLE_OWN * tid - 1]), q.m, q.scale)) : -1;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const bool on = 4 * tid + e < (int)n;
-            p[e] = on ? L.list[4 * tid + e] : SAMPLE_NONE;
+        for (int e = 0; e < SAMPLE_OWN; e++) {
+            const bool on = SAMPLE_OWN * tid + e < (int)n;
+            p[e] = on ? L.list[SAMPLE_OWN * tid + e] : SAMPLE_NONE;
             const double z = on ? sample_log(sample_token(p[e]), q.m, q.scale) : 0.0;
             b[e] = on ? sample_bin(z) : -1;
             w[e] = on ? sample_mass(z, L.pow) : 0;
@@ -342,32 +350,32 @@ __device__ __forceinline__ void sample_finish(const SampleArgs &a, int row, cons
         }
         before = sample_scan(sum, L.wave, total);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
+        for (int e = 0; e < SAMPLE_OWN; e++) {
             if (first[e]) {
                 L.base[b[e]] = before;
-                L.count[b[e]] = (uint32_t)(4 * tid + e);   // the counts are in cupto
+                L.count[b[e]] = (uint32_t)(SAMPLE_OWN * tid + e);   // the counts are in cupto
             }
             before += w[e];
         }
         __syncthreads();
         before -= sum;
-        unsigned long long cum[4];   // up to and with it
+        unsigned long long cum[SAMPLE_OWN];   // up to and with it
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
+        for (int e = 0; e < SAMPLE_OWN; e++) {
             before += w[e];
             cum[e] = b[e] >= 0 ? L.upto[b[e]] + before - L.base[b[e]] : 0;
         }
         if (q.by_k) {
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (b[e] == q.bk && L.cupto[b[e]] + (4 * tid + e - L.count[b[e]]) + 1 == (uint32_t)q.k) L.found[0] = cum[e];
+            for (int e = 0; e < SAMPLE_OWN; e++)
+                if (b[e] == q.bk && L.cupto[b[e]] + (SAMPLE_OWN * tid + e - L.count[b[e]]) + 1 == (uint32_t)q.k) L.found[0] = cum[e];
             __syncthreads();
             kept = L.found[0];
         }
         if (q.by_p) {
             const unsigned long long want = sample_want(q.p, kept);
 #pragma unroll
-            for (int e = 0; e < 4; e++)
+            for (int e = 0; e < SAMPLE_OWN; e++)
                 if (cum[e] - w[e] < want && want <= cum[e]) L.found[1] = cum[e];
             __syncthreads();
             kept = L.found[1];
@@ -375,7 +383,7 @@ __device__ __forceinline__ void sample_finish(const SampleArgs &a, int row, cons
         kept = kept < q.over_min ? kept : q.over_min;
         const unsigned long long over = sample_over(q.u, kept);
 #pragma unroll
-        for (int e = 0; e < 4; e++)
+        for (int e = 0; e < SAMPLE_OWN; e++)
             if (cum[e] - w[e] <= over && over < cum[e]) L.found[2] = p[e];
         __syncthreads();
         place = L.found[2];
@@ -393,8 +401,7 @@ __device__ __forceinline__ void sample_finish(const SampleArgs &a, int row, cons
     if (tid == 0) {
         a.token[row] = (int32_t)(place & 0xFFFFF);
         if (a.prob)
-            a.prob[row] = (float)(sample_pow(sample_log(sample_token(place), q.m, q.scale), L.pow) * SAMPLE_ONE /
-                                  (double)kept);
+            a.prob[row] = (float)(sample_pow(sample_log(sample_token(place), q.m, q.scale), L.pow, 43) / (double)kept);
     }
 }
 
@@ -432,8 +439,8 @@ __device__ __forceinline__ SampleAsk sample_ask(const SampleArgs &a, int row, un
     q.k = a.top_k ? a.top_k[row] : 0;
     q.p = a.top_p ? a.top_p[row] : 1.0f;
     q.u = a.u[row];
-    q.scale = 1.4426950408889634074 / (double)(a.temperature ? a.temperature[row] : 1.0f);
-    q.over_min = 0;
+    q.scale = 256.0 * 1.4426950408889634074 / (double)(a.temperature ? a.temperature[row] : 1.0f);
+    q.over_min = ~0ull;
     return q;
 }
 // The bins of the row's tokens i0 .. i1 - 1 in L.mass and, where its k may
@@ -442,18 +449,16 @@ __device__ __forceinline__ void sample_bins(const SampleArgs &a, int row, Sample
     const int tid = (int)threadIdx.x;
     const float min_p = a.min_p && a.min_p[row] > 0.0f ? fminf(a.min_p[row], 1.0f) : 0.0f;
     const unsigned long long floor_mass = min_p > 0.0f ? (unsigned long long)__builtin_ceil((double)min_p * SAMPLE_ONE) : 0;
-    L.mass[tid] = 0;
-    L.count[tid] = 0;
     L.pow.fill();
-    __syncthreads();
+    sample_clear(L);
     unsigned long long tail = 0, over_min = 0, tails, ntails;
     uint32_t ntail = 0;
     const bool counted = q.k > 0;
-    sample_walk(q.x, i0, i1, [&](float v, int) {
+    const auto add = [&](float v, bool floor) {
         const double z = sample_log(v, q.m, q.scale);
         const int b = sample_bin(z);
         const unsigned long long w = sample_mass(z, L.pow);
-        if (w >= floor_mass) over_min += w;
+        if (floor && w >= floor_mass) over_min += w;
         if (b == SAMPLE_BINS - 1) {   // many of a row's tokens: not one by one to the same bin
             tail += w;
             ntail++;
@@ -461,13 +466,15 @@ __device__ __forceinline__ void sample_bins(const SampleArgs &a, int row, Sample
             atomicAdd(&L.mass[b], w);
             if (counted) atomicAdd(&L.count[b], 1u);
         }
-    });
+    };
+    if (floor_mass) sample_walk(q.x, i0, i1, [&](float v, int) { add(v, true); });
+    else sample_walk(q.x, i0, i1, [&](float v, int) { add(v, false); });
     sample_scan(tail, L.wave, tails);
     sample_scan(ntail, L.wave, ntails);
-    sample_scan(over_min, L.wave, q.over_min);
-    if (tid == SAMPLE_BINS - 1) {
-        L.mass[tid] = tails;
-        L.count[tid] = (uint32_t)ntails;
+    if (floor_mass) sample_scan(over_min, L.wave, q.over_min);
+    if (tid == 0) {
+        L.mass[SAMPLE_BINS - 1] = tails;
+        L.count[SAMPLE_BINS - 1] = (uint32_t)ntails;
     }
     __syncthreads();
 }
@@ -475,7 +482,7 @@ __device__ __forceinline__ void sample_bins(const SampleArgs &a, int row, Sample
 // Grid (chunks, rows): the chunk's first token of the order; the row's counters
 // cleared.
 extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_max(SampleArgs a) {
-    __shared__ unsigned long long wave[16];
+    __shared__ unsigned long long wave[SAMPLE_WAVES];
     const int c = (int)blockIdx.x, row = (int)blockIdx.y;
     const unsigned long long best =
         sample_best(a.logits + (int64_t)row * a.stride, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), wave);
@@ -493,8 +500,10 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_bins(Sample
     SampleAsk q = sample_ask(a, row, best);
     sample_bins(a, row, q, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), L);
     SampleChunk *o = a.bins + (int64_t)row * a.chunks + c;
-    o->mass[tid] = L.mass[tid];
-    if (q.k > 0) o->count[tid] = L.count[tid];
+    for (int b = tid; b < SAMPLE_BINS; b += SAMPLE_NT) {
+        o->mass[b] = L.mass[b];
+        if (q.k > 0) o->count[b] = L.count[b];
+    }
     if (tid == 0) o->over_min = q.over_min;
 }
 
@@ -506,15 +515,38 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_pick(Sample
     if (sample_done(a, row, best, false)) return;
     SampleAsk q = sample_ask(a, row, best);
     const SampleChunk *o = a.bins + (int64_t)row * a.chunks;
-    unsigned long long mass = 0;
-    uint32_t count = 0;
-    for (int i = 0; i < a.chunks; i++) {
-        mass += o[i].mass[tid];
-        if (q.k > 0) count += o[i].count[tid];
-        q.over_min += o[i].over_min;
+    unsigned long long mass[2] = {0, 0}, over_min = 0;
+    uint32_t count[2] = {0, 0};
+    for (int i = 0; i < a.chunks; i += 4) {   // four chunks' loads in flight
+        unsigned long long m[4][2], f[4];
+        uint32_t n[4][2];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const SampleChunk &h = o[min(i + j, a.chunks - 1)];
+            f[j] = h.over_min;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                m[j][e] = h.mass[tid + e * SAMPLE_NT];
+                n[j][e] = q.k > 0 ? h.count[tid + e * SAMPLE_NT] : 0;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (i + j >= a.chunks) break;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                mass[e] += m[j][e];
+                count[e] += n[j][e];
+            }
+            over_min = f[j] == ~0ull ? f[j] : over_min + f[j];
+        }
     }
-    L.mass[tid] = mass;
-    L.count[tid] = count;
+    q.over_min = over_min;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        L.mass[tid + e * SAMPLE_NT] = mass[e];
+        L.count[tid + e * SAMPLE_NT] = count[e];
+    }
     L.pow.fill();
     const float least = sample_bounds(q, L);
     sample_gather(q, least, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), L);

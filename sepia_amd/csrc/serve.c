@@ -224,6 +224,7 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
 #define SAMPLE_ROW_BYTES (4096 * 8 + 8)
 #define SAMPLE_CHUNK_BYTES (1024 * 12 + 16)
 #define SAMPLE_CHUNKS 16    /* chunks of a row at most */
+#define SAMPLE_NT 512
 #define SAMPLE_CHUNK 8192   /* logits of a chunk at least */
 #define SAMPLE_PLACES 512   /* workgroups that the chip holds, two a CU */
 typedef struct {
@@ -291,11 +292,11 @@ int sepia_hip_sample(const SepiaSampleDesc *d, SepiaGpuBuf *logits, int64_t rows
     a.chunks = (int32_t)chunks;
     a.chunk = (int32_t)((vocab + chunks - 1) / chunks);
     void *args[] = { &a };
-    if (chunks == 1) return sepia_serve_launch(SK_SAMPLE, 1, (unsigned)rows, 1, 1024, args, op);
+    if (chunks == 1) return sepia_serve_launch(SK_SAMPLE, 1, (unsigned)rows, 1, SAMPLE_NT, args, op);
     a.rows = (uint8_t *)sepia_scratch((size_t)rows * per, op);
     if (!a.rows) return 0;
     a.bins = a.rows + (size_t)rows * SAMPLE_ROW_BYTES;
     for (int k = SK_SAMPLE_MAX; k <= SK_SAMPLE_PICK; k++)
-        if (!sepia_serve_launch(k, (unsigned)chunks, (unsigned)rows, 1, 1024, args, op)) return 0;
+        if (!sepia_serve_launch(k, (unsigned)chunks, (unsigned)rows, 1, SAMPLE_NT, args, op)) return 0;
     return 1;
 }
