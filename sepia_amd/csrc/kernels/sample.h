@@ -18,9 +18,13 @@
 // row counts and sums the tokens by their weight's logarithm (1024 bins, 32 to
 // the octave). The bins' prefix sums then bound where the k-th token, the
 // top-p border and the draw fall: each decision's bound gives the next one's,
-// a bin or a few in all. A second pass gathers the tokens of those bins, whose
-// exact order gives the three in turn. Where they are too many (flat rows,
-// long runs of equal logits) each decision is found by its digits instead.
+// a bin or a few in all. A second pass gathers the tokens of those bins, and
+// the three are decided in turn: a decision's bin is cut into 1024 pieces by
+// place in the order, its piece again while it has more than 64 tokens (equal
+// logits: by index), and those few are compared with each other. Where the
+// gathered tokens are too many (flat rows, long runs of equal logits) the same
+// is done with passes over the row. (Sorting the gathered tokens by a network
+// took 10 us for 250 of them and 25 us for 1100.)
 //
 // A row is cut into chunks where the rows are fewer than the chip's places,
 // and the passes become launches: each chunk's first token of the order (the
@@ -36,8 +40,7 @@
 #define SAMPLE_NT 512                 // two workgroups a CU (of 1024 threads one: 36 against 26 us at 48 rows)
 #define SAMPLE_WAVES (SAMPLE_NT / 64)
 #define SAMPLE_BINS 1024              // two a thread
-#define SAMPLE_CAP 4096               // gathered tokens: eight a thread
-#define SAMPLE_OWN (SAMPLE_CAP / SAMPLE_NT)
+#define SAMPLE_CAP 4096               // gathered tokens
 
 // In scratch where a row has several chunks: a chunk's bins, and what the
 // row's workgroups gather.
@@ -117,10 +120,11 @@ __device__ __forceinline__ unsigned long long sample_mass(double z, const Sample
 }
 
 struct SampleLds {
-    unsigned long long mass[SAMPLE_BINS], upto[SAMPLE_BINS + 1];   // sums by bin; of the bins before
-    uint32_t count[SAMPLE_BINS], cupto[SAMPLE_BINS + 1];
-    unsigned long long list[SAMPLE_CAP], base[SAMPLE_BINS];
-    unsigned long long wave[SAMPLE_WAVES], set[SAMPLE_BINS / 64], found[3];
+    // by bin, then by a bin's pieces; of the bins before
+    unsigned long long mass[SAMPLE_BINS + 1], upto[SAMPLE_BINS + 1];
+    uint32_t count[SAMPLE_BINS + 1], cupto[SAMPLE_BINS + 1];
+    unsigned long long list[SAMPLE_CAP], few[64];
+    unsigned long long wave[SAMPLE_WAVES], set[SAMPLE_BINS / 64];
     uint32_t n;
     SamplePow pow;
 };
@@ -182,58 +186,32 @@ __device__ __forceinline__ void sample_clear(SampleLds &L) {
     for (int i = (int)threadIdx.x; i < SAMPLE_BINS; i += SAMPLE_NT) L.mass[i] = 0, L.count[i] = 0;
     __syncthreads();
 }
-// Bins' prefix sums from L.mass and L.count.
-__device__ __forceinline__ void sample_prefix(SampleLds &L) {
+// Prefix sums of L.mass and L.count, to `upto` and `cupto` (which may be the
+// same arrays).
+__device__ __forceinline__ void sample_prefix(SampleLds &L, unsigned long long *upto, uint32_t *cupto) {
     const int b = 2 * (int)threadIdx.x;
     unsigned long long total;
     __syncthreads();
-    const unsigned long long m = sample_scan(L.mass[b] + L.mass[b + 1], L.wave, total);
-    L.upto[b] = m;
-    L.upto[b + 1] = m + L.mass[b];
-    if (b == 0) L.upto[SAMPLE_BINS] = total;
-    const unsigned long long c = sample_scan((unsigned long long)L.count[b] + L.count[b + 1], L.wave, total);
-    L.cupto[b] = (uint32_t)c;
-    L.cupto[b + 1] = (uint32_t)c + L.count[b];
-    if (b == 0) L.cupto[SAMPLE_BINS] = (uint32_t)total;
+    const unsigned long long m0 = L.mass[b], c0 = L.count[b];
+    const unsigned long long m = sample_scan(m0 + L.mass[b + 1], L.wave, total);
+    upto[b] = m;
+    upto[b + 1] = m + m0;
+    if (b == 0) upto[SAMPLE_BINS] = total;
+    const unsigned long long c = sample_scan(c0 + L.count[b + 1], L.wave, total);
+    cupto[b] = (uint32_t)c;
+    cupto[b + 1] = (uint32_t)(c + c0);
+    if (b == 0) cupto[SAMPLE_BINS] = (uint32_t)total;
     __syncthreads();
 }
 // The bin with upto[b] <= over < upto[b + 1] (cupto with by_count), by every
 // wave for itself: 64 bins apart, then 16 of them.
-__device__ __forceinline__ int sample_seek(const SampleLds &L, bool by_count, unsigned long long over) {
+__device__ __forceinline__ int sample_seek(const unsigned long long *upto, const uint32_t *cupto, bool by_count,
+                                           unsigned long long over) {
     const int lane = (int)threadIdx.x & 63;
-    const uint64_t far = __ballot((by_count ? L.cupto[16 * lane] : L.upto[16 * lane]) <= over);
+    const uint64_t far = __ballot((by_count ? cupto[16 * lane] : upto[16 * lane]) <= over);
     const int b = 16 * (63 - __builtin_clzll(far)) + (lane & 15);
-    const uint64_t near = __ballot((by_count ? L.cupto[b] : L.upto[b]) <= over) & 0xFFFF;
+    const uint64_t near = __ballot((by_count ? cupto[b] : upto[b]) <= over) & 0xFFFF;
     return 16 * (63 - __builtin_clzll(far)) + 31 - __builtin_clz((uint32_t)near);
-}
-
-// The first token of the order whose cumulative weight (by_count: place from
-// 1) exceeds `over`, and the weight up to and with it, by the order's digits:
-// a pass over the row settles ten bits of the place.
-struct SampleAt {
-    unsigned long long place, cum;
-};
-__device__ __forceinline__ SampleAt sample_find(const float *x, int vocab, float m, double scale, bool by_count,
-                                                unsigned long long over, SampleLds &L) {
-    unsigned long long prefix = 0, mass = 0, last = 0;
-    for (int left = 50; left >= 0; left -= 10) {   // 62 bits hold the 52 of a place
-        sample_clear(L);
-        sample_walk(x, 0, vocab, [&](float v, int i) {
-            const unsigned long long at = sample_place(v, i);
-            if (at >> left >> 10 != prefix) return;
-            const int b = (int)(at >> left) & 1023;
-            atomicAdd(&L.count[b], 1u);
-            atomicAdd(&L.mass[b], sample_mass(sample_log(v, m, scale), L.pow));
-        });
-        sample_prefix(L);
-        const int b = sample_seek(L, by_count, over);
-        over -= by_count ? L.cupto[b] : L.upto[b];
-        mass += L.upto[b];
-        last = L.mass[b];
-        prefix = prefix << 10 | (unsigned)b;
-        __syncthreads();
-    }
-    return SampleAt{prefix, mass + last};
 }
 
 // What a row asks for, as its workgroups need it.
@@ -244,7 +222,6 @@ struct SampleAsk {
     double scale;
     unsigned long long over_min;   // the weight of its tokens of w >= min-p (no min-p: the largest number)
     bool by_k, by_p;
-    int bk;                        // the bin of its k-th token
 };
 __device__ __forceinline__ unsigned long long sample_share(float f, unsigned long long total) {
     return (unsigned long long)((double)f * (double)total);
@@ -258,45 +235,52 @@ __device__ __forceinline__ unsigned long long sample_over(float u, unsigned long
     const unsigned long long over = u > 0.0f ? sample_share(fminf(u, 1.0f), kept) : 0;
     return over >= kept ? kept ? kept - 1 : 0 : over;
 }
+// A logit that no token of bin b lies below, and one that none lies above.
+__device__ __forceinline__ float sample_least(const SampleAsk &q, int b) {
+    if (b == SAMPLE_BINS - 1) return -INFINITY;
+    if (q.m == INFINITY) return q.m;   // all other tokens are in the last bin
+    const double x = (double)q.m - (double)(8 * b + 9) / q.scale;
+    return (float)(x - (fabs(x) + fabs((double)q.m)) * 0x1p-20);   // rounded down, surely
+}
+__device__ __forceinline__ float sample_most(const SampleAsk &q, int b) {
+    if (b == 0 || q.m == INFINITY) return q.m;
+    const double x = (double)q.m - (double)(8 * b - 1) / q.scale;
+    return fminf(q.m, (float)(x + (fabs(x) + fabs((double)q.m)) * 0x1p-20));
+}
 // From the row's bins in L.mass (and L.count, if its k may cut): their prefix
 // sums, and in L.set the bins that decide. Returns the least logit of those.
 __device__ __forceinline__ float sample_bounds(SampleAsk &q, SampleLds &L) {
     const int tid = (int)threadIdx.x;
-    sample_prefix(L);
+    sample_prefix(L, L.upto, L.cupto);
     const unsigned long long all = L.upto[SAMPLE_BINS];
     q.by_k = q.k > 0 && (uint32_t)q.k < L.cupto[SAMPLE_BINS];
     q.by_p = q.p < 1.0f;
-    q.bk = -1;
     // each decision's bin, or the range of bins that the one before leaves it
     unsigned long long lo = all, hi = all;   // the weight kept so far is in [lo, hi]
-    int p0 = 0, p1 = -1;
+    int bk = -1, p0 = 0, p1 = -1;
     if (q.by_k) {
-        q.bk = sample_seek(L, true, (unsigned long long)q.k - 1);
-        lo = L.upto[q.bk];
-        hi = L.upto[q.bk + 1];
+        bk = sample_seek(L.upto, L.cupto, true, (unsigned long long)q.k - 1);
+        lo = L.upto[bk];
+        hi = L.upto[bk + 1];
     }
     if (q.by_p) {
         const unsigned long long w0 = sample_want(q.p, lo), w1 = sample_want(q.p, hi);
-        p0 = sample_seek(L, false, w0 - 1);
-        p1 = w0 == w1 ? p0 : sample_seek(L, false, w1 - 1);
+        p0 = sample_seek(L.upto, L.cupto, false, w0 - 1);
+        p1 = w0 == w1 ? p0 : sample_seek(L.upto, L.cupto, false, w1 - 1);
         lo = w0;
         hi = L.upto[p1 + 1];
     }
     lo = lo < q.over_min ? lo : q.over_min;
     hi = hi < q.over_min ? hi : q.over_min;
-    const int d0 = sample_seek(L, false, sample_over(q.u, lo));
-    const int d1 = lo == hi ? d0 : sample_seek(L, false, sample_over(q.u, hi));
+    const int d0 = sample_seek(L.upto, L.cupto, false, sample_over(q.u, lo));
+    const int d1 = lo == hi ? d0 : sample_seek(L.upto, L.cupto, false, sample_over(q.u, hi));
     for (int b = tid; b < SAMPLE_BINS; b += SAMPLE_NT) {
-        const unsigned long long word = __ballot(b == q.bk || (b >= p0 && b <= p1) || (b >= d0 && b <= d1));
+        const unsigned long long word = __ballot(b == bk || (b >= p0 && b <= p1) || (b >= d0 && b <= d1));
         if ((tid & 63) == 0) L.set[b >> 6] = word;
     }
-    const int last = max(max(q.bk, p1), d1);
     if (tid == 0) L.n = 0;
     __syncthreads();
-    if (last == SAMPLE_BINS - 1) return -INFINITY;
-    if (q.m == INFINITY) return q.m;   // all other tokens are in the last bin
-    const double least = (double)q.m - (double)(8 * last + 9) / q.scale;
-    return (float)(least - (fabs(least) + fabs((double)q.m)) * 0x1p-20);   // rounded down, surely
+    return sample_least(q, max(max(bk, p1), d1));
 }
 // The chosen bins' tokens among the row's i0 .. i1 - 1 into L.list; L.n counts
 // them, also where they are more than the list holds.
@@ -310,95 +294,87 @@ __device__ __forceinline__ void sample_gather(const SampleAsk &q, float least, i
     });
     __syncthreads();
 }
-// The decision from the n gathered tokens in L.list.
-__device__ __forceinline__ void sample_finish(const SampleArgs &a, int row, const SampleAsk &q, uint32_t n, SampleLds &L) {
-    const int tid = (int)threadIdx.x;
-    unsigned long long kept = L.upto[SAMPLE_BINS], place;
-    if (n <= SAMPLE_CAP) {
-        int size = 2;
-        while (size < (int)n) size <<= 1;
-        for (int i = (int)n + tid; i < size; i += SAMPLE_NT) L.list[i] = SAMPLE_NONE;
-        for (int k = 2; k <= size; k <<= 1)
-            for (int j = k >> 1; j; j >>= 1) {
-                __syncthreads();
-                for (int h = tid; h < size / 2; h += SAMPLE_NT) {
-                    const int i = 2 * h - (h & (j - 1)), o = i + j;
-                    const unsigned long long s = L.list[i], t = L.list[o];
-                    if ((s > t) == !(i & k)) {
-                        L.list[i] = t;
-                        L.list[o] = s;
-                    }
-                }
+// The first token of bin b whose cumulative weight from the bin's start
+// (by_count: place from 1) exceeds `over`, and the weight up to and with it,
+// among the n gathered tokens (listed) or the whole row's.
+struct SampleAt {
+    unsigned long long place, cum;
+};
+__device__ __forceinline__ SampleAt sample_settle(const SampleAsk &q, int b, bool by_count, unsigned long long over,
+                                                  bool listed, uint32_t n, SampleLds &L) {
+    const int lane = (int)threadIdx.x & 63;
+    const auto walk = [&](auto f) {
+        if (listed) {
+            for (uint32_t i = threadIdx.x; i < n; i += SAMPLE_NT) {
+                const unsigned long long p = L.list[i];
+                const double z = sample_log(sample_token(p), q.m, q.scale);
+                if (sample_bin(z) == b) f(p, z);
             }
+        } else {
+            sample_walk(q.x, 0, q.vocab, [&](float v, int i) {
+                const double z = sample_log(v, q.m, q.scale);
+                if (sample_bin(z) == b) f(sample_place(v, i), z);
+            });
+        }
+    };
+    // the places from `first` on, 2^bits of them
+    unsigned long long first = (unsigned long long)sample_key(sample_most(q, b)) << 20, before = 0;
+    const unsigned long long last = ((unsigned long long)sample_key(fmaxf(sample_least(q, b), -3.402823466e38f)) << 20) | 0xFFFFF;
+    int bits = 64 - __builtin_clzll((last - first) | 1);
+    uint32_t left = listed ? n : q.by_k ? L.cupto[b + 1] - L.cupto[b] : ~0u;   // at most (bins are counted for a k)
+    while (left > 64) {
+        const int drop = max(bits - 10, 0);
+        sample_clear(L);
+        walk([&](unsigned long long p, double z) {
+            const unsigned long long piece = (p - first) >> drop;
+            if (piece >= SAMPLE_BINS) return;
+            atomicAdd(&L.count[piece], 1u);
+            atomicAdd(&L.mass[piece], sample_mass(z, L.pow));
+        });
+        sample_prefix(L, L.mass, L.count);
+        const int piece = sample_seek(L.mass, L.count, by_count, over);
+        over -= by_count ? L.count[piece] : L.mass[piece];
+        before += L.mass[piece];
+        left = L.count[piece + 1] - L.count[piece];
+        first += (unsigned long long)piece << drop;
+        bits = drop;
         __syncthreads();
-        // some tokens a thread, in order: weights, and the weight before each,
-        // of the bins before its own and then within it
-        unsigned long long p[SAMPLE_OWN], w[SAMPLE_OWN], before, total, sum = 0;
-        int b[SAMPLE_OWN];
-        bool first[SAMPLE_OWN];
-        int prev = tid > 0 && SAMPLE_OWN * tid < (int)n ? sample_bin(sample_log(sample_token(L.list[SAMPLE_OWN * tid - 1]), q.m, q.scale)) : -1;
-#pragma unroll
-        for (int e = 0; e < SAMPLE_OWN; e++) {
-            const bool on = SAMPLE_OWN * tid + e < (int)n;
-            p[e] = on ? L.list[SAMPLE_OWN * tid + e] : SAMPLE_NONE;
-            const double z = on ? sample_log(sample_token(p[e]), q.m, q.scale) : 0.0;
-            b[e] = on ? sample_bin(z) : -1;
-            w[e] = on ? sample_mass(z, L.pow) : 0;
-            first[e] = on && b[e] != prev;
-            prev = b[e];
-            sum += w[e];
-        }
-        before = sample_scan(sum, L.wave, total);
-#pragma unroll
-        for (int e = 0; e < SAMPLE_OWN; e++) {
-            if (first[e]) {
-                L.base[b[e]] = before;
-                L.count[b[e]] = (uint32_t)(SAMPLE_OWN * tid + e);   // the counts are in cupto
-            }
-            before += w[e];
-        }
-        __syncthreads();
-        before -= sum;
-        unsigned long long cum[SAMPLE_OWN];   // up to and with it
-#pragma unroll
-        for (int e = 0; e < SAMPLE_OWN; e++) {
-            before += w[e];
-            cum[e] = b[e] >= 0 ? L.upto[b[e]] + before - L.base[b[e]] : 0;
-        }
-        if (q.by_k) {
-#pragma unroll
-            for (int e = 0; e < SAMPLE_OWN; e++)
-                if (b[e] == q.bk && L.cupto[b[e]] + (SAMPLE_OWN * tid + e - L.count[b[e]]) + 1 == (uint32_t)q.k) L.found[0] = cum[e];
-            __syncthreads();
-            kept = L.found[0];
-        }
-        if (q.by_p) {
-            const unsigned long long want = sample_want(q.p, kept);
-#pragma unroll
-            for (int e = 0; e < SAMPLE_OWN; e++)
-                if (cum[e] - w[e] < want && want <= cum[e]) L.found[1] = cum[e];
-            __syncthreads();
-            kept = L.found[1];
-        }
-        kept = kept < q.over_min ? kept : q.over_min;
-        const unsigned long long over = sample_over(q.u, kept);
-#pragma unroll
-        for (int e = 0; e < SAMPLE_OWN; e++)
-            if (cum[e] - w[e] <= over && over < cum[e]) L.found[2] = p[e];
-        __syncthreads();
-        place = L.found[2];
-    } else {
-        for (int step = q.by_k ? 0 : q.by_p ? 1 : 2;; step = step == 0 && q.by_p ? 1 : 2) {   // top-k, top-p, the draw
-            if (step == 2 && kept > q.over_min) kept = q.over_min;
-            const unsigned long long over = step == 0 ? (unsigned long long)q.k - 1
-                                            : step == 1 ? sample_want(q.p, kept) - 1 : sample_over(q.u, kept);
-            const SampleAt r = sample_find(q.x, q.vocab, q.m, q.scale, step == 0, over, L);
-            place = r.place;
-            if (step == 2) break;
-            kept = r.cum;
-        }
     }
-    if (tid == 0) {
+    // at most 64 tokens: every wave compares them with each other
+    if (threadIdx.x == 0) L.n = 0;
+    __syncthreads();
+    walk([&](unsigned long long p, double) {
+        if ((p - first) >> bits == 0) L.few[atomicAdd(&L.n, 1u)] = p;
+    });
+    __syncthreads();
+    const int m = (int)L.n;
+    const unsigned long long p = lane < m ? L.few[lane] : SAMPLE_NONE;
+    const unsigned long long w = lane < m ? sample_mass(sample_log(sample_token(p), q.m, q.scale), L.pow) : 0;
+    unsigned long long cum = w, place = 1;
+    for (int j = 0; j < m; j++) {
+        const unsigned long long pj = __shfl(p, j, 64), wj = __shfl(w, j, 64);
+        cum += pj < p ? wj : 0;
+        place += pj < p;
+    }
+    const uint64_t hit = __ballot(lane < m && (by_count ? place == over + 1 : cum - w <= over && over < cum));
+    const int l = hit ? __builtin_ctzll(hit) : 0;
+    __syncthreads();
+    return SampleAt{(unsigned long long)__shfl(p, l, 64), before + __shfl(cum, l, 64)};
+}
+// The decisions, from the gathered tokens where they fit L.list: the k-th
+// token, the top-p border, the draw.
+__device__ __forceinline__ void sample_finish(const SampleArgs &a, int row, const SampleAsk &q, uint32_t n, SampleLds &L) {
+    unsigned long long kept = L.upto[SAMPLE_BINS], place = 0;
+    for (int step = q.by_k ? 0 : q.by_p ? 1 : 2; step <= 2; step = step == 0 && q.by_p ? 1 : step == 2 ? 3 : 2) {
+        if (step == 2 && kept > q.over_min) kept = q.over_min;
+        const unsigned long long over = step == 0 ? (unsigned long long)q.k - 1
+                                        : step == 1 ? sample_want(q.p, kept) - 1 : sample_over(q.u, kept);
+        const int b = sample_seek(L.upto, L.cupto, step == 0, over);
+        const SampleAt r = sample_settle(q, b, step == 0, over - (step == 0 ? L.cupto[b] : L.upto[b]), n <= SAMPLE_CAP, n, L);
+        if (step == 2) place = r.place;
+        else kept = L.upto[b] + r.cum;
+    }
+    if (threadIdx.x == 0) {
         a.token[row] = (int32_t)(place & 0xFFFFF);
         if (a.prob)
             a.prob[row] = (float)(sample_pow(sample_log(sample_token(place), q.m, q.scale), L.pow, 43) / (double)kept);
