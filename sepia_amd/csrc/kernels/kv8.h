@@ -41,21 +41,6 @@ struct Kv8Args {
     }
 };
 
-// The sequence that owns `id` (-1: none): 64 sequences a look, so one round
-// for up to 64 of them and two for 4096.
-__device__ __forceinline__ int kv8_find(const Kv8Args &a, int64_t id, int gran, int extra) {
-    const int lane = (int)(threadIdx.x & 63);
-    int lo = 0, n = a.n_seqs;
-    while (true) {
-        const int step = (n + 63) / 64, i = lane * step;
-        const bool le = i < n && kv8_first_id(a.starts[lo + (i < n ? i : 0)], lo + i, gran, extra) <= id;
-        const int c = __builtin_popcountll(__ballot(le));
-        if (c == 0) return -1;
-        lo += (c - 1) * step;
-        n = min(step, n - (c - 1) * step);
-        if (step == 1) return lo;
-    }
-}
 // That sequence's length and rows; 0 where they cannot be used.
 __device__ __forceinline__ int kv8_seq(const Kv8Args &a, int s, int32_t &len, int32_t &r0, int32_t &r1) {
     len = a.lens[s];
@@ -63,10 +48,34 @@ __device__ __forceinline__ int kv8_seq(const Kv8Args &a, int s, int32_t &len, in
     r1 = a.starts[s + 1];
     return kv8_seq_ok(len, r0, r1, a.n, (int64_t)a.max_pages << a.lg);
 }
-// The grid's first workgroup reports sequences that cannot be used (others
-// pass them over, or, where starts fall, may not find them at all).
+// The sequence that owns `id`, its length and rows; -1 if there is none, or
+// one that cannot be used. 64 sequences a look: one round for up to 64 of
+// them, with everything about the one found already loaded, two for 4096.
+__device__ __forceinline__ int kv8_find(const Kv8Args &a, int64_t id, int gran, int extra, int32_t &len, int32_t &r0, int32_t &r1) {
+    const int lane = (int)(threadIdx.x & 63);
+    int lo = 0, n = a.n_seqs;
+    while (true) {
+        const int step = (n + 63) / 64, i = lane * step, s = lo + min(i, n - 1);
+        r0 = a.starts[s];
+        r1 = a.starts[s + 1];
+        len = a.lens[s];
+        const int c = __builtin_popcountll(__ballot(i < n && kv8_first_id(r0, s, gran, extra) <= id));
+        if (c == 0) return -1;
+        if (step == 1) {
+            r0 = __builtin_amdgcn_readlane(r0, c - 1);
+            r1 = __builtin_amdgcn_readlane(r1, c - 1);
+            len = __builtin_amdgcn_readlane(len, c - 1);
+            return kv8_seq_ok(len, r0, r1, a.n, (int64_t)a.max_pages << a.lg) ? lo + c - 1 : -1;
+        }
+        lo += (c - 1) * step;
+        n = min(step, n - (c - 1) * step);
+    }
+}
+// The grid's last workgroup reports sequences that cannot be used (others
+// pass them over, or, where starts fall, may not find them at all). It is the
+// last since that seldom has anything else to do.
 __device__ __forceinline__ void kv8_check(const Kv8Args &a) {
-    if (blockIdx.x | blockIdx.y | blockIdx.z) return;
+    if (blockIdx.x + 1 != gridDim.x || blockIdx.y || blockIdx.z) return;
     bool bad = false;
     int32_t len, r0, r1;
     for (int s = (int)threadIdx.x; s < a.n_seqs; s += (int)blockDim.x) bad |= !kv8_seq(a, s, len, r0, r1);
@@ -117,15 +126,15 @@ __device__ __forceinline__ Kv8Scale kv8_rescale(float *scale, bool fresh, float 
 
 // Grid (ids, Hkv, 2: K and V), a wave for each 16 tokens of a page; gran = P,
 // extra = 2.
-extern "C" __global__ __launch_bounds__(256) void sepia_kv8_append(Kv8Args a, const float *__restrict__ k,
+extern "C" __global__ __launch_bounds__(256, 4) void sepia_kv8_append(Kv8Args a, const float *__restrict__ k,
                                                                    const float *__restrict__ v,
                                                                    const float *__restrict__ norm, float eps) {
     const int hk = (int)blockIdx.y, lane = (int)(threadIdx.x & 63), slot0 = (int)(threadIdx.x >> 6) * 16;
     kv8_check(a);
-    const int s = kv8_find(a, blockIdx.x, a.P(), 2);
     int32_t len, r0, r1;
+    const int s = kv8_find(a, blockIdx.x, a.P(), 2, len, r0, r1);
     Kv8Unit u;
-    if (s < 0 || !kv8_seq(a, s, len, r0, r1)) return;
+    if (s < 0) return;
     if (!kv8_unit(len, r0, r1, (int)(blockIdx.x - kv8_first_id(r0, s, a.P(), 2)), a.lg, &u)) return;
     const int64_t page = kv8_page(a, s, u.page);
     if (page < 0) {
@@ -241,10 +250,10 @@ extern "C" __global__ __launch_bounds__(256) void sepia_kv8_read(Kv8Args a, floa
                                                                  float *__restrict__ v) {
     const int hk = (int)blockIdx.y, lane = (int)(threadIdx.x & 63), slot0 = (int)(threadIdx.x >> 6) * 16;
     kv8_check(a);
-    const int s = kv8_find(a, blockIdx.x, a.P(), 2);
     int32_t len, r0, r1;
+    const int s = kv8_find(a, blockIdx.x, a.P(), 2, len, r0, r1);
     Kv8Unit u;
-    if (s < 0 || !kv8_seq(a, s, len, r0, r1)) return;
+    if (s < 0) return;
     if (!kv8_unit(len, r0, r1, (int)(blockIdx.x - kv8_first_id(r0, s, a.P(), 2)), a.lg, &u)) return;
     const int64_t page = kv8_page(a, s, u.page);
     if (page < 0) {

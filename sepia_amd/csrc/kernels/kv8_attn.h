@@ -39,6 +39,7 @@ struct Kv8Attn {
 
 typedef int32_t kv8_i4 __attribute__((ext_vector_type(4)));
 typedef float kv8_f4 __attribute__((ext_vector_type(4)));
+typedef kv8_f4 kv8_f4u __attribute__((aligned(4)));
 
 // Over the four lane groups (lanes n, n + 16, n + 32, n + 48).
 __device__ __forceinline__ float kv8_max_g(float v) {
@@ -149,7 +150,8 @@ struct Kv8Wave {
     kv8_f4 O[8];
     float m, l, qs, tau;    // row n's maximum; this lane's part of its sum; q's scale times c
     int32_t lo, pos;        // row n's columns (inactive: none)
-    const float *rel;       // row n's rel_logits at distance pos, so that column col's is rel[-col]
+    const float *rel;       // row n's rel_logits
+    int32_t rpos;           // pos, for an inactive row some active one's
     int32_t lo_max, pos_min;   // over the active rows
 
     __device__ __forceinline__ void init(const Kv8Args &a, const Kv8Attn &b, const Kv8Tile &t, int row0, int hk) {
@@ -195,7 +197,8 @@ struct Kv8Wave {
         pos = on ? t.pos0 + ti : -1;
         lo = on ? (b.window > 0 ? max(0, pos - b.window + 1) : 0) : 0x7FFFFFFF;
         tau = b.tau ? b.tau[t.t0 + (on ? ti : 0)] : 1.0f;
-        rel = b.rel ? b.rel + th * b.R + (on ? pos : t.pos0) : nullptr;
+        rel = b.rel ? b.rel + th * b.R : nullptr;
+        rpos = on ? pos : t.pos0;
         lo_max = b.window > 0 ? max(0, t.last - b.window + 1) : 0;
         pos_min = t.pos0;
         m = -INFINITY;
@@ -204,17 +207,22 @@ struct Kv8Wave {
         for (int i = 0; i < 8; i++) O[i] = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // The pages of a step: of this lane's K row and of its columns 16 g .. .
-    // Columns outside [lo, last] of the tile take the nearest page inside.
-    static __device__ __forceinline__ void pages(const Kv8Args &a, const Kv8Plan &p, const Kv8Tile &t, int step, int64_t &pk,
-                                                 int64_t &pv) {
+    // The table's entries for a step: of this lane's K row and of its columns
+    // 16 g .. . Columns outside [lo, last] of the tile take the nearest page
+    // inside. page() checks one when it is used, so that it is not waited for
+    // where it is loaded.
+    static __device__ __forceinline__ void entries(const Kv8Args &a, const Kv8Plan &p, const Kv8Tile &t, int step, int32_t &ek,
+                                                   int32_t &ev) {
         const int lane = (int)(threadIdx.x & 63), first = t.lo >> a.lg, end = t.last >> a.lg;
         const int ik = (64 * step + 16 * ((lane & 15) >> 2)) >> a.lg, iv = (64 * step + 16 * (lane >> 4)) >> a.lg;
-        pk = kv8_page(a, p.s, max(first, min(end, ik)));
-        pv = kv8_page(a, p.s, max(first, min(end, iv)));
-        if (__ballot(pk < 0 || pv < 0)) sepia_report_error(nullptr, KV8_ERR_PAGE, lane);
-        pk = max(pk, (int64_t)0);
-        pv = max(pv, (int64_t)0);
+        const int32_t *row = a.table + (int64_t)p.s * a.max_pages;
+        ek = row[max(first, min(end, ik))];
+        ev = row[max(first, min(end, iv))];
+    }
+    static __device__ __forceinline__ int64_t page(const Kv8Args &a, int32_t entry) {
+        const bool bad = (uint32_t)entry >= (uint64_t)a.n_pages;
+        if (__ballot(bad)) sepia_report_error(nullptr, KV8_ERR_PAGE, (int)(threadIdx.x & 63));
+        return bad ? 0 : entry;
     }
     // K operand [t][ks]: column 16 (n >> 2) + 4 t + (n & 3), dims 64 ks + 16 g.
     static __device__ __forceinline__ void load_k(const Kv8Args &a, int64_t page, int hk, int step, kv8_i4 (&K)[4][2]) {
@@ -234,6 +242,26 @@ struct Kv8Wave {
 #pragma unroll
         for (int ct = 0; ct < 8; ct++) V[ct] = *(const kv8_i4 *)(v + ((int64_t)(FULL || 16 * ct < a.Dh ? 16 * ct : 0) << a.lg));
     }
+    // rel_logits of row n and column 16 g + j of a step in r[15 - j], where the
+    // row sees the column and its band reaches it. 0: no such column in the
+    // step, 1: all are, 2: some are not. (A branch and a load a column, waited
+    // for one after the other, were most of a step: 5.5 us.)
+    __device__ __forceinline__ int load_rel(const Kv8Attn &b, int step, float (&r)[16]) const {
+        const int d0 = rpos - (64 * step + 16 * ((int)(threadIdx.x & 63) >> 4));
+        if (!b.rel || pos_min - (64 * step + 63) >= b.R) return 0;
+        if (__ballot(d0 < 15 || d0 >= b.R) == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const kv8_f4 x = *(const kv8_f4u *)(rel + (d0 - 15 + 4 * i));
+#pragma unroll
+                for (int e = 0; e < 4; e++) r[4 * i + e] = x[e];
+            }
+            return 1;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++) r[15 - j] = rel[max(0, min(b.R - 1, d0 - j))];
+        return 2;
+    }
     // Scores' digit sums of a step.
     __device__ __forceinline__ void dots(const kv8_i4 (&K)[4][2], float (&s)[16]) const {
 #pragma unroll
@@ -251,17 +279,18 @@ struct Kv8Wave {
     // The step's softmax and weighted v; ks, vs: the scales of the page of
     // columns 16 g .. .
     __device__ __forceinline__ void step(const Kv8Args &a, const Kv8Attn &b, int step, float (&s)[16], float ks, float vs,
-                                         const kv8_i4 (&V)[8]) {
+                                         int near, float (&r)[16], const kv8_i4 (&V)[8]) {
         const int g = (int)(threadIdx.x & 63) >> 4, c0 = 64 * step + 16 * g;
         const float sc = qs * ks;
 #pragma unroll
         for (int j = 0; j < 16; j++) s[j] *= sc;
-        if (b.rel && pos_min - (64 * step + 63) < b.R) {
+        if (near == 2) {
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const int d = pos - c0 - j;
-                if (d >= 0 && d < b.R) s[j] = __builtin_fmaf(rel[-(int64_t)(c0 + j)], tau, s[j]);
-            }
+            for (int j = 0; j < 16; j++) r[15 - j] = rpos - c0 - j < b.R ? r[15 - j] : 0.0f;
+        }
+        if (near) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[j] = __builtin_fmaf(r[15 - j], tau, s[j]);
         }
         bool any = true;
         if (64 * step < lo_max || 64 * step + 63 > pos_min) {
@@ -316,25 +345,37 @@ struct Kv8Wave {
             for (int i = 0; i < 4; i++) O[ct][i] = __builtin_fmaf(kv8_join(d[2][i], d[1][i], d[0][i]), back, O[ct][i]);
         }
     }
-    // Steps s0, s0 + stride, .. below s1 (of the tile's steps).
+    // Steps s0, s0 + stride, .. below s1 (of the tile's steps). A step's loads
+    // return in the order they are issued in: the K operand of a step is asked
+    // for a step ahead, by table entries that are asked for another step ahead,
+    // before that step's V (behind V they would be waited for with it).
+    kv8_i4 K[4][2];
+    int32_t ev, nk, nv;      // table entries: V's of the step, both of the next
+    __device__ __forceinline__ void start(const Kv8Args &a, const Kv8Plan &p, const Kv8Tile &t, int s0, int s1, int stride) {
+        if (s0 >= s1) return;
+        int32_t ek;
+        entries(a, p, t, t.step0 + s0, ek, ev);
+        entries(a, p, t, t.step0 + min(s0 + stride, s1 - 1), nk, nv);
+        load_k(a, page(a, ek), p.hk, t.step0 + s0, K);
+    }
     __device__ __forceinline__ void walk(const Kv8Args &a, const Kv8Attn &b, const Kv8Plan &p, const Kv8Tile &t, int s0, int s1,
                                          int stride) {
-        if (s0 >= s1) return;
-        kv8_i4 K[4][2], V[8];
-        int64_t pk, pv, nk, nv;
-        pages(a, p, t, t.step0 + s0, pk, pv);
-        load_k(a, pk, p.hk, t.step0 + s0, K);
         for (int i = s0; i < s1; i += stride) {
-            const int step_i = t.step0 + i;
+            const int at = t.step0 + i;
+            const int64_t pv = page(a, ev);
+            int32_t mk, mv;
+            entries(a, p, t, t.step0 + min(i + 2 * stride, s1 - 1), mk, mv);
             const float ks = *a.scale(pv, 0, p.hk), vs = *a.scale(pv, 1, p.hk);
-            load_v(a, pv, p.hk, step_i, V);
-            const bool more = i + stride < s1;
-            if (more) pages(a, p, t, step_i + stride, nk, nv);
-            float s[16];
+            float r[16], s[16];
+            const int near = load_rel(b, at, r);
+            kv8_i4 V[8];
+            load_v(a, pv, p.hk, at, V);
             dots(K, s);
-            if (more) load_k(a, nk, p.hk, step_i + stride, K);
-            step(a, b, step_i, s, ks, vs, V);
-            pv = nv;
+            if (i + stride < s1) load_k(a, page(a, nk), p.hk, at + stride, K);
+            step(a, b, at, s, ks, vs, near, r, V);
+            ev = nv;
+            nk = mk;
+            nv = mv;
         }
     }
 };
@@ -351,6 +392,7 @@ __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b)
     const int span = (t.steps + p.splits - 1) / p.splits, s0 = p.x * span, s1 = min(t.steps, s0 + span);
     const int w = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4, G = b.H / a.Hkv;
     Kv8Wave<FULL> W;
+    W.start(a, p, t, s0 + w, s1, KV8_NW);
     W.init(a, b, t, 0, p.hk);
     W.walk(a, b, p, t, s0 + w, s1, KV8_NW);
     const float l = kv8_sum_g(W.l);
@@ -390,27 +432,41 @@ __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b)
 extern "C" __global__ __launch_bounds__(64 * KV8_NW, 2) void sepia_kv8_attn(Kv8Args a, Kv8Attn b) { kv8_attn_run<true>(a, b); }
 extern "C" __global__ __launch_bounds__(64 * KV8_NW, 2) void sepia_kv8_attn_d(Kv8Args a, Kv8Attn b) { kv8_attn_run<false>(a, b); }
 
-// Folds the runs of every unit that was cut. Grid: as many workgroups as
-// units that may be, a thread for 4 dims of a row at a time.
+// Folds the runs of every unit that was cut. Grid: as many units as may be cut,
+// rows of a tile. Eight groups of threads take a row's runs in turn, a thread
+// for 4 dims, and meet in LDS (one group after the other runs by itself, for
+// all rows in one workgroup, took 34 us at 63 runs).
 extern "C" __global__ __launch_bounds__(256) void sepia_kv8_fold(Kv8Args a, Kv8Attn b) {
+    __shared__ kv8_f4 so[8][32];
+    __shared__ float sl[8];
     Kv8Plan p;
     if (!kv8_plan<true>(a, b, (int)blockIdx.x, p)) return;
     const Kv8Tile t = kv8_tile(b, p);
     const int span = (t.steps + p.splits - 1) / p.splits, ns = (t.steps + span - 1) / span, G = b.H / a.Hkv;
-    const int per = a.Dh / 4;
-    for (int i = (int)threadIdx.x; i < 16 * per; i += 256) {
-        const int n = i / per, d = 4 * (i - n * per), ti = n / G;
-        if (ti >= t.nt) continue;
-        float M = -INFINITY, L = 0.0f;
-        for (int x = 0; x < ns; x++) M = fmaxf(M, b.ml[((int64_t)p.slot + (int64_t)x * a.Hkv) * 32 + n]);
-        const float ref = M == -INFINITY ? 0.0f : M;
-        kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int x = 0; x < ns; x++) {
-            const int64_t slot = (int64_t)p.slot + (int64_t)x * a.Hkv;
-            const float f = __builtin_amdgcn_exp2f((b.ml[slot * 32 + n] - ref) * KV8_L2E);
-            L += b.ml[slot * 32 + 16 + n] * f;
-            o += *(const kv8_f4 *)(b.part + (slot * 16 + n) * a.Dh + d) * f;
-        }
-        *(kv8_f4 *)(b.out + ((int64_t)(t.t0 + ti) * b.H + p.hk * G + (n - ti * G)) * a.Dh + d) = o / L;
+    const int n = (int)blockIdx.y, ti = n / G, j = (int)threadIdx.x >> 5, d = 4 * ((int)threadIdx.x & 31);
+    if (ti >= t.nt) return;
+    float M = -INFINITY, L = 0.0f;
+    for (int x = (int)threadIdx.x & 63; x < ns; x += 64) M = fmaxf(M, b.ml[((int64_t)p.slot + (int64_t)x * a.Hkv) * 32 + n]);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    const float ref = M == -INFINITY ? 0.0f : M;
+    kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int x = j; x < ns; x += 8) {
+        const int64_t slot = (int64_t)p.slot + (int64_t)x * a.Hkv;
+        const float f = __builtin_amdgcn_exp2f((b.ml[slot * 32 + n] - ref) * KV8_L2E);
+        L += b.ml[slot * 32 + 16 + n] * f;
+        if (d < a.Dh) o += *(const kv8_f4 *)(b.part + (slot * 16 + n) * a.Dh + d) * f;
     }
+    so[j][d / 4] = o;
+    if (d == 0) sl[j] = L;
+    __syncthreads();
+    if (j > 0 || d >= a.Dh) return;
+    L = 0.0f;
+    o = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        o += so[i][d / 4];
+        L += sl[i];
+    }
+    *(kv8_f4 *)(b.out + ((int64_t)(t.t0 + ti) * b.H + p.hk * G + (n - ti * G)) * a.Dh + d) = o / L;
 }

@@ -216,7 +216,7 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
         return 0;
     if (!budget) return 1;
     const int64_t cut = ids * c->n_kv_heads < budget ? ids * c->n_kv_heads : budget;
-    return sepia_serve_launch(SK_KV8_FOLD, (unsigned)cut, 1, 1, 256, args, op);
+    return sepia_serve_launch(SK_KV8_FOLD, (unsigned)cut, 16, 1, 256, args, op);
 }
 
 /* struct SampleArgs of kernels/sample.h, and the bytes of its SampleRow and
