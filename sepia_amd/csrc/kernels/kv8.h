@@ -29,15 +29,16 @@ struct Kv8Args {
     const int32_t *table, *lens, *starts;
     int64_t n_pages;
     int32_t n_seqs, max_pages, Hkv, Dh, lg, n;   // n: rows of the call
+    uint32_t head_bytes, page_bytes;             // of a head's K or V in a page, of a page
     __device__ __forceinline__ int P() const { return 1 << lg; }
-    __device__ __forceinline__ int8_t *k_codes(int64_t page, int hk) const {
-        return codes + ((page * 2) * Hkv + hk) * ((int64_t)Dh << lg);
+    __device__ __forceinline__ int8_t *k_codes(uint32_t page, int hk) const {
+        return codes + (uint64_t)hk * head_bytes + (uint64_t)page * page_bytes;
     }
-    __device__ __forceinline__ int8_t *v_codes(int64_t page, int hk) const {
-        return codes + ((page * 2 + 1) * Hkv + hk) * ((int64_t)Dh << lg);
+    __device__ __forceinline__ int8_t *v_codes(uint32_t page, int hk) const {
+        return codes + (uint64_t)(Hkv + hk) * head_bytes + (uint64_t)page * page_bytes;
     }
-    __device__ __forceinline__ float *scale(int64_t page, int side, int hk) const {
-        return scales + (page * 2 + side) * Hkv + hk;
+    __device__ __forceinline__ float *scale(uint32_t page, int side, int hk) const {
+        return scales + (side * Hkv + hk) + (uint64_t)page * (2u * (uint32_t)Hkv);
     }
 };
 
@@ -82,7 +83,7 @@ __device__ __forceinline__ void kv8_check(const Kv8Args &a) {
     if (bad) sepia_report_error(nullptr, KV8_ERR_SEQ, 0);
 }
 // The pool's page of entry `i` of a sequence's table row, -1 if it has none.
-__device__ __forceinline__ int64_t kv8_page(const Kv8Args &a, int s, int i) {
+__device__ __forceinline__ int kv8_page(const Kv8Args &a, int s, int i) {
     const int32_t p = a.table[(int64_t)s * a.max_pages + i];
     return (uint32_t)p < (uint64_t)a.n_pages ? p : -1;
 }
@@ -136,7 +137,7 @@ extern "C" __global__ __launch_bounds__(256, 4) void sepia_kv8_append(Kv8Args a,
     Kv8Unit u;
     if (s < 0) return;
     if (!kv8_unit(len, r0, r1, (int)(blockIdx.x - kv8_first_id(r0, s, a.P(), 2)), a.lg, &u)) return;
-    const int64_t page = kv8_page(a, s, u.page);
+    const int page = kv8_page(a, s, u.page);
     if (page < 0) {
         sepia_report_error(nullptr, KV8_ERR_PAGE, (int)threadIdx.x);
         return;
@@ -255,7 +256,7 @@ extern "C" __global__ __launch_bounds__(256) void sepia_kv8_read(Kv8Args a, floa
     Kv8Unit u;
     if (s < 0) return;
     if (!kv8_unit(len, r0, r1, (int)(blockIdx.x - kv8_first_id(r0, s, a.P(), 2)), a.lg, &u)) return;
-    const int64_t page = kv8_page(a, s, u.page);
+    const int page = kv8_page(a, s, u.page);
     if (page < 0) {
         sepia_report_error(nullptr, KV8_ERR_PAGE, (int)threadIdx.x);
         return;

@@ -41,14 +41,21 @@ typedef int32_t kv8_i4 __attribute__((ext_vector_type(4)));
 typedef float kv8_f4 __attribute__((ext_vector_type(4)));
 typedef kv8_f4 kv8_f4u __attribute__((aligned(4)));
 
-// Over the four lane groups (lanes n, n + 16, n + 32, n + 48).
+// Over the four lane groups (lanes n, n + 16, n + 32, n + 48): the halves of
+// the rows of 16 lanes change places, then the halves of the wave. (As LDS
+// permutes these four exchanges a step were waited for, 0.1 us each.)
+template <class F>
+__device__ __forceinline__ float kv8_over_g(float v, F f) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    v = f(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return f(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
+}
 __device__ __forceinline__ float kv8_max_g(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    return kv8_over_g(v, [](float x, float y) { return fmaxf(x, y); });
 }
 __device__ __forceinline__ float kv8_sum_g(float v) {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
+    return kv8_over_g(v, [](float x, float y) { return x + y; });
 }
 
 // How a call's work is cut: sequence s has rt row tiles of TT tokens and at
@@ -137,7 +144,10 @@ __device__ __forceinline__ void kv8_planes(const uint32_t *u, int32_t &p0, int32
     p1 = (int32_t)(__builtin_amdgcn_perm(b, a, 0x07060302) ^ 0x80808080u);
     p2 = (int32_t)(c | d);
 }
-// hi 65536 + mid 256 + lo of exact sums (|sum| <= 2^20): mid 256 + lo is exact.
+// hi 65536 + mid 256 + lo of exact sums (|sum| <= 2^21): mid 256 + lo is exact.
+// (lo rounded to a multiple of 256 and added into mid's sum by the matrix op
+// would save 48 of a step's 520 instructions; it was no faster, and four times
+// as far off over 12000 columns.)
 __device__ __forceinline__ float kv8_join(int32_t hi, int32_t mid, int32_t lo) {
     return __builtin_fmaf((float)hi, 65536.0f, (float)(int32_t)(((uint32_t)mid << 8) + (uint32_t)lo));
 }
@@ -146,65 +156,74 @@ __device__ __forceinline__ float kv8_join(int32_t hi, int32_t mid, int32_t lo) {
 // dims; both cover Dh (FULL: Dh is 128).
 template <bool FULL>
 struct Kv8Wave {
+    static __device__ __forceinline__ int dh(const Kv8Args &a) { return FULL ? 128 : a.Dh; }
     kv8_i4 qd[3][2];        // q's digits: lane (n, g) dims 64 ks + 16 g .. + 15 of row n
     kv8_f4 O[8];
     float m, l, qs, tau;    // row n's maximum; this lane's part of its sum; q's scale times c
     int32_t lo, pos;        // row n's columns (inactive: none)
+    int64_t th;             // row n's (token, head)
+    bool on;                // whether there is a row n
     const float *rel;       // row n's rel_logits
-    int32_t rpos;           // pos, for an inactive row some active one's
+    int32_t rpos, R;        // pos, for an inactive row some active one's; the band
     int32_t lo_max, pos_min;   // over the active rows
 
-    __device__ __forceinline__ void init(const Kv8Args &a, const Kv8Attn &b, const Kv8Tile &t, int row0, int hk) {
-        const int lane = (int)(threadIdx.x & 63), n = lane & 15, g = lane >> 4, G = b.H / a.Hkv;
-        const int ti = (row0 + n) / G, h = hk * G + (row0 + n - ti * G);
-        const bool on = ti < t.nt;
-        const int64_t th = (int64_t)(t.t0 + (on ? ti : 0)) * b.H + (on ? h : hk * G);
-        const float *q = b.q + th * a.Dh;
-        float v[2][16], most = 0.0f;
-        bool bad = false;
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++) {
-            const int d = 64 * ks + 16 * g;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                kv8_f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (on && (FULL || d < a.Dh)) x = *(const kv8_f4 *)(q + d + 4 * i);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    v[ks][4 * i + e] = x[e];
-                    most = fmaxf(most, fabsf(x[e]));
-                    bad |= !(fabsf(x[e]) < INFINITY);
-                }
-            }
-        }
-        most = kv8_max_g(bad ? INFINITY : most);
-        const float inv = most > 0.0f && most < INFINITY ? KV8_C / most : 0.0f;
-        qs = most < INFINITY ? most * (b.c / KV8_C) : NAN;
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                uint32_t u[4];
-                int32_t p0, p1, p2;
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    u[e] = (uint32_t)(int32_t)__builtin_rintf(fmaxf(-KV8_C, fminf(KV8_C, v[ks][4 * i + e] * inv))) + 0x8080u;
-                kv8_planes(u, p0, p1, p2);
-                qd[0][ks][i] = p0;
-                qd[1][ks][i] = p1;
-                qd[2][ks][i] = p2;
-            }
+    __device__ __forceinline__ void init(const Kv8Args &a, const Kv8Attn &b, const Kv8Tile &t, int hk) {
+        const int n = (int)(threadIdx.x & 15), G = b.H / a.Hkv, ti = n / G;
+        on = ti < t.nt;
+        th = (int64_t)(t.t0 + (on ? ti : 0)) * b.H + hk * G + (on ? n - ti * G : 0);
         pos = on ? t.pos0 + ti : -1;
         lo = on ? (b.window > 0 ? max(0, pos - b.window + 1) : 0) : 0x7FFFFFFF;
         tau = b.tau ? b.tau[t.t0 + (on ? ti : 0)] : 1.0f;
         rel = b.rel ? b.rel + th * b.R : nullptr;
         rpos = on ? pos : t.pos0;
+        R = b.R;
         lo_max = b.window > 0 ? max(0, t.last - b.window + 1) : 0;
         pos_min = t.pos0;
         m = -INFINITY;
         l = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) O[i] = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // q of row n at dims 64 (i / 4) + 16 g + 4 (i % 4) .. (0 past the rows and Dh).
+    __device__ __forceinline__ void load_q(const Kv8Args &a, const Kv8Attn &b, kv8_f4 (&v)[8]) const {
+        const int g = (int)(threadIdx.x & 63) >> 4;
+        const float *q = b.q + th * dh(a);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int d = 64 * (i / 4) + 16 * g + 4 * (i % 4);
+            v[i] = *(const kv8_f4 *)(q + (FULL || d < a.Dh ? d : 0));
+        }
+    }
+    // Its digits and its scale.
+    __device__ __forceinline__ void digits(const Kv8Args &a, const Kv8Attn &b, kv8_f4 (&v)[8]) {
+        const int g = (int)(threadIdx.x & 63) >> 4;
+        float most = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const bool in = on && (FULL || 64 * (i / 4) + 16 * g < a.Dh);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                v[i][e] = in ? v[i][e] : 0.0f;
+                most = fmaxf(most, fabsf(v[i][e]));
+                bad |= !(fabsf(v[i][e]) < INFINITY);
+            }
+        }
+        most = kv8_max_g(bad ? INFINITY : most);
+        const float inv = most > 0.0f && most < INFINITY ? KV8_C / most : 0.0f;
+        qs = most < INFINITY ? most * (b.c / KV8_C) : NAN;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            uint32_t u[4];
+            int32_t p0, p1, p2;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                u[e] = (uint32_t)(int32_t)__builtin_rintf(fmaxf(-KV8_C, fminf(KV8_C, v[i][e] * inv))) + 0x8080u;
+            kv8_planes(u, p0, p1, p2);
+            qd[0][i / 4][i % 4] = p0;
+            qd[1][i / 4][i % 4] = p1;
+            qd[2][i / 4][i % 4] = p2;
+        }
     }
 
     // The table's entries for a step: of this lane's K row and of its columns
@@ -219,28 +238,28 @@ struct Kv8Wave {
         ek = row[max(first, min(end, ik))];
         ev = row[max(first, min(end, iv))];
     }
-    static __device__ __forceinline__ int64_t page(const Kv8Args &a, int32_t entry) {
+    static __device__ __forceinline__ uint32_t page(const Kv8Args &a, int32_t entry) {
         const bool bad = (uint32_t)entry >= (uint64_t)a.n_pages;
         if (__ballot(bad)) sepia_report_error(nullptr, KV8_ERR_PAGE, (int)(threadIdx.x & 63));
-        return bad ? 0 : entry;
+        return bad ? 0u : (uint32_t)entry;
     }
     // K operand [t][ks]: column 16 (n >> 2) + 4 t + (n & 3), dims 64 ks + 16 g.
-    static __device__ __forceinline__ void load_k(const Kv8Args &a, int64_t page, int hk, int step, kv8_i4 (&K)[4][2]) {
+    static __device__ __forceinline__ void load_k(const Kv8Args &a, uint32_t page, int hk, int step, kv8_i4 (&K)[4][2]) {
         const int lane = (int)(threadIdx.x & 63), n = lane & 15, g = lane >> 4;
         const int slot = (64 * step + 16 * (n >> 2) + (n & 3)) & (a.P() - 1);
-        const int8_t *k = a.k_codes(page, hk) + slot * a.Dh + (FULL || 16 * g < a.Dh ? 16 * g : 0);
+        const int8_t *k = a.k_codes(page, hk) + slot * dh(a) + (FULL || 16 * g < dh(a) ? 16 * g : 0);
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            K[t][0] = *(const kv8_i4 *)(k + 4 * t * a.Dh);
-            K[t][1] = *(const kv8_i4 *)(k + 4 * t * a.Dh + (FULL || 64 + 16 * g < a.Dh ? 64 : 0));
+            K[t][0] = *(const kv8_i4 *)(k + 4 * t * dh(a));
+            K[t][1] = *(const kv8_i4 *)(k + 4 * t * dh(a) + (FULL || 64 + 16 * g < dh(a) ? 64 : 0));
         }
     }
     // V operand [ct]: dim 16 ct + n, columns 16 g .. + 15.
-    static __device__ __forceinline__ void load_v(const Kv8Args &a, int64_t page, int hk, int step, kv8_i4 (&V)[8]) {
+    static __device__ __forceinline__ void load_v(const Kv8Args &a, uint32_t page, int hk, int step, kv8_i4 (&V)[8]) {
         const int lane = (int)(threadIdx.x & 63), n = lane & 15, g = lane >> 4;
         const int8_t *v = a.v_codes(page, hk) + ((int64_t)n << a.lg) + ((64 * step + 16 * g) & (a.P() - 1));
 #pragma unroll
-        for (int ct = 0; ct < 8; ct++) V[ct] = *(const kv8_i4 *)(v + ((int64_t)(FULL || 16 * ct < a.Dh ? 16 * ct : 0) << a.lg));
+        for (int ct = 0; ct < 8; ct++) V[ct] = *(const kv8_i4 *)(v + ((int64_t)(FULL || 16 * ct < dh(a) ? 16 * ct : 0) << a.lg));
     }
     // rel_logits of row n and column 16 g + j of a step in r[15 - j], where the
     // row sees the column and its band reaches it. 0: no such column in the
@@ -276,22 +295,25 @@ struct Kv8Wave {
             for (int i = 0; i < 4; i++) s[4 * t + i] = kv8_join(d[2][i], d[1][i], d[0][i]);
         }
     }
-    // The step's softmax and weighted v; ks, vs: the scales of the page of
-    // columns 16 g .. .
-    __device__ __forceinline__ void step(const Kv8Args &a, const Kv8Attn &b, int step, float (&s)[16], float ks, float vs,
-                                         int near, float (&r)[16], const kv8_i4 (&V)[8]) {
-        const int g = (int)(threadIdx.x & 63) >> 4, c0 = 64 * step + 16 * g;
+    // Scores from their digit sums.
+    __device__ __forceinline__ void scores(int step, float (&s)[16]) {
+        const int d0 = rpos - (64 * step + 16 * ((int)(threadIdx.x & 63) >> 4));
         const float sc = qs * ks;
 #pragma unroll
         for (int j = 0; j < 16; j++) s[j] *= sc;
         if (near == 2) {
 #pragma unroll
-            for (int j = 0; j < 16; j++) r[15 - j] = rpos - c0 - j < b.R ? r[15 - j] : 0.0f;
+            for (int j = 0; j < 16; j++) r[15 - j] = d0 - j < R ? r[15 - j] : 0.0f;
         }
         if (near) {
 #pragma unroll
             for (int j = 0; j < 16; j++) s[j] = __builtin_fmaf(r[15 - j], tau, s[j]);
         }
+    }
+    // The step's softmax and weighted v; vs: the scale of the page of columns
+    // 16 g .. .
+    __device__ __forceinline__ void step(const Kv8Args &a, int step, float (&s)[16], float vs, const kv8_i4 (&V)[8]) {
+        const int g = (int)(threadIdx.x & 63) >> 4, c0 = 64 * step + 16 * g;
         bool any = true;
         if (64 * step < lo_max || 64 * step + 63 > pos_min) {
             any = c0 <= pos && c0 + 15 >= lo;
@@ -345,34 +367,45 @@ struct Kv8Wave {
             for (int i = 0; i < 4; i++) O[ct][i] = __builtin_fmaf(kv8_join(d[2][i], d[1][i], d[0][i]), back, O[ct][i]);
         }
     }
-    // Steps s0, s0 + stride, .. below s1 (of the tile's steps). A step's loads
-    // return in the order they are issued in: the K operand of a step is asked
-    // for a step ahead, by table entries that are asked for another step ahead,
-    // before that step's V (behind V they would be waited for with it).
+    // Steps s0, s0 + stride, .. below s1 (of the tile's steps). Loads return in
+    // the order they are issued in, and HBM's latency under load is a whole
+    // step: a step's K, scales and rel_logits are asked for a step ahead, by
+    // table entries that are asked for another step ahead, and its V at its
+    // beginning, in the order in which they are waited for.
     kv8_i4 K[4][2];
-    int32_t ev, nk, nv;      // table entries: V's of the step, both of the next
-    __device__ __forceinline__ void start(const Kv8Args &a, const Kv8Plan &p, const Kv8Tile &t, int s0, int s1, int stride) {
+    float r[16], ks, vs;     // of the step to come
+    int near;
+    int32_t ev, nk, nv;      // table entries: V's of that step, both of the next
+    __device__ __forceinline__ void ask(const Kv8Args &a, const Kv8Attn &b, const Kv8Plan &p, int step, uint32_t pk, uint32_t pv) {
+        load_k(a, pk, p.hk, step, K);
+        ks = *a.scale(pv, 0, p.hk);
+        vs = *a.scale(pv, 1, p.hk);
+        near = load_rel(b, step, r);
+    }
+    __device__ __forceinline__ void start(const Kv8Args &a, const Kv8Plan &p, const Kv8Tile &t, int s0, int s1, int stride, int32_t &ek) {
         if (s0 >= s1) return;
-        int32_t ek;
         entries(a, p, t, t.step0 + s0, ek, ev);
         entries(a, p, t, t.step0 + min(s0 + stride, s1 - 1), nk, nv);
-        load_k(a, page(a, ek), p.hk, t.step0 + s0, K);
     }
     __device__ __forceinline__ void walk(const Kv8Args &a, const Kv8Attn &b, const Kv8Plan &p, const Kv8Tile &t, int s0, int s1,
-                                         int stride) {
+                                         int stride, int32_t ek) {
+        if (s0 >= s1) return;
+        kv8_f4 q[8];
+        load_q(a, b, q);
+        ask(a, b, p, t.step0 + s0, page(a, ek), page(a, ev));
+        digits(a, b, q);
         for (int i = s0; i < s1; i += stride) {
             const int at = t.step0 + i;
-            const int64_t pv = page(a, ev);
             int32_t mk, mv;
             entries(a, p, t, t.step0 + min(i + 2 * stride, s1 - 1), mk, mv);
-            const float ks = *a.scale(pv, 0, p.hk), vs = *a.scale(pv, 1, p.hk);
-            float r[16], s[16];
-            const int near = load_rel(b, at, r);
             kv8_i4 V[8];
-            load_v(a, pv, p.hk, at, V);
+            load_v(a, page(a, ev), p.hk, at, V);
+            float s[16];
             dots(K, s);
-            if (i + stride < s1) load_k(a, page(a, nk), p.hk, at + stride, K);
-            step(a, b, at, s, ks, vs, near, r, V);
+            scores(at, s);
+            const float vs_i = vs;
+            if (i + stride < s1) ask(a, b, p, at + stride, page(a, nk), page(a, nv));
+            step(a, at, s, vs_i, V);
             ev = nv;
             nk = mk;
             nv = mv;
@@ -392,9 +425,10 @@ __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b)
     const int span = (t.steps + p.splits - 1) / p.splits, s0 = p.x * span, s1 = min(t.steps, s0 + span);
     const int w = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4, G = b.H / a.Hkv;
     Kv8Wave<FULL> W;
-    W.start(a, p, t, s0 + w, s1, KV8_NW);
-    W.init(a, b, t, 0, p.hk);
-    W.walk(a, b, p, t, s0 + w, s1, KV8_NW);
+    int32_t ek;
+    W.start(a, p, t, s0 + w, s1, KV8_NW, ek);
+    W.init(a, b, t, p.hk);
+    W.walk(a, b, p, t, s0 + w, s1, KV8_NW, ek);
     const float l = kv8_sum_g(W.l);
     if (g == 0) {
         sm[w][n] = W.m;
@@ -431,6 +465,38 @@ __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b)
 }
 extern "C" __global__ __launch_bounds__(64 * KV8_NW, 2) void sepia_kv8_attn(Kv8Args a, Kv8Attn b) { kv8_attn_run<true>(a, b); }
 extern "C" __global__ __launch_bounds__(64 * KV8_NW, 2) void sepia_kv8_attn_d(Kv8Args a, Kv8Attn b) { kv8_attn_run<false>(a, b); }
+
+// Many rows (prompts): a wave a unit, KV8_NW row tiles of one kv head side by
+// side in a workgroup, so that they find K and V in the caches; nothing is cut
+// or folded. Grid: (ids of KV8_NW row tiles, kv heads), kv heads fastest, so
+// that with 8 of them an XCD's L2 holds one head's K and V.
+template <bool FULL>
+__device__ __forceinline__ void kv8_attn_rows(const Kv8Args &a, const Kv8Attn &b) {
+    kv8_check(a);
+    Kv8Plan p;
+    const int id = (int)blockIdx.x / a.Hkv, gran = KV8_NW * b.TT;
+    p.hk = (int)blockIdx.x - id * a.Hkv;
+    p.s = kv8_find(a, id, gran, 1, p.len, p.r0, p.r1);
+    if (p.s < 0) return;
+    p.k = (id - (int)kv8_first_id(p.r0, p.s, gran, 1)) * KV8_NW + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    if ((int64_t)p.k * b.TT >= p.r1 - p.r0) return;
+    const Kv8Tile t = kv8_tile(b, p);
+    const int lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4, G = b.H / a.Hkv;
+    Kv8Wave<FULL> W;
+    int32_t ek;
+    W.start(a, p, t, 0, t.steps, 1, ek);
+    W.init(a, b, t, p.hk);
+    W.walk(a, b, p, t, 0, t.steps, 1, ek);
+    const float inv = 1.0f / kv8_sum_g(W.l);
+    const int ti = n / G;
+    if (ti >= t.nt) return;
+    float *o = b.out + ((int64_t)(t.t0 + ti) * b.H + p.hk * G + (n - ti * G)) * a.Dh + 4 * g;
+#pragma unroll
+    for (int ct = 0; ct < 8; ct++)
+        if (FULL || 16 * ct < a.Dh) *(kv8_f4 *)(o + 16 * ct) = W.O[ct] * inv;
+}
+extern "C" __global__ __launch_bounds__(64 * KV8_NW, 2) void sepia_kv8_rows(Kv8Args a, Kv8Attn b) { kv8_attn_rows<true>(a, b); }
+extern "C" __global__ __launch_bounds__(64 * KV8_NW, 2) void sepia_kv8_rows_d(Kv8Args a, Kv8Attn b) { kv8_attn_rows<false>(a, b); }
 
 // Folds the runs of every unit that was cut. Grid: as many units as may be cut,
 // rows of a tile. Eight groups of threads take a row's runs in turn, a thread

@@ -107,8 +107,8 @@ static const char *const k_names[K_COUNT] = {
 /* Kernels of the second code object, sepia_serve.hsaco (the SK_* of
  * internal.h); their ids follow the first's. */
 static const char *const serve_names[SK_COUNT] = {
-    "sepia_kv8_append", "sepia_kv8_read", "sepia_kv8_attn", "sepia_kv8_attn_d", "sepia_kv8_fold", "sepia_sample_max",
-    "sepia_sample_bins", "sepia_sample_pick", "sepia_sample",
+    "sepia_kv8_append", "sepia_kv8_read", "sepia_kv8_attn", "sepia_kv8_attn_d", "sepia_kv8_rows", "sepia_kv8_rows_d",
+    "sepia_kv8_fold", "sepia_sample_max", "sepia_sample_bins", "sepia_sample_pick", "sepia_sample",
 };
 #define K_ALL (K_COUNT + SK_COUNT)
 static const char *k_name(int k) { return k < K_COUNT ? k_names[k] : serve_names[k - K_COUNT]; }

@@ -19,6 +19,7 @@ typedef struct {
     const int32_t *table, *lens, *starts;
     int64_t n_pages;
     int32_t n_seqs, max_pages, Hkv, Dh, lg, n;
+    uint32_t head_bytes, page_bytes;
 } Kv8Args;
 
 /* Checks a cache and a call's rows, and fills the kernels' arguments; `write`:
@@ -76,6 +77,8 @@ static int kv8_args(const char *op, const SepiaKv8Cache *c, SepiaGpuBuf *lens, S
     a->Dh = c->head_dim;
     a->lg = c->page == 16 ? 4 : c->page == 32 ? 5 : 6;
     a->n = (int32_t)n;
+    a->head_bytes = (uint32_t)(c->page * c->head_dim);
+    a->page_bytes = (uint32_t)page;
     return 1;
 }
 
@@ -147,6 +150,7 @@ int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *
 }
 
 /* struct Kv8Attn of kernels/kv8_attn.h */
+#define KV8_ROWS 1024       /* units from which each has a wave of its own */
 #define KV8_BUDGET 512      /* runs of a call whose units alone leave the chip idle: two workgroups a CU */
 typedef struct {
     const float *q, *rel, *tau;
@@ -193,12 +197,19 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
     b.R = (int32_t)rel_extent;
     b.window = window > 0x7FFFFFFF ? 0 : (int32_t)window;
     b.c = inv_head_dim;
-    /* 16 rows a wave; units (row tile, kv head) are cut into runs of steps
-     * where they are few, and the runs folded */
+    /* 16 rows a wave. Many units (row tile, kv head): a wave each. Few: cut
+     * into runs of steps, whose partials are folded. */
     b.TT = (int32_t)(16 / (n_heads / c->n_kv_heads));
-    const int64_t ids = n / b.TT + c->n_seqs, few = n / b.TT > c->n_seqs ? n / b.TT : n < c->n_seqs ? n : c->n_seqs;
+    const int full = c->head_dim == 128;
+    const int64_t units = (n / b.TT > c->n_seqs ? n / b.TT : n < c->n_seqs ? n : c->n_seqs) * c->n_kv_heads;
+    if (units >= KV8_ROWS) {
+        void *args[] = { &a, &b };
+        return sepia_serve_launch(full ? SK_KV8_ROWS : SK_KV8_ROWS_D, (unsigned)((n / (4 * b.TT) + c->n_seqs) * c->n_kv_heads),
+                                  1, 1, 256, args, op);
+    }
+    const int64_t ids = n / b.TT + c->n_seqs;
     const size_t per = 16 * (size_t)c->head_dim * 4, limit = sepia_scratch_limit();
-    int64_t budget = few * c->n_kv_heads < 2 * KV8_BUDGET ? KV8_BUDGET : 0, slots = 2 * budget + 64;
+    int64_t budget = KV8_BUDGET, slots = 2 * budget + 64;
     while (budget && (size_t)slots * (per + 128) > limit) {
         budget /= 2;
         slots = 2 * budget + 64;
@@ -211,7 +222,7 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
     }
     b.budget = (int32_t)budget;
     void *args[] = { &a, &b };
-    if (!sepia_serve_launch(c->head_dim == 128 ? SK_KV8_ATTN : SK_KV8_ATTN_D, (unsigned)(budget + ids * c->n_kv_heads), 1, 1,
+    if (!sepia_serve_launch(full ? SK_KV8_ATTN : SK_KV8_ATTN_D, (unsigned)(budget + ids * c->n_kv_heads), 1, 1,
                             256, args, op))
         return 0;
     if (!budget) return 1;

@@ -168,6 +168,9 @@ ATTNS = [
     (4, 2, 128, 16, [33], [100], 50, 40), (8, 8, 128, 64, [130], [140], 0, 128), (16, 2, 128, 16, [0], [200], 1, 8),
     (64, 8, 128, 16, [300, 0], [33, 64], 0, 512), (3, 3, 96, 32, [0] * 80, [k % 4 for k in range(80)], 0, 5),
     (16, 1, 16, 16, [1000], [1], 100, 7), (8, 2, 128, 32, [3000], [1], 0, 100),
+    # many rows: a wave a unit
+    (128, 64, 128, 16, [200, 0, 3], [130, 0, 9], 0, 64), (96, 32, 128, 64, [64], [180], 90, 0),
+    (48, 16, 64, 32, [70, 0], [200, 150], 100, 40), (112, 56, 80, 16, [17, 0], [100, 60], 0, 300),
 ]
 
 
