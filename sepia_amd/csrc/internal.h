@@ -40,12 +40,16 @@ SEPIA_HIDDEN int sepia_prep_out(SepiaGpuBuf *b, const char *op);
  * many a call may ask for: what there is while the stream is being captured,
  * else any number. */
 SEPIA_HIDDEN void *sepia_scratch(size_t need, const char *op);
+/* Once there is scratch: SEPIA_COUNTERS arrival counters in front of it, zero
+ * between launches (a kernel that uses one leaves it so). */
+#define SEPIA_COUNTERS 16384
+SEPIA_HIDDEN uint32_t *sepia_counters(void);
 SEPIA_HIDDEN size_t sepia_scratch_limit(void);
 
 /* Kernels of the second code object (kernels/sepia_serve.hip), and a launch
  * of one on the library's stream, timed when the profiler is on. */
-enum { SK_KV8_APPEND, SK_KV8_READ, SK_KV8_ATTN, SK_KV8_ATTN_D, SK_KV8_ROWS, SK_KV8_ROWS_D, SK_KV8_FOLD, SK_SAMPLE_MAX, SK_SAMPLE_BINS, SK_SAMPLE_PICK,
-       SK_SAMPLE, SK_COUNT };
+enum { SK_KV8_APPEND, SK_KV8_READ, SK_KV8_ATTN, SK_KV8_ROWS = SK_KV8_ATTN + 4,   /* head dims 128, up to 128, 64, up to 64 */
+       SK_KV8_FOLD = SK_KV8_ROWS + 4, SK_SAMPLE_MAX, SK_SAMPLE_BINS, SK_SAMPLE_PICK, SK_SAMPLE, SK_COUNT };
 SEPIA_HIDDEN int sepia_serve_launch(int k, unsigned gx, unsigned gy, unsigned gz, unsigned block, void **args,
                                     const char *op);
 

@@ -32,7 +32,8 @@
 struct Kv8Attn {
     const float *q, *rel, *tau;
     float *out;
-    float *part, *ml;        // per split: O [16][Dh]; maxima [16], sums [16]
+    float *part, *ml;        // per run: O [16][Dh]; maxima [16], sums [16]
+    uint32_t *arrived;       // per unit (at its first run's place): runs done; NULL: sepia_kv8_fold folds
     int32_t H, R, window, TT, budget;   // TT: tokens of a row tile
     float c;
 };
@@ -65,56 +66,70 @@ __device__ __forceinline__ float kv8_sum_g(float v) {
 struct Kv8Plan {
     int s, k, hk, x, splits, slot, len, r0, r1;   // slot: of split 0 of the unit (splits > 1); + Hkv a split
 };
-__device__ __forceinline__ void kv8_cost(const Kv8Args &a, const Kv8Attn &b, int s, int &rt, int &steps) {
+__device__ __forceinline__ void kv8_cost(const Kv8Args &a, const Kv8Attn &b, int s, int &rt, int &steps, int &len, int &r0,
+                                         int &r1) {
     rt = steps = 0;
-    int32_t len, r0, r1;
     if (s >= a.n_seqs || !kv8_seq(a, s, len, r0, r1) || r1 == r0) return;
     const int end = len + (r1 - r0);
     rt = (r1 - r0 + b.TT - 1) / b.TT;
     steps = (end + 63) / 64;
     if (b.window > 0) steps = min(steps, (int)(((int64_t)b.window + b.TT + 61) / 64) + 1);
 }
-// The id-th run (combine: the id-th unit that is cut) in the order sequence,
+// Inclusive sums over the wave's lanes.
+template <class T>
+__device__ __forceinline__ T kv8_scan(T v) {
+#define KV8_DPP(ctrl, rows, ctl)                                                                                        \
+    v += __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, rows, 0xF, ctl))
+    KV8_DPP(0x111, 0xF, true);    // row_shr 1, 2, 4, 8
+    KV8_DPP(0x112, 0xF, true);
+    KV8_DPP(0x114, 0xF, true);
+    KV8_DPP(0x118, 0xF, true);
+    KV8_DPP(0x142, 0xA, false);   // the last lane of a row to the next, of two rows to the next two
+    KV8_DPP(0x143, 0xC, false);
+#undef KV8_DPP
+    return v;
+}
+template <class T>
+__device__ __forceinline__ T kv8_last(T v) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+// The id-th run (FOLD: the id-th unit that may be cut) in the order sequence,
 // row tile, split, kv head; 0 past the last.
-template <bool COMBINE>
+template <bool FOLD>
 __device__ __forceinline__ int kv8_plan(const Kv8Args &a, const Kv8Attn &b, int id, Kv8Plan &p) {
     const int lane = (int)(threadIdx.x & 63);
     float total = 0.0f;
+    int rt, steps, len, r0, r1;
     for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
-        int rt, steps;
-        kv8_cost(a, b, s0 + lane, rt, steps);
-        total += wave_sum((float)rt * (float)steps);
+        kv8_cost(a, b, s0 + lane, rt, steps, len, r0, r1);
+        total += kv8_last(kv8_scan((float)rt * (float)steps));
     }
     const int chunk = b.budget > 0 ? max(KV8_NW, (int)ceilf(fminf(total * (float)a.Hkv / (float)b.budget, 1e9f))) : 0x7FFFFFFF;
     p.hk = id % a.Hkv;
     const int at = id / a.Hkv;
     int base = 0, slots = 0;
     for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
-        int rt, steps;
-        kv8_cost(a, b, s0 + lane, rt, steps);
+        if (a.n_seqs > 64) kv8_cost(a, b, s0 + lane, rt, steps, len, r0, r1);   // else they are still here
         const int splits = (int)(((int64_t)steps + chunk - 1) / chunk);
-        const int mine = COMBINE ? (splits > 1 ? rt : 0) : rt * splits;
+        const int mine = FOLD ? (splits > 1 ? rt : 0) : rt * splits;
         const int cut = splits > 1 ? rt * splits : 0;
-        int sum = mine, csum = cut;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(sum, o, 64), v = __shfl_up(csum, o, 64);
-            if (lane >= o) sum += u, csum += v;
-        }
+        const int sum = kv8_scan(mine), csum = kv8_scan(cut);
         const uint64_t hit = __ballot(at >= base + sum - mine && at < base + sum);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             p.s = s0 + l;
             p.splits = __builtin_amdgcn_readlane(splits, l);
             const int i = at - base - __builtin_amdgcn_readlane(sum - mine, l);
-            p.k = COMBINE ? i : i / p.splits;
-            p.x = COMBINE ? 0 : i - p.k * p.splits;
+            p.k = FOLD ? i : i / p.splits;
+            p.x = FOLD ? 0 : i - p.k * p.splits;
             p.slot = (slots + __builtin_amdgcn_readlane(csum - cut, l) + p.k * p.splits) * a.Hkv + p.hk;
-            kv8_seq(a, p.s, p.len, p.r0, p.r1);
+            p.len = __builtin_amdgcn_readlane(len, l);
+            p.r0 = __builtin_amdgcn_readlane(r0, l);
+            p.r1 = __builtin_amdgcn_readlane(r1, l);
             return 1;
         }
-        base += __builtin_amdgcn_readlane(sum, 63);
-        slots += __builtin_amdgcn_readlane(csum, 63);
+        base += kv8_last(sum);
+        slots += kv8_last(csum);
     }
     return 0;
 }
@@ -122,8 +137,9 @@ __device__ __forceinline__ int kv8_plan(const Kv8Args &a, const Kv8Attn &b, int 
 // A row tile's tokens and its steps of 64 columns.
 struct Kv8Tile {
     int t0, nt, pos0, lo, last, step0, steps;   // lo, last: the first and last column any row sees
+    int span, runs;                             // steps of a run, runs that have any
 };
-__device__ __forceinline__ Kv8Tile kv8_tile(const Kv8Attn &b, const Kv8Plan &p) {
+__device__ __forceinline__ Kv8Tile kv8_tile(const Kv8Attn &b, const Kv8Plan &p, int splits) {
     Kv8Tile t;
     t.t0 = p.r0 + p.k * b.TT;
     t.nt = min(b.TT, p.r1 - t.t0);
@@ -132,6 +148,8 @@ __device__ __forceinline__ Kv8Tile kv8_tile(const Kv8Attn &b, const Kv8Plan &p) 
     t.lo = b.window > 0 ? max(0, t.pos0 - b.window + 1) : 0;
     t.step0 = t.lo >> 6;
     t.steps = (t.last >> 6) - t.step0 + 1;
+    t.span = (t.steps + splits - 1) / splits;
+    t.runs = (t.steps + t.span - 1) / t.span;
     return t;
 }
 
@@ -152,13 +170,14 @@ __device__ __forceinline__ float kv8_join(int32_t hi, int32_t mid, int32_t lo) {
     return __builtin_fmaf((float)hi, 65536.0f, (float)(int32_t)(((uint32_t)mid << 8) + (uint32_t)lo));
 }
 
-// One wave's 16 rows. NK: K operands a row (64 dims each), NC: tiles of 16
-// dims; both cover Dh (FULL: Dh is 128).
-template <bool FULL>
+// One wave's 16 rows of D dims (FULL), or of up to D (a.Dh). NK: K operands a
+// row (64 dims each), NC: tiles of 16 dims.
+template <int D, bool FULL>
 struct Kv8Wave {
-    static __device__ __forceinline__ int dh(const Kv8Args &a) { return FULL ? 128 : a.Dh; }
-    kv8_i4 qd[3][2];        // q's digits: lane (n, g) dims 64 ks + 16 g .. + 15 of row n
-    kv8_f4 O[8];
+    static constexpr int NK = D / 64, NC = D / 16;
+    static __device__ __forceinline__ int dh(const Kv8Args &a) { return FULL ? D : a.Dh; }
+    kv8_i4 qd[3][NK];       // q's digits: lane (n, g) dims 64 ks + 16 g .. + 15 of row n
+    kv8_f4 O[NC];
     float m, l, qs, tau;    // row n's maximum; this lane's part of its sum; q's scale times c
     int32_t lo, pos;        // row n's columns (inactive: none)
     int64_t th;             // row n's (token, head)
@@ -182,25 +201,25 @@ struct Kv8Wave {
         m = -INFINITY;
         l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) O[i] = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < NC; i++) O[i] = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     // q of row n at dims 64 (i / 4) + 16 g + 4 (i % 4) .. (0 past the rows and Dh).
-    __device__ __forceinline__ void load_q(const Kv8Args &a, const Kv8Attn &b, kv8_f4 (&v)[8]) const {
+    __device__ __forceinline__ void load_q(const Kv8Args &a, const Kv8Attn &b, kv8_f4 (&v)[4 * NK]) const {
         const int g = (int)(threadIdx.x & 63) >> 4;
         const float *q = b.q + th * dh(a);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < 4 * NK; i++) {
             const int d = 64 * (i / 4) + 16 * g + 4 * (i % 4);
             v[i] = *(const kv8_f4 *)(q + (FULL || d < a.Dh ? d : 0));
         }
     }
     // Its digits and its scale.
-    __device__ __forceinline__ void digits(const Kv8Args &a, const Kv8Attn &b, kv8_f4 (&v)[8]) {
+    __device__ __forceinline__ void digits(const Kv8Args &a, const Kv8Attn &b, kv8_f4 (&v)[4 * NK]) {
         const int g = (int)(threadIdx.x & 63) >> 4;
         float most = 0.0f;
         bool bad = false;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < 4 * NK; i++) {
             const bool in = on && (FULL || 64 * (i / 4) + 16 * g < a.Dh);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -213,7 +232,7 @@ struct Kv8Wave {
         const float inv = most > 0.0f && most < INFINITY ? KV8_C / most : 0.0f;
         qs = most < INFINITY ? most * (b.c / KV8_C) : NAN;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < 4 * NK; i++) {
             uint32_t u[4];
             int32_t p0, p1, p2;
 #pragma unroll
@@ -244,22 +263,22 @@ struct Kv8Wave {
         return bad ? 0u : (uint32_t)entry;
     }
     // K operand [t][ks]: column 16 (n >> 2) + 4 t + (n & 3), dims 64 ks + 16 g.
-    static __device__ __forceinline__ void load_k(const Kv8Args &a, uint32_t page, int hk, int step, kv8_i4 (&K)[4][2]) {
+    static __device__ __forceinline__ void load_k(const Kv8Args &a, uint32_t page, int hk, int step, kv8_i4 (&K)[4][NK]) {
         const int lane = (int)(threadIdx.x & 63), n = lane & 15, g = lane >> 4;
         const int slot = (64 * step + 16 * (n >> 2) + (n & 3)) & (a.P() - 1);
         const int8_t *k = a.k_codes(page, hk) + slot * dh(a) + (FULL || 16 * g < dh(a) ? 16 * g : 0);
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             K[t][0] = *(const kv8_i4 *)(k + 4 * t * dh(a));
-            K[t][1] = *(const kv8_i4 *)(k + 4 * t * dh(a) + (FULL || 64 + 16 * g < dh(a) ? 64 : 0));
+            if constexpr (NK == 2) K[t][1] = *(const kv8_i4 *)(k + 4 * t * dh(a) + (FULL || 64 + 16 * g < dh(a) ? 64 : 0));
         }
     }
     // V operand [ct]: dim 16 ct + n, columns 16 g .. + 15.
-    static __device__ __forceinline__ void load_v(const Kv8Args &a, uint32_t page, int hk, int step, kv8_i4 (&V)[8]) {
+    static __device__ __forceinline__ void load_v(const Kv8Args &a, uint32_t page, int hk, int step, kv8_i4 (&V)[NC]) {
         const int lane = (int)(threadIdx.x & 63), n = lane & 15, g = lane >> 4;
         const int8_t *v = a.v_codes(page, hk) + ((int64_t)n << a.lg) + ((64 * step + 16 * g) & (a.P() - 1));
 #pragma unroll
-        for (int ct = 0; ct < 8; ct++) V[ct] = *(const kv8_i4 *)(v + ((int64_t)(FULL || 16 * ct < dh(a) ? 16 * ct : 0) << a.lg));
+        for (int ct = 0; ct < NC; ct++) V[ct] = *(const kv8_i4 *)(v + ((int64_t)(FULL || 16 * ct < dh(a) ? 16 * ct : 0) << a.lg));
     }
     // rel_logits of row n and column 16 g + j of a step in r[15 - j], where the
     // row sees the column and its band reaches it. 0: no such column in the
@@ -282,14 +301,14 @@ struct Kv8Wave {
         return 2;
     }
     // Scores' digit sums of a step.
-    __device__ __forceinline__ void dots(const kv8_i4 (&K)[4][2], float (&s)[16]) const {
+    __device__ __forceinline__ void dots(const kv8_i4 (&K)[4][NK], float (&s)[16]) const {
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             kv8_i4 d[3];
 #pragma unroll
             for (int p = 0; p < 3; p++) {
                 d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(K[t][0], qd[p][0], kv8_i4{0, 0, 0, 0}, 0, 0, 0);
-                d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(K[t][1], qd[p][1], d[p], 0, 0, 0);
+                if constexpr (NK == 2) d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(K[t][1], qd[p][1], d[p], 0, 0, 0);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) s[4 * t + i] = kv8_join(d[2][i], d[1][i], d[0][i]);
@@ -312,7 +331,7 @@ struct Kv8Wave {
     }
     // The step's softmax and weighted v; vs: the scale of the page of columns
     // 16 g .. .
-    __device__ __forceinline__ void step(const Kv8Args &a, int step, float (&s)[16], float vs, const kv8_i4 (&V)[8]) {
+    __device__ __forceinline__ void step(const Kv8Args &a, int step, float (&s)[16], float vs, const kv8_i4 (&V)[NC]) {
         const int g = (int)(threadIdx.x & 63) >> 4, c0 = 64 * step + 16 * g;
         bool any = true;
         if (64 * step < lo_max || 64 * step + 63 > pos_min) {
@@ -329,7 +348,7 @@ struct Kv8Wave {
             const float al = __builtin_amdgcn_exp2f((m - ref) * KV8_L2E);   // 1 where the maximum stays
             l *= al;
 #pragma unroll
-            for (int ct = 0; ct < 8; ct++) O[ct] *= al;
+            for (int ct = 0; ct < NC; ct++) O[ct] *= al;
             m = mn;
         }
         vs = any ? vs : 0.0f;
@@ -358,7 +377,7 @@ struct Kv8Wave {
         }
         l += sum;
 #pragma unroll
-        for (int ct = 0; ct < 8; ct++) {
+        for (int ct = 0; ct < NC; ct++) {
             if (!FULL && 16 * ct >= a.Dh) break;
             kv8_i4 d[3];
 #pragma unroll
@@ -372,7 +391,7 @@ struct Kv8Wave {
     // step: a step's K, scales and rel_logits are asked for a step ahead, by
     // table entries that are asked for another step ahead, and its V at its
     // beginning, in the order in which they are waited for.
-    kv8_i4 K[4][2];
+    kv8_i4 K[4][NK];
     float r[16], ks, vs;     // of the step to come
     int near;
     int32_t ev, nk, nv;      // table entries: V's of that step, both of the next
@@ -390,7 +409,7 @@ struct Kv8Wave {
     __device__ __forceinline__ void walk(const Kv8Args &a, const Kv8Attn &b, const Kv8Plan &p, const Kv8Tile &t, int s0, int s1,
                                          int stride, int32_t ek) {
         if (s0 >= s1) return;
-        kv8_f4 q[8];
+        kv8_f4 q[4 * NK];
         load_q(a, b, q);
         ask(a, b, p, t.step0 + s0, page(a, ek), page(a, ev));
         digits(a, b, q);
@@ -398,7 +417,7 @@ struct Kv8Wave {
             const int at = t.step0 + i;
             int32_t mk, mv;
             entries(a, p, t, t.step0 + min(i + 2 * stride, s1 - 1), mk, mv);
-            kv8_i4 V[8];
+            kv8_i4 V[NC];
             load_v(a, page(a, ev), p.hk, at, V);
             float s[16];
             dots(K, s);
@@ -413,18 +432,40 @@ struct Kv8Wave {
     }
 };
 
+// Partials cross workgroups as relaxed agent-scope atomics (kv8_attn_run).
+__device__ __forceinline__ void kv8_put(float *p, kv8_f4 v) {
+    unsigned long long w[2];
+    __builtin_memcpy(w, &v, 16);
+    __hip_atomic_store((unsigned long long *)p, w[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store((unsigned long long *)p + 1, w[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ kv8_f4 kv8_get(const float *p) {
+    kv8_f4 v;
+    unsigned long long w[2];
+    w[0] = __hip_atomic_load((const unsigned long long *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    w[1] = __hip_atomic_load((const unsigned long long *)p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_memcpy(&v, w, 16);
+    return v;
+}
+__device__ __forceinline__ float *kv8_out(const Kv8Args &a, const Kv8Attn &b, const Kv8Plan &p, const Kv8Tile &t, int n) {
+    const int G = b.H / a.Hkv, ti = n / G;
+    return b.out + ((int64_t)(t.t0 + ti) * b.H + p.hk * G + (n - ti * G)) * a.Dh;
+}
+#define KV8_AHEAD 8   // partials whose loads are in flight at a time
+
 // Grid: the plan's runs, KV8_NW waves each.
-template <bool FULL>
+template <int D, bool FULL>
 __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b) {
-    __shared__ kv8_f4 so[KV8_NW][8][64];
+    __shared__ kv8_f4 so[KV8_NW][Kv8Wave<D, FULL>::NC][64];
     __shared__ float sm[KV8_NW][16], sl[KV8_NW][16];
     kv8_check(a);
     Kv8Plan p;
     if (!kv8_plan<false>(a, b, (int)blockIdx.x, p)) return;
-    const Kv8Tile t = kv8_tile(b, p);
-    const int span = (t.steps + p.splits - 1) / p.splits, s0 = p.x * span, s1 = min(t.steps, s0 + span);
-    const int w = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4, G = b.H / a.Hkv;
-    Kv8Wave<FULL> W;
+    const Kv8Tile t = kv8_tile(b, p, p.splits);
+    const int s0 = p.x * t.span, s1 = min(t.steps, s0 + t.span);
+    if (s0 >= s1) return;
+    const int w = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    Kv8Wave<D, FULL> W;
     int32_t ek;
     W.start(a, p, t, s0 + w, s1, KV8_NW, ek);
     W.init(a, b, t, p.hk);
@@ -435,7 +476,7 @@ __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b)
         sl[w][n] = l;
     }
 #pragma unroll
-    for (int ct = 0; ct < 8; ct++) so[w][ct][lane] = W.O[ct];
+    for (int ct = 0; ct < Kv8Wave<D, FULL>::NC; ct++) so[w][ct][lane] = W.O[ct];
     __syncthreads();
     // fold the waves: wave w takes dims 16 ct .. of ct = w, w + NW
     float M = -INFINITY, f[KV8_NW], L = 0.0f;
@@ -447,30 +488,82 @@ __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b)
         f[i] = __builtin_amdgcn_exp2f((sm[i][n] - ref) * KV8_L2E);
         L += sl[i][n] * f[i];
     }
-    const int ti = n / G;
-    if (ti >= t.nt) return;
-    const int64_t th = (int64_t)(t.t0 + ti) * b.H + p.hk * G + (n - ti * G);
     const int64_t slot = p.slot + (int64_t)p.x * a.Hkv;
-    for (int ct = w; 16 * ct < a.Dh; ct += KV8_NW) {
-        kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int rows = t.nt * (b.H / a.Hkv);
+    if (n < rows) {
+        float *out = kv8_out(a, b, p, t, n);
+        for (int ct = w; 16 * ct < a.Dh; ct += KV8_NW) {
+            kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < KV8_NW; i++) o += so[i][ct][lane] * f[i];
-        if (p.splits > 1) *(kv8_f4 *)(b.part + (slot * 16 + n) * a.Dh + 16 * ct + 4 * g) = o;
-        else *(kv8_f4 *)(b.out + th * a.Dh + 16 * ct + 4 * g) = o / L;
+            for (int i = 0; i < KV8_NW; i++) o += so[i][ct][lane] * f[i];
+            if (t.runs > 1) kv8_put(b.part + (slot * 16 + n) * a.Dh + 16 * ct + 4 * g, o);
+            else *(kv8_f4 *)(out + 16 * ct + 4 * g) = o / L;
+        }
     }
-    if (p.splits > 1 && w == 0 && g == 0) {
-        b.ml[slot * 32 + n] = M;
-        b.ml[slot * 32 + 16 + n] = L;
+    if (t.runs == 1) return;
+    if (w == 0 && g == 0) {
+        __hip_atomic_store(&b.ml[slot * 32 + n], M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&b.ml[slot * 32 + 16 + n], L, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (!b.arrived) return;
+    // The last of a unit's runs to arrive folds them, in their order. What
+    // crosses workgroups are relaxed agent-scope atomics: the wait and the
+    // barrier order the stores before the arrival, and the last arriver's loads
+    // come after its own (a release fence would write back the whole L2).
+    __shared__ uint32_t before;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0)
+        before = __hip_atomic_fetch_add(&b.arrived[p.slot], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (before + 1 != (uint32_t)t.runs) return;
+    if (threadIdx.x == 0) __hip_atomic_store(&b.arrived[p.slot], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int per = a.Dh / 4;
+    for (int i = (int)threadIdx.x; i < rows * per; i += 64 * KV8_NW) {
+        const int row = i / per, d = 4 * (i - row * per);
+        // the sums so far, relative to their maximum
+        float top = -INFINITY, sum = 0.0f;
+        kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int x0 = 0; x0 < t.runs; x0 += KV8_AHEAD) {
+            kv8_f4 v[KV8_AHEAD];
+            float vm[KV8_AHEAD], vl[KV8_AHEAD], mx = top;
+#pragma unroll
+            for (int j = 0; j < KV8_AHEAD; j++) {
+                const int64_t at = p.slot + (int64_t)min(x0 + j, t.runs - 1) * a.Hkv;
+                v[j] = kv8_get(b.part + (at * 16 + row) * a.Dh + d);
+                vm[j] = __hip_atomic_load(&b.ml[at * 32 + row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                vl[j] = __hip_atomic_load(&b.ml[at * 32 + 16 + row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+#pragma unroll
+            for (int j = 0; j < KV8_AHEAD; j++) mx = fmaxf(mx, vm[j]);
+            const float from = mx == -INFINITY ? 0.0f : mx, al = __builtin_amdgcn_exp2f((top - from) * KV8_L2E);
+            sum *= al;
+            o *= al;
+            top = mx;
+#pragma unroll
+            for (int j = 0; j < KV8_AHEAD; j++) {
+                const float e = x0 + j < t.runs ? __builtin_amdgcn_exp2f((vm[j] - from) * KV8_L2E) : 0.0f;
+                if (x0 + j < t.runs) {
+                    sum += vl[j] * e;
+                    o += v[j] * e;
+                }
+            }
+        }
+        *(kv8_f4 *)(kv8_out(a, b, p, t, row) + d) = o / sum;
     }
 }
-extern "C" __global__ __launch_bounds__(64 * KV8_NW, 2) void sepia_kv8_attn(Kv8Args a, Kv8Attn b) { kv8_attn_run<true>(a, b); }
-extern "C" __global__ __launch_bounds__(64 * KV8_NW, 2) void sepia_kv8_attn_d(Kv8Args a, Kv8Attn b) { kv8_attn_run<false>(a, b); }
+#define KV8_KERNEL(name, run, D, FULL) \
+    extern "C" __global__ __launch_bounds__(64 * KV8_NW, 2) void name(Kv8Args a, Kv8Attn b) { run<D, FULL>(a, b); }
+KV8_KERNEL(sepia_kv8_attn_128, kv8_attn_run, 128, true)
+KV8_KERNEL(sepia_kv8_attn_to128, kv8_attn_run, 128, false)
+KV8_KERNEL(sepia_kv8_attn_64, kv8_attn_run, 64, true)
+KV8_KERNEL(sepia_kv8_attn_to64, kv8_attn_run, 64, false)
 
 // Many rows (prompts): a wave a unit, KV8_NW row tiles of one kv head side by
 // side in a workgroup, so that they find K and V in the caches; nothing is cut
 // or folded. Grid: (ids of KV8_NW row tiles, kv heads), kv heads fastest, so
 // that with 8 of them an XCD's L2 holds one head's K and V.
-template <bool FULL>
+template <int D, bool FULL>
 __device__ __forceinline__ void kv8_attn_rows(const Kv8Args &a, const Kv8Attn &b) {
     kv8_check(a);
     Kv8Plan p;
@@ -480,48 +573,60 @@ __device__ __forceinline__ void kv8_attn_rows(const Kv8Args &a, const Kv8Attn &b
     if (p.s < 0) return;
     p.k = (id - (int)kv8_first_id(p.r0, p.s, gran, 1)) * KV8_NW + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     if ((int64_t)p.k * b.TT >= p.r1 - p.r0) return;
-    const Kv8Tile t = kv8_tile(b, p);
-    const int lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4, G = b.H / a.Hkv;
-    Kv8Wave<FULL> W;
+    const Kv8Tile t = kv8_tile(b, p, 1);
+    const int lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    Kv8Wave<D, FULL> W;
     int32_t ek;
     W.start(a, p, t, 0, t.steps, 1, ek);
     W.init(a, b, t, p.hk);
     W.walk(a, b, p, t, 0, t.steps, 1, ek);
     const float inv = 1.0f / kv8_sum_g(W.l);
-    const int ti = n / G;
-    if (ti >= t.nt) return;
-    float *o = b.out + ((int64_t)(t.t0 + ti) * b.H + p.hk * G + (n - ti * G)) * a.Dh + 4 * g;
+    if (n >= t.nt * (b.H / a.Hkv)) return;
+    float *o = kv8_out(a, b, p, t, n) + 4 * g;
 #pragma unroll
-    for (int ct = 0; ct < 8; ct++)
+    for (int ct = 0; ct < Kv8Wave<D, FULL>::NC; ct++)
         if (FULL || 16 * ct < a.Dh) *(kv8_f4 *)(o + 16 * ct) = W.O[ct] * inv;
 }
-extern "C" __global__ __launch_bounds__(64 * KV8_NW, 2) void sepia_kv8_rows(Kv8Args a, Kv8Attn b) { kv8_attn_rows<true>(a, b); }
-extern "C" __global__ __launch_bounds__(64 * KV8_NW, 2) void sepia_kv8_rows_d(Kv8Args a, Kv8Attn b) { kv8_attn_rows<false>(a, b); }
+KV8_KERNEL(sepia_kv8_rows_128, kv8_attn_rows, 128, true)
+KV8_KERNEL(sepia_kv8_rows_to128, kv8_attn_rows, 128, false)
+KV8_KERNEL(sepia_kv8_rows_64, kv8_attn_rows, 64, true)
+KV8_KERNEL(sepia_kv8_rows_to64, kv8_attn_rows, 64, false)
 
-// Folds the runs of every unit that was cut. Grid: as many units as may be cut,
-// rows of a tile. Eight groups of threads take a row's runs in turn, a thread
-// for 4 dims, and meet in LDS (one group after the other runs by itself, for
-// all rows in one workgroup, took 34 us at 63 runs).
+// Folds the runs of the units that were cut, where those are few and of many
+// runs each (one user's token over a long context): a workgroup a unit's row,
+// eight groups of threads that take its runs in turn, a thread for 4 dims.
+// Grid: (units that may be cut, rows of a tile).
 extern "C" __global__ __launch_bounds__(256) void sepia_kv8_fold(Kv8Args a, Kv8Attn b) {
     __shared__ kv8_f4 so[8][32];
     __shared__ float sl[8];
     Kv8Plan p;
     if (!kv8_plan<true>(a, b, (int)blockIdx.x, p)) return;
-    const Kv8Tile t = kv8_tile(b, p);
-    const int span = (t.steps + p.splits - 1) / p.splits, ns = (t.steps + span - 1) / span, G = b.H / a.Hkv;
-    const int n = (int)blockIdx.y, ti = n / G, j = (int)threadIdx.x >> 5, d = 4 * ((int)threadIdx.x & 31);
-    if (ti >= t.nt) return;
+    const Kv8Tile t = kv8_tile(b, p, p.splits);
+    const int n = (int)blockIdx.y, j = (int)threadIdx.x >> 5, d = 4 * ((int)threadIdx.x & 31);
+    if (t.runs == 1 || n >= t.nt * (b.H / a.Hkv)) return;
     float M = -INFINITY, L = 0.0f;
-    for (int x = (int)threadIdx.x & 63; x < ns; x += 64) M = fmaxf(M, b.ml[((int64_t)p.slot + (int64_t)x * a.Hkv) * 32 + n]);
+    for (int x = (int)threadIdx.x & 63; x < t.runs; x += 64) M = fmaxf(M, b.ml[((int64_t)p.slot + (int64_t)x * a.Hkv) * 32 + n]);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
     const float ref = M == -INFINITY ? 0.0f : M;
     kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int x = j; x < ns; x += 8) {
-        const int64_t slot = (int64_t)p.slot + (int64_t)x * a.Hkv;
-        const float f = __builtin_amdgcn_exp2f((b.ml[slot * 32 + n] - ref) * KV8_L2E);
-        L += b.ml[slot * 32 + 16 + n] * f;
-        if (d < a.Dh) o += *(const kv8_f4 *)(b.part + (slot * 16 + n) * a.Dh + d) * f;
+    for (int x0 = j; x0 < t.runs; x0 += 8 * KV8_AHEAD) {
+        kv8_f4 v[KV8_AHEAD];
+        float vm[KV8_AHEAD], vl[KV8_AHEAD];
+#pragma unroll
+        for (int i = 0; i < KV8_AHEAD; i++) {
+            const int64_t at = (int64_t)p.slot + (int64_t)min(x0 + 8 * i, t.runs - 1) * a.Hkv;
+            v[i] = *(const kv8_f4 *)(b.part + (at * 16 + n) * a.Dh + (d < a.Dh ? d : 0));
+            vm[i] = b.ml[at * 32 + n];
+            vl[i] = b.ml[at * 32 + 16 + n];
+        }
+#pragma unroll
+        for (int i = 0; i < KV8_AHEAD; i++) {
+            if (x0 + 8 * i >= t.runs) break;
+            const float f = __builtin_amdgcn_exp2f((vm[i] - ref) * KV8_L2E);
+            L += vl[i] * f;
+            o += v[i] * f;
+        }
     }
     so[j][d / 4] = o;
     if (d == 0) sl[j] = L;
@@ -534,5 +639,5 @@ extern "C" __global__ __launch_bounds__(256) void sepia_kv8_fold(Kv8Args a, Kv8A
         o += so[i][d / 4];
         L += sl[i];
     }
-    *(kv8_f4 *)(b.out + ((int64_t)(t.t0 + ti) * b.H + p.hk * G + (n - ti * G)) * a.Dh + d) = o / L;
+    *(kv8_f4 *)(kv8_out(a, b, p, t, n) + d) = o / L;
 }

@@ -107,8 +107,10 @@ static const char *const k_names[K_COUNT] = {
 /* Kernels of the second code object, sepia_serve.hsaco (the SK_* of
  * internal.h); their ids follow the first's. */
 static const char *const serve_names[SK_COUNT] = {
-    "sepia_kv8_append", "sepia_kv8_read", "sepia_kv8_attn", "sepia_kv8_attn_d", "sepia_kv8_rows", "sepia_kv8_rows_d",
-    "sepia_kv8_fold", "sepia_sample_max", "sepia_sample_bins", "sepia_sample_pick", "sepia_sample",
+    "sepia_kv8_append", "sepia_kv8_read",
+    "sepia_kv8_attn_128", "sepia_kv8_attn_to128", "sepia_kv8_attn_64", "sepia_kv8_attn_to64",
+    "sepia_kv8_rows_128", "sepia_kv8_rows_to128", "sepia_kv8_rows_64", "sepia_kv8_rows_to64", "sepia_kv8_fold",
+    "sepia_sample_max", "sepia_sample_bins", "sepia_sample_pick", "sepia_sample",
 };
 #define K_ALL (K_COUNT + SK_COUNT)
 static const char *k_name(int k) { return k < K_COUNT ? k_names[k] : serve_names[k - K_COUNT]; }
@@ -940,6 +942,8 @@ int sepia_chk(const SepiaGpuBuf *b, size_t off, size_t n, const char *op, const 
 int sepia_prep_in(SepiaGpuBuf *b, size_t off, size_t n, const char *op) { return prep_in_r(b, off, n, op); }
 int sepia_prep_out(SepiaGpuBuf *b, const char *op) { return prep_out(b, op); }
 void *sepia_scratch(size_t need, const char *op) { return scratch(need, op); }
+_Static_assert(SEPIA_COUNTERS * 4 == CNT_BYTES, "the counters fill their region");
+uint32_t *sepia_counters(void) { return (uint32_t *)g_scratch; }
 int sepia_serve_launch(int k, unsigned gx, unsigned gy, unsigned gz, unsigned block, void **args, const char *op) {
     return launch3(K_COUNT + k, gx, gy, gz, block, 0, args, op);
 }

@@ -151,11 +151,13 @@ int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *
 
 /* struct Kv8Attn of kernels/kv8_attn.h */
 #define KV8_ROWS 1024       /* units from which each has a wave of its own */
+#define KV8_RUNS 16         /* runs of a unit, on average, above which a launch folds them */
 #define KV8_BUDGET 512      /* runs of a call whose units alone leave the chip idle: two workgroups a CU */
 typedef struct {
     const float *q, *rel, *tau;
     float *out;
     float *part, *ml;
+    uint32_t *arrived;
     int32_t H, R, window, TT, budget;
     float c;
 } Kv8Attn;
@@ -200,11 +202,11 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
     /* 16 rows a wave. Many units (row tile, kv head): a wave each. Few: cut
      * into runs of steps, whose partials are folded. */
     b.TT = (int32_t)(16 / (n_heads / c->n_kv_heads));
-    const int full = c->head_dim == 128;
+    const int dim = 2 * (c->head_dim <= 64) + (c->head_dim % 64 != 0);   /* which of the four kernels */
     const int64_t units = (n / b.TT > c->n_seqs ? n / b.TT : n < c->n_seqs ? n : c->n_seqs) * c->n_kv_heads;
     if (units >= KV8_ROWS) {
         void *args[] = { &a, &b };
-        return sepia_serve_launch(full ? SK_KV8_ROWS : SK_KV8_ROWS_D, (unsigned)((n / (4 * b.TT) + c->n_seqs) * c->n_kv_heads),
+        return sepia_serve_launch(SK_KV8_ROWS + dim, (unsigned)((n / (4 * b.TT) + c->n_seqs) * c->n_kv_heads),
                                   1, 1, 256, args, op);
     }
     const int64_t ids = n / b.TT + c->n_seqs;
@@ -214,18 +216,20 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
         budget /= 2;
         slots = 2 * budget + 64;
     }
+    /* Units of many runs are folded by a launch of their own, of few by the
+     * run that ends last. */
+    const int fold = units * KV8_RUNS < budget;
     if (budget) {
         uint8_t *s = (uint8_t *)sepia_scratch((size_t)slots * (per + 128), op);
         if (!s) return 0;
         b.part = (float *)s;
         b.ml = (float *)(s + (size_t)slots * per);
+        if (!fold) b.arrived = sepia_counters();   /* slots of them: fewer than there are */
     }
     b.budget = (int32_t)budget;
     void *args[] = { &a, &b };
-    if (!sepia_serve_launch(full ? SK_KV8_ATTN : SK_KV8_ATTN_D, (unsigned)(budget + ids * c->n_kv_heads), 1, 1,
-                            256, args, op))
-        return 0;
-    if (!budget) return 1;
+    if (!sepia_serve_launch(SK_KV8_ATTN + dim, (unsigned)(budget + ids * c->n_kv_heads), 1, 1, 256, args, op)) return 0;
+    if (!fold) return 1;
     const int64_t cut = ids * c->n_kv_heads < budget ? ids * c->n_kv_heads : budget;
     return sepia_serve_launch(SK_KV8_FOLD, (unsigned)cut, 16, 1, 256, args, op);
 }
