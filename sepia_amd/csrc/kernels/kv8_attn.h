@@ -378,7 +378,6 @@ struct Kv8Wave {
         l += sum;
 #pragma unroll
         for (int ct = 0; ct < NC; ct++) {
-            if (!FULL && 16 * ct >= a.Dh) break;
             kv8_i4 d[3];
 #pragma unroll
             for (int p = 0; p < 3; p++) d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(V[ct], pd[p], kv8_i4{0, 0, 0, 0}, 0, 0, 0);

@@ -20,7 +20,7 @@
 // top-p border and the draw fall: each decision's bound gives the next one's,
 // a bin or a few in all. A second pass gathers the tokens of those bins, and
 // the three are decided in turn: a decision's bin is cut into 1024 pieces by
-// place in the order, its piece again while it has more than 64 tokens (equal
+// place in the order, its piece again while it has more than a few tokens (equal
 // logits: by index), and those few are compared with each other. Where the
 // gathered tokens are too many (flat rows, long runs of equal logits) the same
 // is done with passes over the row. (Sorting the gathered tokens by a network
@@ -41,6 +41,7 @@
 #define SAMPLE_WAVES (SAMPLE_NT / 64)
 #define SAMPLE_BINS 1024              // two a thread
 #define SAMPLE_CAP 4096               // gathered tokens
+#define SAMPLE_FEW 16                 // tokens that are compared with each other (60 of them took 4 us)
 
 // In scratch where a row has several chunks: a chunk's bins, and what the
 // row's workgroups gather.
@@ -123,7 +124,7 @@ struct SampleLds {
     // by bin, then by a bin's pieces; of the bins before
     unsigned long long mass[SAMPLE_BINS + 1], upto[SAMPLE_BINS + 1];
     uint32_t count[SAMPLE_BINS + 1], cupto[SAMPLE_BINS + 1];
-    unsigned long long list[SAMPLE_CAP], few[64];
+    unsigned long long list[SAMPLE_CAP], few[SAMPLE_FEW];
     unsigned long long wave[SAMPLE_WAVES], set[SAMPLE_BINS / 64];
     uint32_t n;
     SamplePow pow;
@@ -145,6 +146,10 @@ __device__ __forceinline__ void sample_walk(const float *__restrict__ x, int i0,
     }
 }
 
+__device__ __forceinline__ unsigned long long sample_lane(unsigned long long v, int l) {
+    return (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)v, l) |
+           (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32;
+}
 // Exclusive prefix sums over the workgroup's threads; the total too.
 __device__ __forceinline__ unsigned long long sample_scan(unsigned long long v, unsigned long long *wave,
                                                           unsigned long long &total) {
@@ -186,9 +191,9 @@ __device__ __forceinline__ void sample_clear(SampleLds &L) {
     for (int i = (int)threadIdx.x; i < SAMPLE_BINS; i += SAMPLE_NT) L.mass[i] = 0, L.count[i] = 0;
     __syncthreads();
 }
-// Prefix sums of L.mass and L.count, to `upto` and `cupto` (which may be the
-// same arrays).
-__device__ __forceinline__ void sample_prefix(SampleLds &L, unsigned long long *upto, uint32_t *cupto) {
+// Prefix sums of L.mass and, where counted, L.count, to `upto` and `cupto`
+// (which may be the same arrays).
+__device__ __forceinline__ void sample_prefix(SampleLds &L, unsigned long long *upto, uint32_t *cupto, bool counted) {
     const int b = 2 * (int)threadIdx.x;
     unsigned long long total;
     __syncthreads();
@@ -197,6 +202,10 @@ __device__ __forceinline__ void sample_prefix(SampleLds &L, unsigned long long *
     upto[b] = m;
     upto[b + 1] = m + m0;
     if (b == 0) upto[SAMPLE_BINS] = total;
+    if (!counted) {
+        __syncthreads();
+        return;
+    }
     const unsigned long long c = sample_scan(c0 + L.count[b + 1], L.wave, total);
     cupto[b] = (uint32_t)c;
     cupto[b + 1] = (uint32_t)(c + c0);
@@ -251,9 +260,9 @@ __device__ __forceinline__ float sample_most(const SampleAsk &q, int b) {
 // sums, and in L.set the bins that decide. Returns the least logit of those.
 __device__ __forceinline__ float sample_bounds(SampleAsk &q, SampleLds &L) {
     const int tid = (int)threadIdx.x;
-    sample_prefix(L, L.upto, L.cupto);
+    sample_prefix(L, L.upto, L.cupto, q.k > 0);
     const unsigned long long all = L.upto[SAMPLE_BINS];
-    q.by_k = q.k > 0 && (uint32_t)q.k < L.cupto[SAMPLE_BINS];
+    q.by_k = q.k > 0 && (uint32_t)q.k < L.cupto[SAMPLE_BINS];   // counts are there for a k alone
     q.by_p = q.p < 1.0f;
     // each decision's bin, or the range of bins that the one before leaves it
     unsigned long long lo = all, hi = all;   // the weight kept so far is in [lo, hi]
@@ -322,7 +331,7 @@ __device__ __forceinline__ SampleAt sample_settle(const SampleAsk &q, int b, boo
     const unsigned long long last = ((unsigned long long)sample_key(fmaxf(sample_least(q, b), -3.402823466e38f)) << 20) | 0xFFFFF;
     int bits = 64 - __builtin_clzll((last - first) | 1);
     uint32_t left = listed ? n : q.by_k ? L.cupto[b + 1] - L.cupto[b] : ~0u;   // at most (bins are counted for a k)
-    while (left > 64) {
+    while (left > SAMPLE_FEW) {
         const int drop = max(bits - 10, 0);
         sample_clear(L);
         walk([&](unsigned long long p, double z) {
@@ -331,7 +340,7 @@ __device__ __forceinline__ SampleAt sample_settle(const SampleAsk &q, int b, boo
             atomicAdd(&L.count[piece], 1u);
             atomicAdd(&L.mass[piece], sample_mass(z, L.pow));
         });
-        sample_prefix(L, L.mass, L.count);
+        sample_prefix(L, L.mass, L.count, true);
         const int piece = sample_seek(L.mass, L.count, by_count, over);
         over -= by_count ? L.count[piece] : L.mass[piece];
         before += L.mass[piece];
@@ -340,26 +349,38 @@ __device__ __forceinline__ SampleAt sample_settle(const SampleAsk &q, int b, boo
         bits = drop;
         __syncthreads();
     }
-    // at most 64 tokens: every wave compares them with each other
-    if (threadIdx.x == 0) L.n = 0;
-    __syncthreads();
-    walk([&](unsigned long long p, double) {
-        if ((p - first) >> bits == 0) L.few[atomicAdd(&L.n, 1u)] = p;
-    });
-    __syncthreads();
-    const int m = (int)L.n;
-    const unsigned long long p = lane < m ? L.few[lane] : SAMPLE_NONE;
-    const unsigned long long w = lane < m ? sample_mass(sample_log(sample_token(p), q.m, q.scale), L.pow) : 0;
+    // a few tokens: every wave compares them with each other
+    int m = (int)n;
+    unsigned long long p = SAMPLE_NONE, w = 0;
+    if (listed && n <= SAMPLE_FEW) {
+        if (lane < m) p = L.list[lane];
+    } else {
+        if (threadIdx.x == 0) L.n = 0;
+        __syncthreads();
+        walk([&](unsigned long long p, double) {
+            if ((p - first) >> bits == 0) L.few[atomicAdd(&L.n, 1u)] = p;
+        });
+        __syncthreads();
+        m = (int)L.n;
+        if (lane < m) p = L.few[lane];
+        __syncthreads();
+    }
+    bool here = p != SAMPLE_NONE;
+    if (here) {
+        const double z = sample_log(sample_token(p), q.m, q.scale);
+        here = sample_bin(z) == b;
+        if (here) w = sample_mass(z, L.pow);
+        else p = SAMPLE_NONE;
+    }
     unsigned long long cum = w, place = 1;
     for (int j = 0; j < m; j++) {
-        const unsigned long long pj = __shfl(p, j, 64), wj = __shfl(w, j, 64);
+        const unsigned long long pj = sample_lane(p, j), wj = sample_lane(w, j);
         cum += pj < p ? wj : 0;
         place += pj < p;
     }
-    const uint64_t hit = __ballot(lane < m && (by_count ? place == over + 1 : cum - w <= over && over < cum));
+    const uint64_t hit = __ballot(here && (by_count ? place == over + 1 : cum - w <= over && over < cum));
     const int l = hit ? __builtin_ctzll(hit) : 0;
-    __syncthreads();
-    return SampleAt{(unsigned long long)__shfl(p, l, 64), before + __shfl(cum, l, 64)};
+    return SampleAt{sample_lane(p, l), before + sample_lane(cum, l)};
 }
 // The decisions, from the gathered tokens where they fit L.list: the k-th
 // token, the top-p border, the draw.
