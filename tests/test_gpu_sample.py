@@ -67,7 +67,7 @@ def test_filters(dev, vocab, pad, rows, params):
     check(dev, logits(rng, rows, vocab, pad), vocab, rng.random(rows).astype(np.float32), **params)
 
 
-@pytest.mark.parametrize("rows,vocab", [(70, 3001), (300, 700), (2, 200003)])
+@pytest.mark.parametrize("rows,vocab", [(70, 3001), (300, 700), (2, 200003), (30, 30011), (600, 9001)])
 def test_mixed_rows(dev, rows, vocab):
     """Each row with filters of its own."""
     rng = np.random.default_rng(rows)
