@@ -30,6 +30,7 @@ struct Kv8Args {
     int64_t n_pages;
     int32_t n_seqs, max_pages, Hkv, Dh, lg, n;   // n: rows of the call
     uint32_t head_bytes, page_bytes;             // of a head's K or V in a page, of a page
+    int32_t gran, extra;                         // the id space of the pages (kv8_map.h)
     __device__ __forceinline__ int P() const { return 1 << lg; }
     __device__ __forceinline__ int8_t *k_codes(uint32_t page, int hk) const {
         return codes + (uint64_t)hk * head_bytes + (uint64_t)page * page_bytes;
@@ -49,6 +50,19 @@ __device__ __forceinline__ int kv8_seq(const Kv8Args &a, int s, int32_t &len, in
     r1 = a.starts[s + 1];
     return kv8_seq_ok(len, r0, r1, a.n, (int64_t)a.max_pages << a.lg);
 }
+// Kernel entry: the first BYTES of the arguments, a scalar load a 64-byte line,
+// waited for at once; else each group of them that a branch reads is a memory
+// round trip of its own. BYTES is at most the kernel's argument segment.
+template <int BYTES>
+__device__ __forceinline__ void serve_args() {
+    const __attribute__((address_space(4))) uint32_t *ka =
+        (const __attribute__((address_space(4))) uint32_t *)__builtin_amdgcn_kernarg_segment_ptr();
+    uint32_t acc = 0;
+#pragma unroll
+    for (int o = 0; o < BYTES; o += 64) acc ^= ka[o / 4];
+    asm volatile("" : : "s"(acc));
+}
+
 // The sequence that owns `id`, its length and rows; -1 if there is none, or
 // one that cannot be used. 64 sequences a look: one round for up to 64 of
 // them, with everything about the one found already loaded, two for 4096.
@@ -101,42 +115,84 @@ __device__ __forceinline__ uint32_t kv8_again(uint32_t word, double ratio) {
     return r;
 }
 
-// The unit's scale from each wave's largest value (bad: one is not finite),
-// and what its codes are multiplied with: the new rows' 1 / scale, the old
-// codes' old / new (1 where the scale did not grow).
+// 1 / v for a positive v of f32's range, within a rounding or two of 2^-53.
+__device__ __forceinline__ double kv8_rcp(double v) {
+    double r = __builtin_amdgcn_rcp(v);
+    r = __builtin_fma(__builtin_fma(-v, r, 1.0), r, r);
+    return __builtin_fma(__builtin_fma(-v, r, 1.0), r, r);
+}
+// Sum over the 8 lanes of a token; every lane gets it.
+__device__ __forceinline__ double kv8_sum8(double v) {
+#define KV8_SWAP(ctrl)                                                                                                  \
+    {                                                                                                                   \
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);                                                             \
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, ctrl, 0xF, 0xF, true);           \
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), ctrl, 0xF, 0xF, true);   \
+        v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);                                                       \
+    }
+    KV8_SWAP(0xB1)    // lanes 1 0 3 2
+    KV8_SWAP(0x4E)    // lanes 2 3 0 1
+    KV8_SWAP(0x141)   // the half row mirrored: the other four lanes
+#undef KV8_SWAP
+    return v;
+}
+// The largest of a value over the wave; every lane gets it.
+__device__ __forceinline__ float kv8_wave_max(float v) {
+#define KV8_ROR(n)                                                                                                   \
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 | n, 0xF, 0xF, true)))
+    KV8_ROR(8);
+    KV8_ROR(4);
+    KV8_ROR(2);
+    KV8_ROR(1);
+#undef KV8_ROR
+    const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    v = fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
+}
+
+// The unit's scale from its waves' largest values (bad: one is not finite; old:
+// the scale there was, 0 for none), and what its codes are multiplied with: the
+// new rows' 1 / scale, the old codes' old / new (1 where the scale did not
+// grow). `waves` waves are a unit.
 struct Kv8Scale {
     double inv, ratio;
 };
-__device__ __forceinline__ Kv8Scale kv8_rescale(float *scale, bool fresh, float most, bool bad) {
+__device__ __forceinline__ Kv8Scale kv8_rescale(float *scale, float old, float most, bool bad, int wave, int waves, bool mine) {
     __shared__ float red[4];
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+    const int w0 = wave & ~(waves - 1);
+    most = kv8_wave_max(most);
     if (__ballot(bad)) most = INFINITY;
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
-    const float old = fresh ? 0.0f : *scale;
+    if ((threadIdx.x & 63) == 0) red[wave] = most;
     __syncthreads();   // every wave has the old scale, and the maxima
-    for (unsigned w = 0; w < blockDim.x / 64; w++) most = fmaxf(most, red[w]);
+    for (int w = 0; w < waves; w++) most = fmaxf(most, red[w0 + w]);
     float s = fmaxf(old, most * (1.0f / 127.0f));
     if (!(s < INFINITY) || old != old) s = NAN;
-    if (threadIdx.x == 0) *scale = s;
+    if (mine && wave == w0 && (threadIdx.x & 63) == 0) *scale = s;
     Kv8Scale r;
-    r.inv = s > 0.0f ? 1.0 / (double)s : 0.0;
-    r.ratio = s > old && old > 0.0f ? (double)old / (double)s : 1.0;
+    r.inv = s > 0.0f ? kv8_rcp((double)s) : 0.0;
+    r.ratio = s > old && old > 0.0f ? (double)old * r.inv : 1.0;
     return r;
 }
 
-// Grid (ids, Hkv, 2: K and V), a wave for each 16 tokens of a page; gran = P,
-// extra = 2.
+// Grid (ids, kv heads / what a workgroup takes of them, 2: K and V), a wave for
+// each 16 tokens of a page: four heads a workgroup with pages of 16, two of 32,
+// one of 64 (a workgroup a head and page was as fast for one token and 20%
+// slower for 61).
 extern "C" __global__ __launch_bounds__(256, 4) void sepia_kv8_append(Kv8Args a, const float *__restrict__ k,
                                                                    const float *__restrict__ v,
                                                                    const float *__restrict__ norm, float eps) {
-    const int hk = (int)blockIdx.y, lane = (int)(threadIdx.x & 63), slot0 = (int)(threadIdx.x >> 6) * 16;
+    serve_args<64>();
+    const int waves = a.P() / 16, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)(threadIdx.x & 63);
+    const int head = (int)blockIdx.y * (4 / waves) + wave / waves, slot0 = (wave & (waves - 1)) * 16;
+    const int hk = min(head, a.Hkv - 1);
+    const bool mine = head < a.Hkv;   // else the wave only keeps the others company at the barrier
     kv8_check(a);
     int32_t len, r0, r1;
-    const int s = kv8_find(a, blockIdx.x, a.P(), 2, len, r0, r1);
+    const int s = kv8_find(a, blockIdx.x, a.gran, a.extra, len, r0, r1);
     Kv8Unit u;
     if (s < 0) return;
-    if (!kv8_unit(len, r0, r1, (int)(blockIdx.x - kv8_first_id(r0, s, a.P(), 2)), a.lg, &u)) return;
+    if (!kv8_unit(len, r0, r1, (int)(blockIdx.x - kv8_first_id(r0, s, a.gran, a.extra)), a.lg, &u)) return;
     const int page = kv8_page(a, s, u.page);
     if (page < 0) {
         sepia_report_error(nullptr, KV8_ERR_PAGE, (int)threadIdx.x);
@@ -147,99 +203,131 @@ extern "C" __global__ __launch_bounds__(256, 4) void sepia_kv8_append(Kv8Args a,
     bool bad = false;
     if (blockIdx.z == 0) {
         // K: 8 lanes a token, 8 tokens a pass; lane j of a token holds dims
-        // 32 i + 4 j .. + 3, so that every access of the eight is a whole line
+        // 32 i + 4 j .. + 3, so that every access of the eight is a whole line.
+        // A pass without new tokens is passed over.
         const int j = lane & 7;
+        const float old = u.s0 == 0 ? 0.0f : *a.scale(page, 0, hk);
         float x[2][16], w[16];
-        double rms[2];
+        double rms[2] = {1.0, 1.0};
+        bool some[2];
+#pragma unroll
+        for (int i = 0; i < 16; i++) w[i] = 1.0f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int d = 32 * i + 4 * j;
-            float4 t = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-            if (norm && d < a.Dh) t = *(const float4 *)(norm + d);
+            if (!norm) break;
+            const float4 t = *(const float4 *)(norm + (d < a.Dh ? d : 0));
             w[4 * i] = t.x, w[4 * i + 1] = t.y, w[4 * i + 2] = t.z, w[4 * i + 3] = t.w;
         }
 #pragma unroll
         for (int p = 0; p < 2; p++) {
-            const int slot = slot0 + 8 * p + (lane >> 3);
-            const bool on = slot >= u.s0 && slot < u.s1;
-            const float *row = k + (int64_t)(u.row + (on ? slot - u.s0 : 0)) * ld + (int64_t)hk * a.Dh;
-            double ss = 0.0;
+            some[p] = mine && slot0 + 8 * p < u.s1 && slot0 + 8 * p + 8 > u.s0;
+            if (!some[p]) continue;
+            const int slot = max(u.s0, min(u.s1 - 1, slot0 + 8 * p + (lane >> 3)));   // rows that repeat change nothing
+            const float *row = k + (int64_t)(u.row + slot - u.s0) * ld + (int64_t)hk * a.Dh;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int d = 32 * i + 4 * j;
-                float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (on && d < a.Dh) t = *(const float4 *)(row + d);
+                float4 t = *(const float4 *)(row + (d < a.Dh ? d : 0));
+                if (d >= a.Dh) t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 x[p][4 * i] = t.x, x[p][4 * i + 1] = t.y, x[p][4 * i + 2] = t.z, x[p][4 * i + 3] = t.w;
+            }
+        }
 #pragma unroll
-                for (int c = 0; c < 4; c++) ss = __builtin_fma((double)x[p][4 * i + c], (double)x[p][4 * i + c], ss);
+        for (int p = 0; p < 2; p++) {
+            if (!some[p]) continue;
+            if (norm) {
+                double ss[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+                for (int i = 0; i < 16; i++) ss[i & 3] = __builtin_fma((double)x[p][i], (double)x[p][i], ss[i & 3]);
+                rms[p] = rsqrt(kv8_sum8((ss[0] + ss[1]) + (ss[2] + ss[3])) / a.Dh + (double)eps);
             }
 #pragma unroll
-            for (int o = 1; o <= 4; o <<= 1) ss += __shfl_xor(ss, o, 64);
-            rms[p] = norm ? 1.0 / __builtin_sqrt(ss / a.Dh + (double)eps) : 1.0;
-#pragma unroll
             for (int i = 0; i < 16; i++) {
-                const float y = on ? (float)((double)x[p][i] * rms[p] * (double)w[i]) : 0.0f;
+                const float y = (float)((double)x[p][i] * rms[p] * (double)w[i]);
                 most = fmaxf(most, fabsf(y));
                 bad |= !(fabsf(y) < INFINITY);
             }
         }
-        const Kv8Scale sc = kv8_rescale(a.scale(page, 0, hk), u.s0 == 0, most, bad);
-        int8_t *c0 = a.k_codes(page, hk);
+        const Kv8Scale sc = kv8_rescale(a.scale(page, 0, hk), old, most, bad, wave, waves, mine);
+        if (!mine) return;
+        uint32_t *codes = (uint32_t *)(a.k_codes(page, hk) + (slot0 + (lane >> 3)) * a.Dh) + j;
+        if (sc.ratio != 1.0 && slot0 < u.s0) {   // the codes before the unit, all asked for before one is waited for
+            uint32_t c[2][4];
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) c[p][i] = codes[2 * p * a.Dh + (32 * i + 4 * j < a.Dh ? 8 * i : 0)];
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (slot0 + 8 * p + (lane >> 3) < u.s0 && 32 * i + 4 * j < a.Dh)
+                        codes[2 * p * a.Dh + 8 * i] = kv8_again(c[p][i], sc.ratio);
+        }
 #pragma unroll
         for (int p = 0; p < 2; p++) {
+            if (!some[p]) continue;
             const int slot = slot0 + 8 * p + (lane >> 3);
-            const bool on = slot >= u.s0 && slot < u.s1, again = slot < u.s0 && sc.ratio != 1.0;
-            uint32_t *c = (uint32_t *)(c0 + slot * a.Dh);
+            const bool on = slot >= u.s0 && slot < u.s1;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (32 * i + 4 * j >= a.Dh) continue;
-                if (on) {
-                    uint32_t word = 0;
+                uint32_t word = 0;
 #pragma unroll
-                    for (int b = 0; b < 4; b++)
-                        word |= kv8_code((double)x[p][4 * i + b] * rms[p] * (double)w[4 * i + b], sc.inv) << (8 * b);
-                    c[8 * i + j] = word;
-                } else if (again) {
-                    c[8 * i + j] = kv8_again(c[8 * i + j], sc.ratio);
-                }
+                for (int b = 0; b < 4; b++)
+                    word |= kv8_code((double)x[p][4 * i + b] * rms[p] * (double)w[4 * i + b], sc.inv) << (8 * b);
+                if (on && 32 * i + 4 * j < a.Dh) codes[2 * p * a.Dh + 8 * i] = word;
             }
         }
     } else {
-        // V: lane j holds dims 2 j and 2 j + 1 of 16 tokens, whose codes are 32
+        // V: lane j has dims 2 j and 2 j + 1 of 16 tokens, whose codes are 32
         // bytes of the page in a row
-        const int d = 2 * lane;
-        float x[2][16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int slot = slot0 + i;
-            float2 t = make_float2(0.0f, 0.0f);
-            if (slot >= u.s0 && slot < u.s1 && d < a.Dh)
-                t = *(const float2 *)(v + (int64_t)(u.row + slot - u.s0) * ld + (int64_t)hk * a.Dh + d);
-            x[0][i] = t.x, x[1][i] = t.y;
-            most = fmaxf(most, fmaxf(fabsf(t.x), fabsf(t.y)));
-            bad |= !(fabsf(t.x) < INFINITY) || !(fabsf(t.y) < INFINITY);
-        }
-        const Kv8Scale sc = kv8_rescale(a.scale(page, 1, hk), u.s0 == 0, most, bad);
-        if (d >= a.Dh || slot0 >= u.s1 || (slot0 + 16 <= u.s0 && sc.ratio == 1.0)) return;
+        const int d = 2 * lane, dd = d < a.Dh ? d : 0;
+        const float old = u.s0 == 0 ? 0.0f : *a.scale(page, 1, hk);
+        uint4 *codes[2], was[2];
         const bool whole = slot0 >= u.s0 && slot0 + 16 <= u.s1;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            uint4 *c = (uint4 *)(a.v_codes(page, hk) + ((int64_t)(d + e) << a.lg) + slot0);
-            const uint4 was = whole ? make_uint4(0, 0, 0, 0) : *c;
-            const uint32_t old[4] = {was.x, was.y, was.z, was.w};
-            uint32_t now[4];
+            codes[e] = (uint4 *)(a.v_codes(page, hk) + ((int64_t)(dd + e) << a.lg) + slot0);
+            if (!whole) was[e] = *codes[e];
+        }
+        // a slot's row, or the nearest of the unit's: loads without branches are
+        // in flight together
+        const float *rows = v + (int64_t)hk * a.Dh + dd;
+        float x[2][16];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t kept = sc.ratio != 1.0 ? kv8_again(old[i], sc.ratio) : old[i];
-                now[i] = 0;
+        for (int i = 0; i < 16; i++) {
+            const float2 t = *(const float2 *)(rows + (int64_t)(u.row + max(0, min(u.s1 - 1, slot0 + i) - u.s0)) * ld);
+            x[0][i] = t.x, x[1][i] = t.y;
+        }
+        if (d < a.Dh) {
 #pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    const int slot = slot0 + 4 * i + b;
-                    const uint32_t byte = slot < u.s0 ? kept >> (8 * b) : slot < u.s1 ? kv8_code((double)x[e][4 * i + b], sc.inv) : old[i] >> (8 * b);
-                    now[i] |= (byte & 0xFFu) << (8 * b);
-                }
+            for (int i = 0; i < 16; i++) {   // rows that repeat change nothing
+                most = fmaxf(most, fmaxf(fabsf(x[0][i]), fabsf(x[1][i])));
+                bad |= !(fabsf(x[0][i]) < INFINITY) || !(fabsf(x[1][i]) < INFINITY);
             }
-            *c = make_uint4(now[0], now[1], now[2], now[3]);
+        }
+        const Kv8Scale sc = kv8_rescale(a.scale(page, 1, hk), old, most, bad, wave, waves, mine);
+        if (!mine || d >= a.Dh || slot0 >= u.s1 || (slot0 + 16 <= u.s0 && sc.ratio == 1.0)) return;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            uint32_t now[4] = {was[e].x, was[e].y, was[e].z, was[e].w};
+            if (sc.ratio != 1.0)   // the old codes are the first; what lies behind the new ones stays
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int n = u.s0 - slot0 - 4 * i;   // old codes of the word
+                    if (n <= 0) continue;
+                    const uint32_t keep = n >= 4 ? 0u : ~0u << (8 * n);
+                    now[i] = (kv8_again(now[i], sc.ratio) & ~keep) | (now[i] & keep);
+                }
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int slot = slot0 + i;
+                const uint32_t at = 0xFFu << (8 * (i % 4));
+                if (slot >= u.s0 && slot < u.s1)
+                    now[i / 4] = (now[i / 4] & ~at) | kv8_code((double)x[e][i], sc.inv) << (8 * (i % 4));
+            }
+            *codes[e] = make_uint4(now[0], now[1], now[2], now[3]);
         }
     }
 }
@@ -249,13 +337,17 @@ extern "C" __global__ __launch_bounds__(256, 4) void sepia_kv8_append(Kv8Args a,
 // tokens of a page.
 extern "C" __global__ __launch_bounds__(256) void sepia_kv8_read(Kv8Args a, float *__restrict__ k,
                                                                  float *__restrict__ v) {
-    const int hk = (int)blockIdx.y, lane = (int)(threadIdx.x & 63), slot0 = (int)(threadIdx.x >> 6) * 16;
+    serve_args<64>();
+    const int waves = a.P() / 16, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)(threadIdx.x & 63);
+    const int head = (int)blockIdx.y * (4 / waves) + wave / waves, slot0 = (wave & (waves - 1)) * 16;
+    const int hk = head;
     kv8_check(a);
+    if (head >= a.Hkv) return;
     int32_t len, r0, r1;
-    const int s = kv8_find(a, blockIdx.x, a.P(), 2, len, r0, r1);
+    const int s = kv8_find(a, blockIdx.x, a.gran, a.extra, len, r0, r1);
     Kv8Unit u;
     if (s < 0) return;
-    if (!kv8_unit(len, r0, r1, (int)(blockIdx.x - kv8_first_id(r0, s, a.P(), 2)), a.lg, &u)) return;
+    if (!kv8_unit(len, r0, r1, (int)(blockIdx.x - kv8_first_id(r0, s, a.gran, a.extra)), a.lg, &u)) return;
     const int page = kv8_page(a, s, u.page);
     if (page < 0) {
         sepia_report_error(nullptr, KV8_ERR_PAGE, (int)threadIdx.x);

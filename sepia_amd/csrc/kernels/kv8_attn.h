@@ -457,6 +457,7 @@ template <int D, bool FULL>
 __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b) {
     __shared__ kv8_f4 so[KV8_NW][Kv8Wave<D, FULL>::NC][64];
     __shared__ float sm[KV8_NW][16], sl[KV8_NW][16];
+    serve_args<128>();
     kv8_check(a);
     Kv8Plan p;
     if (!kv8_plan<false>(a, b, (int)blockIdx.x, p)) return;
@@ -564,6 +565,7 @@ KV8_KERNEL(sepia_kv8_attn_to64, kv8_attn_run, 64, false)
 // that with 8 of them an XCD's L2 holds one head's K and V.
 template <int D, bool FULL>
 __device__ __forceinline__ void kv8_attn_rows(const Kv8Args &a, const Kv8Attn &b) {
+    serve_args<128>();
     kv8_check(a);
     Kv8Plan p;
     const int id = (int)blockIdx.x / a.Hkv, gran = KV8_NW * b.TT;
@@ -598,6 +600,7 @@ KV8_KERNEL(sepia_kv8_rows_to64, kv8_attn_rows, 64, false)
 extern "C" __global__ __launch_bounds__(256) void sepia_kv8_fold(Kv8Args a, Kv8Attn b) {
     __shared__ kv8_f4 so[8][32];
     __shared__ float sl[8];
+    serve_args<128>();
     Kv8Plan p;
     if (!kv8_plan<true>(a, b, (int)blockIdx.x, p)) return;
     const Kv8Tile t = kv8_tile(b, p, p.splits);

@@ -9,7 +9,8 @@
 // space that is fixed by n and the number of sequences alone: sequence s owns
 // the ids from starts[s] / gran + extra s up to the next sequence's, which
 // are at least as many as its units when a sequence of r rows has at most
-// r / gran + extra units. An id past a sequence's last unit has no work.
+// r / gran + extra units (pages touched: r / page + 2, and also r; row tiles of
+// t rows: r / t + 1). An id past a sequence's last unit has no work.
 #pragma once
 #include <stdint.h>
 

@@ -20,6 +20,7 @@ typedef struct {
     int64_t n_pages;
     int32_t n_seqs, max_pages, Hkv, Dh, lg, n;
     uint32_t head_bytes, page_bytes;
+    int32_t gran, extra;
 } Kv8Args;
 
 /* Checks a cache and a call's rows, and fills the kernels' arguments; `write`:
@@ -91,11 +92,16 @@ static int kv8_apart(const char *op, const SepiaKv8Cache *c, const SepiaGpuBuf *
     return 0;
 }
 
-/* Units of pages (kv8_map.h: a sequence of r rows touches at most r / page +
- * 2), kv heads, K and V; a wave for each 16 tokens of a page. */
-static int kv8_pages(int k, const SepiaKv8Cache *c, int64_t n, void **args, const char *op) {
-    return sepia_serve_launch(k, (unsigned)(n / c->page + 2 * (int64_t)c->n_seqs), (unsigned)c->n_kv_heads, 2,
-                              (unsigned)c->page * 4, args, op);
+/* Units of pages, kv heads, K and V; four waves, one for each 16 tokens of a
+ * page and head. A sequence of r > 0 rows touches at most r / page + 2 pages,
+ * and at most r: the id space (kv8_map.h) that is the smaller for the call
+ * (for a token a sequence it has an id a page and no others, which end at once
+ * but take places: 12.4 us with them at 61 sequences). */
+static int kv8_pages(int k, const SepiaKv8Cache *c, int64_t n, Kv8Args *a, void **args, const char *op) {
+    const int heads = 64 / c->page, few = n <= n / c->page + 2 * (int64_t)c->n_seqs;
+    a->gran = few ? 1 : c->page;
+    a->extra = few ? 0 : 2;
+    return sepia_serve_launch(k, (unsigned)(few ? n : n / c->page + 2 * (int64_t)c->n_seqs), (unsigned)((c->n_kv_heads + heads - 1) / heads), 2, 256, args, op);
 }
 
 int sepia_hip_kv8_append(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n, SepiaGpuBuf *k,
@@ -127,7 +133,7 @@ int sepia_hip_kv8_append(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf 
     const float *kp = (const float *)sepia_buf_dev(k), *vp = (const float *)sepia_buf_dev(v);
     const float *np = (const float *)sepia_buf_dev(k_norm);
     void *args[] = { &a, &kp, &vp, &np, &eps };
-    return kv8_pages(SK_KV8_APPEND, c, n, args, op);
+    return kv8_pages(SK_KV8_APPEND, c, n, &a, args, op);
 }
 
 int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *starts, int64_t n, SepiaGpuBuf *k,
@@ -146,7 +152,7 @@ int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *
     if (n == 0) return 1;
     float *kp = (float *)sepia_buf_dev(k), *vp = (float *)sepia_buf_dev(v);
     void *args[] = { &a, &kp, &vp };
-    return kv8_pages(SK_KV8_READ, c, n, args, op);
+    return kv8_pages(SK_KV8_READ, c, n, &a, args, op);
 }
 
 /* struct Kv8Attn of kernels/kv8_attn.h */

@@ -35,12 +35,13 @@ int main(void) {
         starts[n_seqs] = n;
         n += behind;
         unsigned char *seen = calloc(n + 1, 1);
-        const long ids = kv8_ids(n, n_seqs, P, 2);
+        const int gran = round % 2 ? P : 1, extra = round % 2 ? 2 : 0;   /* both id spaces of the pages */
+        const long ids = kv8_ids(n, n_seqs, gran, extra);
         for (long id = 0; id < ids; id++) {
-            const int s = find(starts, n_seqs, id, P, 2);
+            const int s = find(starts, n_seqs, id, gran, extra);
             Kv8Unit u;
             if (s < 0) continue;
-            if (!kv8_unit(lens[s], starts[s], starts[s + 1], (int)(id - kv8_first_id(starts[s], s, P, 2)), lg, &u)) continue;
+            if (!kv8_unit(lens[s], starts[s], starts[s + 1], (int)(id - kv8_first_id(starts[s], s, gran, extra)), lg, &u)) continue;
             if (u.s0 < 0 || u.s0 >= u.s1 || u.s1 > P) return 1;
             for (int i = u.s0; i < u.s1; i++) {
                 const int row = u.row + i - u.s0;
