@@ -67,8 +67,9 @@ class Cache:
         for p in range(lo, hi):
             page = self.table[s, p // self.page]
             for side in range(2):
-                out[side][p - lo] = (self.views(page)[side][p % self.page].astype(np.float64) *
-                                     self.scales[page, side][:, None].astype(np.float64))
+                with np.errstate(invalid="ignore"):   # a page may be NaN, and a code 0 of an infinite scale is
+                    out[side][p - lo] = (self.views(page)[side][p % self.page].astype(np.float64) *
+                                         self.scales[page, side][:, None].astype(np.float64))
         return out
 
     def attn(self, lens, starts, q, rel=None, tau=None, window=0, c=1.0, fill=np.nan):
