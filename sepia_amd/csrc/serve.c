@@ -309,8 +309,13 @@ int sepia_hip_sample(const SepiaSampleDesc *d, SepiaGpuBuf *logits, int64_t rows
     a.prob = (float *)sepia_buf_dev(prob);
     a.stride = stride;
     a.vocab = (int32_t)vocab;
-    /* chunks of a row: as many as the rows leave places for */
+    /* chunks of a row: as many as the rows leave places for. Two more launches
+     * cost 10 us, what one workgroup takes for 24000 logits: below three chunks
+     * a row stays whole (1 row, 127 rows in chunks against whole: 33, 39 against
+     * 27, 32 us of 11625 logits, 33, 48 against 32, 42 of 20000; 33, 52 against
+     * 40, 54 of 32000). */
     int64_t chunks = (vocab + SAMPLE_CHUNK - 1) / SAMPLE_CHUNK;
+    if (vocab < 3 * SAMPLE_CHUNK) chunks = 1;
     if (chunks > SAMPLE_PLACES / rows) chunks = SAMPLE_PLACES / rows;
     if (chunks > SAMPLE_CHUNKS) chunks = SAMPLE_CHUNKS;
     const size_t per = SAMPLE_ROW_BYTES + SAMPLE_CHUNK_BYTES * (size_t)(chunks > 0 ? chunks : 1);

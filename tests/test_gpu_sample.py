@@ -88,6 +88,19 @@ def test_equal_logits(dev, vocab):
         check(dev, x, vocab, u, exact_ties=True, **params)
 
 
+@pytest.mark.parametrize("vocab", [9000, 100003])
+def test_far_below_the_largest(dev, vocab):
+    """All tokens but one lie 14 to 60 octaves down, where bins are wider, then weigh nothing: borders on either side."""
+    rng = np.random.default_rng(vocab)
+    x = (-np.log(2.0) * np.where(rng.random((6, vocab)) < 500 / vocab, rng.uniform(14, 30, (6, vocab)),
+                                 rng.uniform(30, 60, (6, vocab)))).astype(np.float32)
+    x[:, vocab // 3] = 0.0
+    u = np.array([0.2, 0.999, 0.99, 0.9999, 1.0 - 2.0 ** -14, 0.97], np.float32)
+    for k in (0, 2, 300, vocab // 20, vocab // 2, vocab - 1):
+        for params in (dict(), dict(top_p=1.0 - 2.0 ** -9), dict(top_p=0.995, min_p=2.0 ** -15)):
+            check(dev, x, vocab, u, top_k=k, **params)
+
+
 def test_few_distinct_logits(dev):
     """Long runs of equal logits below a few others: the border falls inside a run."""
     rng = np.random.default_rng(4)
