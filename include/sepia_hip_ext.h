@@ -207,8 +207,11 @@ int sepia_hip_set_iq2xxs_grid(const uint64_t *grid256);
  * rows) to at least `bytes` now, so that later calls of the same or smaller
  * shapes allocate nothing. A call whose scratch would have to grow while the
  * stream is being captured fails instead (an allocation cannot be captured):
- * run the call once, or reserve, before beginning a capture. (banded_attn
- * takes fewer splits first, moe_prefill may run in parts, above.) Needs init. */
+ * run the call once, or reserve, before beginning a capture. (banded_attn and
+ * kv8_attn take fewer splits first, sample a workgroup a row; moe_prefill may
+ * run in parts, above.) A captured call's scratch stays until shutdown when a
+ * later call grows the region, so its graph may still be replayed; graphs are
+ * replayed on the library's stream, whose scratch they share. Needs init. */
 int sepia_hip_reserve_scratch(size_t bytes);
 
 /* Bytes of the library's growable scratch region (0 before its first use).

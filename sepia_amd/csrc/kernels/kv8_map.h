@@ -43,8 +43,9 @@ typedef struct {
 } Kv8Unit;
 KV8_FN int kv8_unit(int32_t len, int32_t r0, int32_t r1, int32_t k, int32_t lg, Kv8Unit *u) {
     if (r1 <= r0) return 0;
-    const int32_t end = len + (r1 - r0), page = (len >> lg) + k, base = page << lg;
+    const int32_t end = len + (r1 - r0), page = (len >> lg) + k;
     if (page > ((end - 1) >> lg)) return 0;
+    const int32_t base = page << lg;
     u->page = page;
     u->s0 = len > base ? len - base : 0;
     u->s1 = end - base < (1 << lg) ? end - base : (1 << lg);

@@ -384,26 +384,42 @@ static int prep_out(SepiaGpuBuf *b, const char *op) {
 #define CNT_BYTES (64u * 1024u)
 static void *g_scratch;
 static size_t g_scratch_len;
+static int g_scratch_held;                  /* a captured call has its address */
+static void *g_scratch_old[64];             /* held regions that were outgrown */
+static int g_scratch_olds;
 
 /* Data region of at least `need` bytes (the counters sit in front of it).
  * Growing waits for the stream, since queued kernels may still use the old
  * region; the new allocation is cleared so every counter starts at zero.
  * None of that may enter a stream capture: while the library's stream is
  * being captured a region that is too small is an error (run the same call
- * once before the capture, or reserve with sepia_hip_reserve_scratch). */
+ * once before the capture, or reserve with sepia_hip_reserve_scratch). A region
+ * that a captured call was given stays until the library shuts down, since its
+ * graph may be replayed after a later call has grown the scratch. */
 static void *scratch(size_t need, const char *op) {
-    if (g_scratch && need <= g_scratch_len - CNT_BYTES) return (uint8_t *)g_scratch + CNT_BYTES;
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(g_stream, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone) {
+    const int capturing = hipStreamIsCapturing(g_stream, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone;
+    if (g_scratch && need <= g_scratch_len - CNT_BYTES) {
+        g_scratch_held |= capturing;
+        return (uint8_t *)g_scratch + CNT_BYTES;
+    }
+    if (capturing) {
         LOG("%s: needs %zu bytes of scratch but has %zu, and the stream is being captured (growing it would "
             "allocate); run the call once before the capture or call sepia_hip_reserve_scratch",
             op, need, g_scratch ? g_scratch_len - CNT_BYTES : (size_t)0);
         return NULL;
     }
+    if (g_scratch_held && g_scratch_olds == (int)(sizeof g_scratch_old / sizeof *g_scratch_old)) {
+        LOG("%s: the scratch has been outgrown %d times with captured calls in it; reserve it before capturing", op,
+            g_scratch_olds);
+        return NULL;
+    }
     hipStreamSynchronize(g_stream);
-    if (g_scratch) hipFree(g_scratch);
+    if (g_scratch_held) g_scratch_old[g_scratch_olds++] = g_scratch;
+    else if (g_scratch) hipFree(g_scratch);
     g_scratch = NULL;
     g_scratch_len = 0;
+    g_scratch_held = 0;
     size_t want = CNT_BYTES + (need < (4u << 20) ? (4u << 20) : need);
     g_allocs++;
     hipError_t e = hipMalloc(&g_scratch, want);
@@ -821,8 +837,10 @@ void sepia_gpu_shutdown(void) {
     sepia_store_shutdown();
     pool_release_all();
     if (g_scratch) hipFree(g_scratch);
+    while (g_scratch_olds > 0) hipFree(g_scratch_old[--g_scratch_olds]);
     g_scratch = NULL;
     g_scratch_len = 0;
+    g_scratch_held = 0;
     unload_kernels();
     hipStreamDestroy(g_stream);
     g_available = 0;
@@ -944,8 +962,12 @@ int sepia_prep_out(SepiaGpuBuf *b, const char *op) { return prep_out(b, op); }
 void *sepia_scratch(size_t need, const char *op) { return scratch(need, op); }
 _Static_assert(SEPIA_COUNTERS * 4 == CNT_BYTES, "the counters fill their region");
 uint32_t *sepia_counters(void) { return (uint32_t *)g_scratch; }
-int sepia_serve_launch(int k, unsigned gx, unsigned gy, unsigned gz, unsigned block, void **args, const char *op) {
-    return launch3(K_COUNT + k, gx, gy, gz, block, 0, args, op);
+int sepia_serve_launch(int k, uint64_t gx, unsigned gy, unsigned gz, unsigned block, void **args, const char *op) {
+    if (gx * block > UINT32_MAX) {   /* HIP's limit of a launch's threads in x */
+        LOG("%s: %llu workgroups, more than a launch can have", op, (unsigned long long)gx);
+        return 0;
+    }
+    return launch3(K_COUNT + k, (unsigned)gx, gy, gz, block, 0, args, op);
 }
 
 static int launch2(int k, unsigned gx, unsigned gy, unsigned block, size_t lds, void **args, const char *op) {

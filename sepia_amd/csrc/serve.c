@@ -92,16 +92,15 @@ static int kv8_apart(const char *op, const SepiaKv8Cache *c, const SepiaGpuBuf *
     return 0;
 }
 
-/* Units of pages, kv heads, K and V; four waves, one for each 16 tokens of a
- * page and head. A sequence of r > 0 rows touches at most r / page + 2 pages,
- * and at most r: the id space (kv8_map.h) that is the smaller for the call
- * (for a token a sequence it has an id a page and no others, which end at once
- * but take places: 12.4 us with them at 61 sequences). */
+/* Units of pages, kv heads, K and V; a workgroup takes 64 tokens of the pages'
+ * heads. A sequence of r > 0 rows touches at most r / page + 2 pages,
+ * and at most r: the id space (kv8_map.h) that is the smaller for the call. */
 static int kv8_pages(int k, const SepiaKv8Cache *c, int64_t n, Kv8Args *a, void **args, const char *op) {
     const int heads = 64 / c->page, few = n <= n / c->page + 2 * (int64_t)c->n_seqs;
     a->gran = few ? 1 : c->page;
     a->extra = few ? 0 : 2;
-    return sepia_serve_launch(k, (unsigned)(few ? n : n / c->page + 2 * (int64_t)c->n_seqs), (unsigned)((c->n_kv_heads + heads - 1) / heads), 2, 256, args, op);
+    const uint64_t ids = (uint64_t)(few ? n : n / c->page + 2 * (int64_t)c->n_seqs);
+    return sepia_serve_launch(k, ids, (unsigned)((c->n_kv_heads + heads - 1) / heads), 2, 256, args, op);
 }
 
 int sepia_hip_kv8_append(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n, SepiaGpuBuf *k,
@@ -212,7 +211,7 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
     const int64_t units = (n / b.TT > c->n_seqs ? n / b.TT : n < c->n_seqs ? n : c->n_seqs) * c->n_kv_heads;
     if (units >= KV8_ROWS) {
         void *args[] = { &a, &b };
-        return sepia_serve_launch(SK_KV8_ROWS + dim, (unsigned)((n / (4 * b.TT) + c->n_seqs) * c->n_kv_heads),
+        return sepia_serve_launch(SK_KV8_ROWS + dim, (uint64_t)(n / (4 * b.TT) + c->n_seqs) * (uint64_t)c->n_kv_heads,
                                   1, 1, 256, args, op);
     }
     const int64_t ids = n / b.TT + c->n_seqs;
@@ -239,10 +238,10 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
     }
     b.budget = (int32_t)budget;
     void *args[] = { &a, &b };
-    if (!sepia_serve_launch(SK_KV8_ATTN + dim, (unsigned)(budget + ids * c->n_kv_heads), 1, 1, 256, args, op)) return 0;
+    if (!sepia_serve_launch(SK_KV8_ATTN + dim, (uint64_t)(budget + ids * c->n_kv_heads), 1, 1, 256, args, op)) return 0;
     if (!fold) return 1;
     const int64_t cut = ids * c->n_kv_heads < budget ? ids * c->n_kv_heads : budget;
-    return sepia_serve_launch(SK_KV8_FOLD, (unsigned)cut, 16, 1, 256, args, op);
+    return sepia_serve_launch(SK_KV8_FOLD, (uint64_t)cut, 16, 1, 256, args, op);
 }
 
 /* struct SampleArgs of kernels/sample.h, and the bytes of its SampleRow and
@@ -328,6 +327,6 @@ int sepia_hip_sample(const SepiaSampleDesc *d, SepiaGpuBuf *logits, int64_t rows
     if (!a.rows) return 0;
     a.bins = a.rows + (size_t)rows * SAMPLE_ROW_BYTES;
     for (int k = SK_SAMPLE_MAX; k <= SK_SAMPLE_PICK; k++)
-        if (!sepia_serve_launch(k, (unsigned)chunks, (unsigned)rows, 1, SAMPLE_NT, args, op)) return 0;
+        if (!sepia_serve_launch(k, (uint64_t)chunks, (unsigned)rows, 1, SAMPLE_NT, args, op)) return 0;
     return 1;
 }

@@ -204,6 +204,70 @@ def test_captured_step_follows_lengths(dev, H, heads, page, room):
         dev.free(b)
 
 
+def test_graphs_outlive_their_scratch(dev):
+    """Captured attention whose units are cut and sampling in chunks, replayed after later calls have grown the scratch
+    twice: the graph's region is still there, and its arrival counters. Bit for bit what the calls give eagerly."""
+    L, h = dev.L, Hip(dev)
+    rng = np.random.default_rng(14)
+    heads, dim, page, H, rows, vocab = 2, 64, 32, 16, 4, 40007
+    lens = [4000, 17, 900]
+    c, starts, n = make(rng, heads, dim, page, lens, [1, 1, 1])
+    c.table[c.table < 0] = 0
+    bufs, d = on_gpu(h, c)
+    q, x, u = normal(rng, n, H, dim), normal(rng, rows, vocab, scale=3.0), rng.random(rows).astype(np.float32)
+    lb, sb, qb, xb, ub = [h.private(a) for a in (np.array(lens, np.int32), np.array(starts, np.int32), q, x, u)]
+    ob, tb, pb = [dev.alloc(m, private=True) for m in (q.nbytes, 4 * rows, 4 * rows)]
+    desc = hip.SampleDesc(u=ub)
+    ops = (lambda: L.sepia_hip_kv8_attn(B(d), lb, sb, n, qb, None, None, ob, H, 0, 0, 1 / dim),
+           lambda: L.sepia_hip_sample(B(desc), xb, rows, vocab, vocab, tb, pb))
+
+    def results():
+        return [h.get(ob, q.shape).view(np.uint32), h.get(tb, rows, np.int32), h.get(pb, rows).view(np.uint32)]
+
+    def eager():
+        dev.begin()
+        assert [op() for op in ops] == [1, 1]
+        dev.end()
+
+    eager()
+    first = results()
+    want, tol = c.attn(lens, starts, q, None, None, 0, 1 / dim)
+    assert np.all(np.abs(h.get(ob, q.shape) - want) <= tol + np.abs(want) * 2.0 ** -23)
+    assert list(first[1]) == [sample(x[r], u[r])[0] for r in range(rows)]
+    graphs = [h.capture(*ops)]
+    for _ in range(2):
+        size = L.sepia_hip_scratch_bytes()
+        assert L.sepia_hip_reserve_scratch(size + 1) == 1 and L.sepia_hip_scratch_bytes() > size
+        graphs.append(h.capture(*ops))
+        for exe in graphs + graphs:
+            for b, m in ((ob, q.size), (tb, rows), (pb, rows)):
+                h.put(b, np.zeros(m, np.float32))
+            h.replay(exe)
+            assert all(np.array_equal(a, b) for a, b in zip(results(), first))
+            eager()
+            assert all(np.array_equal(a, b) for a, b in zip(results(), first))
+    assert L.sepia_hip_take_device_error() == 0
+    for e in graphs:
+        h.R.hipGraphExecDestroy(e)
+    for b in bufs + [lb, sb, qb, xb, ub, ob, tb, pb]:
+        dev.free(b)
+
+
+def test_grid_past_the_launch_limit(dev):
+    """65536 sequences of 300 kv heads: more workgroups than a launch can have; refused, not cut short."""
+    L = dev.L
+    n_seqs, heads = 65536, 300
+    bufs = [dev.alloc(m) for m in (2 * heads * 16 * 16, 2 * heads * 4, 4 * n_seqs, 4 * n_seqs, 4 * n_seqs + 4, 4 * heads * 16 * 4)]
+    d = hip.Kv8Cache(n_pages=1, max_pages=1, n_seqs=n_seqs, n_kv_heads=heads, head_dim=16, page=16, codes=bufs[0],
+                     scales=bufs[1], table=bufs[2])
+    dev.begin()
+    for n in (1, 4):
+        assert L.sepia_hip_kv8_attn(B(d), bufs[3], bufs[4], n, bufs[5], None, None, bufs[5], heads, 0, 0, 1.0) == 0
+    dev.end()
+    for b in bufs:
+        dev.free(b)
+
+
 CHILD = r"""
 import sys
 sys.path[:0] = [sys.argv[1], sys.argv[1] + "/tests"]
