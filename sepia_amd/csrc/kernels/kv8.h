@@ -177,9 +177,13 @@ __device__ __forceinline__ Kv8Scale kv8_rescale(float *scale, float old, float m
 
 // Grid (ids, kv heads / what a workgroup takes of them, 2: K and V), a wave for
 // each 16 tokens of a page: four heads a workgroup with pages of 16, two of 32,
-// one of 64 (a workgroup a head and page was as fast for one token and 20%
-// slower for 61).
-extern "C" __global__ __launch_bounds__(256, 4) void sepia_kv8_append(Kv8Args a, const float *__restrict__ k,
+// one of 64. What bounds it is the chain of dependent loads (arguments,
+// lengths, table entry, the old scale and codes) and the launch: 4.7 us for one
+// token (8 heads of 128), 8.6 for 61 sequences' tokens (16 heads), 19.9 for 5157
+// rows of prompts (8 heads; 53 MB, 2.7 TB/s). Twice as many waves of half the
+// work took 11.3 us for the 61 and as long for the prompts; four waves a SIMD in
+// the place of three spilled and took 8.9 and 20.6.
+extern "C" __global__ __launch_bounds__(256, 3) void sepia_kv8_append(Kv8Args a, const float *__restrict__ k,
                                                                    const float *__restrict__ v,
                                                                    const float *__restrict__ norm, float eps) {
     serve_args<64>();
@@ -193,11 +197,8 @@ extern "C" __global__ __launch_bounds__(256, 4) void sepia_kv8_append(Kv8Args a,
     Kv8Unit u;
     if (s < 0) return;
     if (!kv8_unit(len, r0, r1, (int)(blockIdx.x - kv8_first_id(r0, s, a.gran, a.extra)), a.lg, &u)) return;
+    // The rows are asked for before the table's entry is waited for.
     const int page = kv8_page(a, s, u.page);
-    if (page < 0) {
-        sepia_report_error(nullptr, KV8_ERR_PAGE, (int)threadIdx.x);
-        return;
-    }
     const int64_t ld = (int64_t)a.Hkv * a.Dh;
     float most = 0.0f;
     bool bad = false;
@@ -206,7 +207,6 @@ extern "C" __global__ __launch_bounds__(256, 4) void sepia_kv8_append(Kv8Args a,
         // 32 i + 4 j .. + 3, so that every access of the eight is a whole line.
         // A pass without new tokens is passed over.
         const int j = lane & 7;
-        const float old = u.s0 == 0 ? 0.0f : *a.scale(page, 0, hk);
         float x[2][16], w[16];
         double rms[2] = {1.0, 1.0};
         bool some[2];
@@ -233,6 +233,11 @@ extern "C" __global__ __launch_bounds__(256, 4) void sepia_kv8_append(Kv8Args a,
                 x[p][4 * i] = t.x, x[p][4 * i + 1] = t.y, x[p][4 * i + 2] = t.z, x[p][4 * i + 3] = t.w;
             }
         }
+        if (page < 0) {
+            sepia_report_error(nullptr, KV8_ERR_PAGE, (int)threadIdx.x);
+            return;
+        }
+        const float old = u.s0 == 0 ? 0.0f : *a.scale(page, 0, hk);
 #pragma unroll
         for (int p = 0; p < 2; p++) {
             if (!some[p]) continue;
@@ -283,14 +288,6 @@ extern "C" __global__ __launch_bounds__(256, 4) void sepia_kv8_append(Kv8Args a,
         // V: lane j has dims 2 j and 2 j + 1 of 16 tokens, whose codes are 32
         // bytes of the page in a row
         const int d = 2 * lane, dd = d < a.Dh ? d : 0;
-        const float old = u.s0 == 0 ? 0.0f : *a.scale(page, 1, hk);
-        uint4 *codes[2], was[2];
-        const bool whole = slot0 >= u.s0 && slot0 + 16 <= u.s1;
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            codes[e] = (uint4 *)(a.v_codes(page, hk) + ((int64_t)(dd + e) << a.lg) + slot0);
-            if (!whole) was[e] = *codes[e];
-        }
         // a slot's row, or the nearest of the unit's: loads without branches are
         // in flight together
         const float *rows = v + (int64_t)hk * a.Dh + dd;
@@ -299,6 +296,18 @@ extern "C" __global__ __launch_bounds__(256, 4) void sepia_kv8_append(Kv8Args a,
         for (int i = 0; i < 16; i++) {
             const float2 t = *(const float2 *)(rows + (int64_t)(u.row + max(0, min(u.s1 - 1, slot0 + i) - u.s0)) * ld);
             x[0][i] = t.x, x[1][i] = t.y;
+        }
+        if (page < 0) {
+            sepia_report_error(nullptr, KV8_ERR_PAGE, (int)threadIdx.x);
+            return;
+        }
+        const float old = u.s0 == 0 ? 0.0f : *a.scale(page, 1, hk);
+        uint4 *codes[2], was[2];
+        const bool whole = slot0 >= u.s0 && slot0 + 16 <= u.s1;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            codes[e] = (uint4 *)(a.v_codes(page, hk) + ((int64_t)(dd + e) << a.lg) + slot0);
+            if (!whole) was[e] = *codes[e];
         }
         if (d < a.Dh) {
 #pragma unroll
@@ -334,7 +343,7 @@ extern "C" __global__ __launch_bounds__(256, 4) void sepia_kv8_append(Kv8Args a,
 
 // ---------------------------------------------------------------- read -----
 // Rows of the cache as f32 (code * scale): the same units, a wave for each 16
-// tokens of a page.
+// tokens of a page. Bound by its writes from some thousand rows on.
 extern "C" __global__ __launch_bounds__(256) void sepia_kv8_read(Kv8Args a, float *__restrict__ k,
                                                                  float *__restrict__ v) {
     serve_args<64>();

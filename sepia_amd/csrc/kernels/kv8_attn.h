@@ -43,8 +43,7 @@ typedef float kv8_f4 __attribute__((ext_vector_type(4)));
 typedef kv8_f4 kv8_f4u __attribute__((aligned(4)));
 
 // Over the four lane groups (lanes n, n + 16, n + 32, n + 48): the halves of
-// the rows of 16 lanes change places, then the halves of the wave. (As LDS
-// permutes these four exchanges a step were waited for, 0.1 us each.)
+// the rows of 16 lanes change places, then the halves of the wave.
 template <class F>
 __device__ __forceinline__ float kv8_over_g(float v, F f) {
     const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
