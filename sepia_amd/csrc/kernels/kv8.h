@@ -18,6 +18,7 @@
 #pragma once
 #include "common.h"
 #include "kv8_map.h"
+#include "serve.h"
 
 #define KV8_ERR_PAGE 6u   // device error: a page of the table outside the pool
 #define KV8_ERR_SEQ 7u    // device error: lens or starts that do not fit the call
@@ -49,18 +50,6 @@ __device__ __forceinline__ int kv8_seq(const Kv8Args &a, int s, int32_t &len, in
     r0 = a.starts[s];
     r1 = a.starts[s + 1];
     return kv8_seq_ok(len, r0, r1, a.n, (int64_t)a.max_pages << a.lg);
-}
-// Kernel entry: the first BYTES of the arguments, a scalar load a 64-byte line,
-// waited for at once; else each group of them that a branch reads is a memory
-// round trip of its own. BYTES is at most the kernel's argument segment.
-template <int BYTES>
-__device__ __forceinline__ void serve_args() {
-    const __attribute__((address_space(4))) uint32_t *ka =
-        (const __attribute__((address_space(4))) uint32_t *)__builtin_amdgcn_kernarg_segment_ptr();
-    uint32_t acc = 0;
-#pragma unroll
-    for (int o = 0; o < BYTES; o += 64) acc ^= ka[o / 4];
-    asm volatile("" : : "s"(acc));
 }
 
 // The sequence that owns `id`, its length and rows; -1 if there is none, or

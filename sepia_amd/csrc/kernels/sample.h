@@ -36,6 +36,7 @@
 // out at the memory's side.)
 #pragma once
 #include "common.h"
+#include "serve.h"
 
 #define SAMPLE_ONE 8796093022208.0    // 2^43: the largest weight
 #define SAMPLE_NT 512                 // two workgroups a CU (of 1024 threads one: 36 against 26 us at 48 rows)
@@ -235,7 +236,7 @@ __device__ __forceinline__ int sample_seek(const unsigned long long *upto, const
 // What a row asks for, as its workgroups need it.
 struct SampleAsk {
     const float *x;
-    float m, p, u;
+    float m, t, p, f, u;           // largest logit, temperature, top-p, min-p (0: off), u
     int vocab, k;
     double scale;
     unsigned long long over_min;   // the weight of its tokens of w >= min-p (no min-p: the largest number)
@@ -426,35 +427,40 @@ __device__ __forceinline__ unsigned long long sample_first(const SampleArgs &a, 
     if ((int)threadIdx.x < a.chunks) best = a.bins[(int64_t)row * a.chunks + (int)threadIdx.x].best;
     return sample_min(best, wave);
 }
-// Whether the row's first token is all there is to decide; the workgroup of
-// `write` says so.
-__device__ __forceinline__ bool sample_done(const SampleArgs &a, int row, unsigned long long best, bool write) {
-    const float temperature = a.temperature ? a.temperature[row] : 1.0f;
-    if (best != SAMPLE_NONE && temperature > 0.0f && !(a.top_k && a.top_k[row] == 1)) return false;
+// A row's parameters: loads without branches, in flight together at a kernel's
+// entry (what is not there is read from u, and the value that is off taken).
+__device__ __forceinline__ SampleAsk sample_ask(const SampleArgs &a, int row) {
+    SampleAsk q;
+    const float t = (a.temperature ? a.temperature : a.u)[row], p = (a.top_p ? a.top_p : a.u)[row];
+    const float f = (a.min_p ? a.min_p : a.u)[row];
+    const int k = (a.top_k ? a.top_k : (const int32_t *)a.u)[row];
+    q.u = a.u[row];
+    q.x = a.logits + (int64_t)row * a.stride;
+    q.vocab = a.vocab;
+    q.t = a.temperature ? t : 1.0f;
+    q.p = a.top_p ? p : 1.0f;
+    q.f = a.min_p && f > 0.0f ? fminf(f, 1.0f) : 0.0f;
+    q.k = a.top_k ? k : 0;
+    q.over_min = ~0ull;
+    return q;
+}
+// From the row's first token its largest logit and scale; whether that token is
+// all there is to decide (the workgroup of `write` says so).
+__device__ __forceinline__ bool sample_done(const SampleArgs &a, int row, SampleAsk &q, unsigned long long best, bool write) {
+    q.m = sample_logit((uint32_t)(best >> 20));
+    q.scale = 256.0 * 1.4426950408889634074 / (double)q.t;
+    if (best != SAMPLE_NONE && q.t > 0.0f && q.k != 1) return false;
     if (write && threadIdx.x == 0) {
         a.token[row] = best == SAMPLE_NONE ? -1 : (int32_t)(best & 0xFFFFF);
         if (a.prob) a.prob[row] = best == SAMPLE_NONE ? 0.0f : 1.0f;
     }
     return true;
 }
-__device__ __forceinline__ SampleAsk sample_ask(const SampleArgs &a, int row, unsigned long long best) {
-    SampleAsk q;
-    q.x = a.logits + (int64_t)row * a.stride;
-    q.m = sample_logit((uint32_t)(best >> 20));
-    q.vocab = a.vocab;
-    q.k = a.top_k ? a.top_k[row] : 0;
-    q.p = a.top_p ? a.top_p[row] : 1.0f;
-    q.u = a.u[row];
-    q.scale = 256.0 * 1.4426950408889634074 / (double)(a.temperature ? a.temperature[row] : 1.0f);
-    q.over_min = ~0ull;
-    return q;
-}
 // The bins of the row's tokens i0 .. i1 - 1 in L.mass and, where its k may
 // cut, L.count; q.over_min.
-__device__ __forceinline__ void sample_bins(const SampleArgs &a, int row, SampleAsk &q, int i0, int i1, SampleLds &L) {
+__device__ __forceinline__ void sample_bins(SampleAsk &q, int i0, int i1, SampleLds &L) {
     const int tid = (int)threadIdx.x;
-    const float min_p = a.min_p && a.min_p[row] > 0.0f ? fminf(a.min_p[row], 1.0f) : 0.0f;
-    const unsigned long long floor_mass = min_p > 0.0f ? (unsigned long long)__builtin_ceil((double)min_p * SAMPLE_ONE) : 0;
+    const unsigned long long floor_mass = q.f > 0.0f ? (unsigned long long)__builtin_ceil((double)q.f * SAMPLE_ONE) : 0;
     L.pow.fill();
     sample_clear(L);
     unsigned long long tail = 0, over_min = 0, tails, ntails;
@@ -489,6 +495,7 @@ __device__ __forceinline__ void sample_bins(const SampleArgs &a, int row, Sample
 // cleared.
 extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_max(SampleArgs a) {
     __shared__ unsigned long long wave[SAMPLE_WAVES];
+    serve_args<64>();
     const int c = (int)blockIdx.x, row = (int)blockIdx.y;
     const unsigned long long best =
         sample_best(a.logits + (int64_t)row * a.stride, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), wave);
@@ -500,11 +507,11 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_max(SampleA
 // Grid (chunks, rows): the chunk's bins.
 extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_bins(SampleArgs a) {
     __shared__ SampleLds L;
+    serve_args<64>();
     const int c = (int)blockIdx.x, row = (int)blockIdx.y, tid = (int)threadIdx.x;
-    const unsigned long long best = sample_first(a, row, L.wave);
-    if (sample_done(a, row, best, c == 0)) return;
-    SampleAsk q = sample_ask(a, row, best);
-    sample_bins(a, row, q, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), L);
+    SampleAsk q = sample_ask(a, row);
+    if (sample_done(a, row, q, sample_first(a, row, L.wave), c == 0)) return;
+    sample_bins(q, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), L);
     SampleChunk *o = a.bins + (int64_t)row * a.chunks + c;
     for (int b = tid; b < SAMPLE_BINS; b += SAMPLE_NT) {
         o->mass[b] = L.mass[b];
@@ -516,10 +523,10 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_bins(Sample
 // Grid (chunks, rows): the decision, over the chunks' bins.
 extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_pick(SampleArgs a) {
     __shared__ SampleLds L;
+    serve_args<64>();
     const int c = (int)blockIdx.x, row = (int)blockIdx.y, tid = (int)threadIdx.x;
-    const unsigned long long best = sample_first(a, row, L.wave);
-    if (sample_done(a, row, best, false)) return;
-    SampleAsk q = sample_ask(a, row, best);
+    SampleAsk q = sample_ask(a, row);
+    if (sample_done(a, row, q, sample_first(a, row, L.wave), false)) return;
     const SampleChunk *o = a.bins + (int64_t)row * a.chunks;
     unsigned long long mass[2] = {0, 0}, over_min = 0;
     uint32_t count[2] = {0, 0};
@@ -582,11 +589,11 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_pick(Sample
 // Grid (1, rows): a row by one workgroup.
 extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample(SampleArgs a) {
     __shared__ SampleLds L;
+    serve_args<64>();
     const int row = (int)blockIdx.y;
-    const unsigned long long best = sample_best(a.logits + (int64_t)row * a.stride, 0, a.vocab, L.wave);
-    if (sample_done(a, row, best, true)) return;
-    SampleAsk q = sample_ask(a, row, best);
-    sample_bins(a, row, q, 0, a.vocab, L);
+    SampleAsk q = sample_ask(a, row);
+    if (sample_done(a, row, q, sample_best(q.x, 0, a.vocab, L.wave), true)) return;
+    sample_bins(q, 0, a.vocab, L);
     const float least = sample_bounds(q, L);
     sample_gather(q, least, 0, a.vocab, L);
     sample_finish(a, row, q, L.n, L);
