@@ -169,9 +169,20 @@ __device__ __forceinline__ float kv8_join(int32_t hi, int32_t mid, int32_t lo) {
     return __builtin_fmaf((float)hi, 65536.0f, (float)(int32_t)(((uint32_t)mid << 8) + (uint32_t)lo));
 }
 
+// A wave's place for a step's rel_logits; rows 272 bytes apart, so that 16 rows'
+// 16-byte pieces lie in different banks.
+struct Kv8Rel {
+    alignas(16) float at[16][68];
+};
+// A value that is the same in all lanes, in scalar registers.
+__device__ __forceinline__ int64_t kv8_same(int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32);
+}
+
 // One wave's 16 rows of D dims (FULL), or of up to D (a.Dh). NK: K operands a
-// row (64 dims each), NC: tiles of 16 dims.
-template <int D, bool FULL>
+// row (64 dims each), NC: tiles of 16 dims. LINES: rel_logits by whole rows.
+template <int D, bool FULL, bool LINES>
 struct Kv8Wave {
     static constexpr int NK = D / 64, NC = D / 16;
     static __device__ __forceinline__ int dh(const Kv8Args &a) { return FULL ? D : a.Dh; }
@@ -183,6 +194,12 @@ struct Kv8Wave {
     bool on;                // whether there is a row n
     const float *rel;       // row n's rel_logits
     int32_t rpos, R;        // pos, for an inactive row some active one's; the band
+    // LINES: the element of the first row and column 0, the first and the last
+    // step whose elements all rows' lie inside the buffer, and this lane's four
+    // pieces, bytes behind the first row
+    int64_t rel0;
+    int32_t rel_s0, rel_s1;
+    uint32_t piece[4];
     int32_t lo_max, pos_min;   // over the active rows
 
     __device__ __forceinline__ void init(const Kv8Args &a, const Kv8Attn &b, const Kv8Tile &t, int hk) {
@@ -195,6 +212,22 @@ struct Kv8Wave {
         rel = b.rel ? b.rel + th * b.R : nullptr;
         rpos = on ? pos : t.pos0;
         R = b.R;
+        if (LINES && b.rel) {
+            // elements of the buffer before and behind the tile's first and last
+            // row's column 0; a step needs 63 + 64 step of them before
+            const int rows = t.nt * G, gi = (rows - 1) % G;
+            const int64_t before = ((int64_t)t.t0 * b.H + hk * G) * b.R + t.pos0;
+            const int64_t span = ((int64_t)(t.nt - 1) * b.H + gi) * b.R + t.nt - 1;
+            const int64_t behind = (int64_t)a.n * b.H * b.R - 1 - before - span;
+            rel0 = kv8_same(before);
+            rel_s0 = behind >= 0 ? 0 : (int32_t)min((int64_t)0x7FFFFFFF, (63 - behind) >> 6);
+            rel_s1 = before < 63 || span > 0x1FFFFFFF ? -1 : (int32_t)min((int64_t)0x7FFFFFFF, (before - 63) >> 6);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int row = 4 * i + ((int)(threadIdx.x & 63) >> 4), r = row < rows ? row : 0, ri = r / G;
+                piece[i] = 4u * ((uint32_t)(ri * b.H + r - ri * G) * (uint32_t)b.R + (uint32_t)ri + 4u * (threadIdx.x & 15));
+            }
+        }
         lo_max = b.window > 0 ? max(0, t.last - b.window + 1) : 0;
         pos_min = t.pos0;
         m = -INFINITY;
@@ -279,13 +312,31 @@ struct Kv8Wave {
 #pragma unroll
         for (int ct = 0; ct < NC; ct++) V[ct] = *(const kv8_i4 *)(v + ((int64_t)(FULL || 16 * ct < dh(a) ? 16 * ct : 0) << a.lg));
     }
-    // rel_logits of row n and column 16 g + j of a step in r[15 - j], where the
-    // row sees the column and its band reaches it. 0: no such column in the
+    // rel_logits of row n and column 16 g + j of a step, where the row sees the
+    // column and its band reaches it, in r[15 - j]. 0: no such column in the
     // step, 1: all are, 2: some are not. (A branch and a load a column, waited
     // for one after the other, were most of a step: 5.5 us.)
+    // LINES: a lane's own 16 elements are a quarter of the lines that each load
+    // touches, and every line is asked for four times. So the step's 64 elements
+    // of each row are loaded side by side, r[4 i + e] being element 4 (lane % 16)
+    // + e of row 4 i + lane / 16 (5: all in the bands, 6: not all), and
+    // spread_rel() brings them to the lanes that want them: a chunk of 500 rows
+    // 115 -> 104 us, of which 22 and 11 for rel_logits. Not where those would lie
+    // outside the buffer, nor in the kernels of few rows (16.7 -> 20.4 us at dim
+    // 64, whose third wave a SIMD it costs; as long as before at 128).
     __device__ __forceinline__ int load_rel(const Kv8Attn &b, int step, float (&r)[16]) const {
-        const int d0 = rpos - (64 * step + 16 * ((int)(threadIdx.x & 63) >> 4));
         if (!b.rel || pos_min - (64 * step + 63) >= b.R) return 0;
+        const int d0 = rpos - (64 * step + 16 * ((int)(threadIdx.x & 63) >> 4));
+        if (LINES && step >= rel_s0 && step <= rel_s1) {
+            const char *from = (const char *)(b.rel + (rel0 - 64 * (int64_t)__builtin_amdgcn_readfirstlane(step) - 63));
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const kv8_f4 x = *(const kv8_f4u *)(from + piece[i]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) r[4 * i + e] = x[e];
+            }
+            return __ballot(d0 < 15 || d0 >= b.R) == 0 ? 5 : 6;
+        }
         if (__ballot(d0 < 15 || d0 >= b.R) == 0) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -298,6 +349,22 @@ struct Kv8Wave {
 #pragma unroll
         for (int j = 0; j < 16; j++) r[15 - j] = rel[max(0, min(b.R - 1, d0 - j))];
         return 2;
+    }
+    // r[15 - j] from the pieces, through the wave's own rows of shared memory.
+    __device__ __forceinline__ void spread_rel(Kv8Rel &rows) {
+        const int lane = (int)(threadIdx.x & 63);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            *(kv8_f4 *)&rows.at[4 * i + (lane >> 4)][4 * (lane & 15)] = kv8_f4{r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]};
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const kv8_f4 x = *(const kv8_f4 *)&rows.at[lane & 15][48 - 16 * (lane >> 4) + 4 * i];
+#pragma unroll
+            for (int e = 0; e < 4; e++) r[4 * i + e] = x[e];
+        }
     }
     // Scores' digit sums of a step.
     __device__ __forceinline__ void dots(const kv8_i4 (&K)[4][NK], float (&s)[16]) const {
@@ -314,12 +381,13 @@ struct Kv8Wave {
         }
     }
     // Scores from their digit sums.
-    __device__ __forceinline__ void scores(int step, float (&s)[16]) {
+    __device__ __forceinline__ void scores(int step, float (&s)[16], Kv8Rel *rows) {
         const int d0 = rpos - (64 * step + 16 * ((int)(threadIdx.x & 63) >> 4));
         const float sc = qs * ks;
 #pragma unroll
         for (int j = 0; j < 16; j++) s[j] *= sc;
-        if (near == 2) {
+        if (LINES && (near & 4)) spread_rel(*rows);
+        if (near & 2) {
 #pragma unroll
             for (int j = 0; j < 16; j++) r[15 - j] = d0 - j < R ? r[15 - j] : 0.0f;
         }
@@ -405,7 +473,7 @@ struct Kv8Wave {
         entries(a, p, t, t.step0 + min(s0 + stride, s1 - 1), nk, nv);
     }
     __device__ __forceinline__ void walk(const Kv8Args &a, const Kv8Attn &b, const Kv8Plan &p, const Kv8Tile &t, int s0, int s1,
-                                         int stride, int32_t ek) {
+                                         int stride, int32_t ek, Kv8Rel *rows) {
         if (s0 >= s1) return;
         kv8_f4 q[4 * NK];
         load_q(a, b, q);
@@ -419,7 +487,7 @@ struct Kv8Wave {
             load_v(a, page(a, ev), p.hk, at, V);
             float s[16];
             dots(K, s);
-            scores(at, s);
+            scores(at, s, rows);
             const float vs_i = vs;
             if (i + stride < s1) ask(a, b, p, at + stride, page(a, nk), page(a, nv));
             step(a, at, s, vs_i, V);
@@ -454,7 +522,7 @@ __device__ __forceinline__ float *kv8_out(const Kv8Args &a, const Kv8Attn &b, co
 // Grid: the plan's runs, KV8_NW waves each.
 template <int D, bool FULL>
 __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b) {
-    __shared__ kv8_f4 so[KV8_NW][Kv8Wave<D, FULL>::NC][64];
+    __shared__ kv8_f4 so[KV8_NW][Kv8Wave<D, FULL, false>::NC][64];
     __shared__ float sm[KV8_NW][16], sl[KV8_NW][16];
     serve_args<128>();
     kv8_check(a);
@@ -464,18 +532,18 @@ __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b)
     const int s0 = p.x * t.span, s1 = min(t.steps, s0 + t.span);
     if (s0 >= s1) return;
     const int w = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    Kv8Wave<D, FULL> W;
+    Kv8Wave<D, FULL, false> W;
     int32_t ek;
     W.start(a, p, t, s0 + w, s1, KV8_NW, ek);
     W.init(a, b, t, p.hk);
-    W.walk(a, b, p, t, s0 + w, s1, KV8_NW, ek);
+    W.walk(a, b, p, t, s0 + w, s1, KV8_NW, ek, nullptr);
     const float l = kv8_sum_g(W.l);
     if (g == 0) {
         sm[w][n] = W.m;
         sl[w][n] = l;
     }
 #pragma unroll
-    for (int ct = 0; ct < Kv8Wave<D, FULL>::NC; ct++) so[w][ct][lane] = W.O[ct];
+    for (int ct = 0; ct < Kv8Wave<D, FULL, false>::NC; ct++) so[w][ct][lane] = W.O[ct];
     __syncthreads();
     // fold the waves: wave w takes dims 16 ct .. of ct = w, w + NW
     float M = -INFINITY, f[KV8_NW], L = 0.0f;
@@ -564,6 +632,7 @@ KV8_KERNEL(sepia_kv8_attn_to64, kv8_attn_run, 64, false)
 // that with 8 of them an XCD's L2 holds one head's K and V.
 template <int D, bool FULL>
 __device__ __forceinline__ void kv8_attn_rows(const Kv8Args &a, const Kv8Attn &b) {
+    __shared__ Kv8Rel rel[KV8_NW];
     serve_args<128>();
     kv8_check(a);
     Kv8Plan p;
@@ -575,16 +644,16 @@ __device__ __forceinline__ void kv8_attn_rows(const Kv8Args &a, const Kv8Attn &b
     if ((int64_t)p.k * b.TT >= p.r1 - p.r0) return;
     const Kv8Tile t = kv8_tile(b, p, 1);
     const int lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    Kv8Wave<D, FULL> W;
+    Kv8Wave<D, FULL, true> W;
     int32_t ek;
     W.start(a, p, t, 0, t.steps, 1, ek);
     W.init(a, b, t, p.hk);
-    W.walk(a, b, p, t, 0, t.steps, 1, ek);
+    W.walk(a, b, p, t, 0, t.steps, 1, ek, &rel[threadIdx.x >> 6]);
     const float inv = 1.0f / kv8_sum_g(W.l);
     if (n >= t.nt * (b.H / a.Hkv)) return;
     float *o = kv8_out(a, b, p, t, n) + 4 * g;
 #pragma unroll
-    for (int ct = 0; ct < Kv8Wave<D, FULL>::NC; ct++)
+    for (int ct = 0; ct < Kv8Wave<D, FULL, true>::NC; ct++)
         if (FULL || 16 * ct < a.Dh) *(kv8_f4 *)(o + 16 * ct) = W.O[ct] * inv;
 }
 KV8_KERNEL(sepia_kv8_rows_128, kv8_attn_rows, 128, true)

@@ -223,6 +223,25 @@ def test_attn_masked_values(dev):
     g.free()
 
 
+@pytest.mark.parametrize("H,heads,R", [(32, 32, 1), (64, 32, 3), (32, 32, 37), (96, 32, 64), (30, 30, 131), (128, 32, 300)])
+def test_attn_many_rows_rel(dev, H, heads, R):
+    """A wave a unit: rel_logits of other rows lie beside a row's own, in rows of every alignment; those nobody sees (past
+    the row's position) are NaN, infinite or the lowest value, up to the buffer's first and last element."""
+    rng = np.random.default_rng(H + R)
+    lens, news, dim = [0, 90, 7], [150, 1, 400], 16 if R % 2 else 64
+    c, starts, n = make(rng, heads, dim, 16, lens, news)
+    q, rel = normal(rng, n, H, dim, scale=3.0), normal(rng, n, H, R, scale=0.7)
+    tau = rng.uniform(0.8, 1.4, n).astype(np.float32)
+    pos = np.concatenate([a + np.arange(b) for a, b in zip(lens, news)])
+    unseen = np.broadcast_to(np.arange(R) > pos[:, None, None], rel.shape)
+    want, tol = c.attn(lens, starts, q, np.where(unseen, 0, rel), tau, 0, np.float32(1 / dim))
+    rel[unseen] = rng.choice(np.array([np.nan, np.inf, -np.inf, np.finfo(np.float32).min], np.float32), int(unseen.sum()))
+    g = OnGpu(dev, c)
+    got = attn(dev, g, lens, starts, q, rel, tau, 0, 1 / dim)
+    assert np.all(np.abs(got - want) <= tol + np.abs(want) * 2.0 ** -23), float((np.abs(got - want) - tol).max())
+    g.free()
+
+
 @pytest.mark.parametrize("T", [1, 40])
 def test_attn_nonfinite(dev, T):
     """A NaN scale of K or V reaches exactly the rows and heads that see its page; a NaN or infinite q its own head."""
