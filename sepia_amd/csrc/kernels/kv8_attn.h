@@ -28,6 +28,7 @@
 #define KV8_C 8355711.0f     // 0x7F7F7F: the largest magnitude of three digits
 #define KV8_CP 4177855.0f    // half of it: a weight's place relative to a power of two
 #define KV8_L2E 1.44269504f
+#define KV8_LAZY 5.0f        // how far a maximum may rise before the sums are scaled anew
 
 struct Kv8Attn {
     const float *q, *rel, *tau;
@@ -188,7 +189,9 @@ struct Kv8Wave {
     static __device__ __forceinline__ int dh(const Kv8Args &a) { return FULL ? D : a.Dh; }
     kv8_i4 qd[3][NK];       // q's digits: lane (n, g) dims 64 ks + 16 g .. + 15 of row n
     kv8_f4 O[NC];
-    float m, l, qs, tau;    // row n's maximum; this lane's part of its sum; q's scale times c
+    // Row n's reference, its maximum or at most KV8_LAZY below; this lane's part
+    // of its sum; q's scale times c.
+    float m, l, qs, tau;
     int32_t lo, pos;        // row n's columns (inactive: none)
     int64_t th;             // row n's (token, head)
     bool on;                // whether there is a row n
@@ -410,14 +413,14 @@ struct Kv8Wave {
 #pragma unroll
         for (int j = 1; j < 16; j++) mx = fmaxf(mx, s[j]);
         const float mn = fmaxf(m, kv8_max_g(mx));
-        const float ref = mn == -INFINITY ? 0.0f : mn;
-        if (__ballot(mn != m)) {
-            const float al = __builtin_amdgcn_exp2f((m - ref) * KV8_L2E);   // 1 where the maximum stays
+        if (__ballot(mn > m + KV8_LAZY)) {
+            const float al = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * KV8_L2E);   // 1 where the maximum stays
             l *= al;
 #pragma unroll
             for (int ct = 0; ct < NC; ct++) O[ct] *= al;
             m = mn;
         }
+        const float ref = m == -INFINITY ? 0.0f : m;
         vs = any ? vs : 0.0f;
         // the row's largest product, as the power of two below it
         const float wm = kv8_max_g(__builtin_amdgcn_exp2f((mx - ref) * KV8_L2E) * vs);
