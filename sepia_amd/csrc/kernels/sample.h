@@ -24,7 +24,8 @@
 // place in the order, its piece again while it has more than a few tokens (equal
 // logits: by index), and those few are compared with each other. Where the
 // gathered tokens are too many (flat rows, long runs of equal logits) the same
-// is done with passes over the row. (Sorting the gathered tokens by a network
+// is done with passes over the row. (One row of 256 that gathered 5376 of 199999
+// tokens, with room for 4096, made the call 340 us in the place of 196.) (Sorting the gathered tokens by a network
 // took 10 us for 250 of them and 25 us for 1100.)
 //
 // A row is cut into chunks where the rows are fewer than the chip's places,
@@ -42,7 +43,8 @@
 #define SAMPLE_NT 512                 // two workgroups a CU (of 1024 threads one: 36 against 26 us at 48 rows)
 #define SAMPLE_WAVES (SAMPLE_NT / 64)
 #define SAMPLE_BINS 1024              // two a thread
-#define SAMPLE_CAP 4096               // gathered tokens
+#define SAMPLE_CAP 4096               // gathered tokens in shared memory
+#define SAMPLE_MANY 16384             // and in scratch
 #define SAMPLE_FEW 16                 // tokens that are compared with each other (60 of them took 4 us)
 
 // In scratch where a row has several chunks: a chunk's bins, and what the
@@ -52,7 +54,7 @@ struct SampleChunk {
     uint32_t count[SAMPLE_BINS];
 };
 struct SampleRow {
-    unsigned long long list[SAMPLE_CAP];
+    unsigned long long list[SAMPLE_MANY];
     uint32_t n, arrived;
 };
 struct SampleArgs {
@@ -301,33 +303,53 @@ __device__ __forceinline__ float sample_bounds(SampleAsk &q, SampleLds &L) {
     __syncthreads();
     return sample_least(q, max(max(bk, p1), d1));
 }
+// One to the row's list in scratch; r->n counts them, also past its end.
+__device__ __forceinline__ void sample_put(SampleRow *r, uint32_t at, unsigned long long place) {
+    if (at < SAMPLE_MANY) __hip_atomic_store(&r->list[at], place, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 // The chosen bins' tokens among the row's i0 .. i1 - 1 into L.list; L.n counts
-// them, also where they are more than the list holds.
-__device__ __forceinline__ void sample_gather(const SampleAsk &q, float least, int i0, int i1, SampleLds &L) {
+// them, also where they are more than the list holds. Those go to the row's
+// list, if there is one.
+__device__ __forceinline__ void sample_gather(const SampleAsk &q, float least, int i0, int i1, SampleLds &L, SampleRow *r) {
     sample_walk(q.x, i0, i1, [&](float v, int i) {
         if (!(v >= least)) return;
         const int b = sample_bin(sample_log(v, q.m, q.scale));
         if (!(L.set[b >> 6] >> (b & 63) & 1)) return;
         const uint32_t at = atomicAdd(&L.n, 1u);
         if (at < SAMPLE_CAP) L.list[at] = sample_place(v, i);
+        else if (r) sample_put(r, __hip_atomic_fetch_add(&r->n, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), sample_place(v, i));
     });
     __syncthreads();
 }
 // The first token of bin b whose cumulative weight from the bin's start
 // (by_count: place from 1) exceeds `over`, and the weight up to and with it,
-// among the n gathered tokens (listed) or the whole row's.
+// among the n gathered tokens, in shared memory where they fit, else in the
+// row's list (far), or among the whole row's (neither).
 struct SampleAt {
     unsigned long long place, cum;
 };
 __device__ __forceinline__ SampleAt sample_settle(const SampleAsk &q, int b, bool by_count, unsigned long long over,
-                                                  bool listed, uint32_t n, SampleLds &L) {
+                                                  uint32_t n, const SampleRow *far, SampleLds &L) {
     const int lane = (int)threadIdx.x & 63;
+    const bool listed = n <= SAMPLE_CAP;
     const auto walk = [&](auto f) {
         if (listed) {
             for (uint32_t i = threadIdx.x; i < n; i += SAMPLE_NT) {
                 const unsigned long long p = L.list[i];
                 const double z = sample_log(sample_token(p), q.m, q.scale);
                 if (sample_bin(z) == b) f(p, z);
+            }
+        } else if (far) {
+            for (uint32_t i = threadIdx.x; i < n; i += SAMPLE_LOADS * SAMPLE_NT) {
+                unsigned long long p[SAMPLE_LOADS];
+#pragma unroll
+                for (uint32_t j = 0; j < SAMPLE_LOADS; j++)
+                    p[j] = __hip_atomic_load(&far->list[min(i + j * SAMPLE_NT, n - 1)], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+                for (uint32_t j = 0; j < SAMPLE_LOADS; j++) {
+                    const double z = sample_log(sample_token(p[j]), q.m, q.scale);
+                    if (i + j * SAMPLE_NT < n && sample_bin(z) == b) f(p[j], z);
+                }
             }
         } else {
             sample_walk(q.x, 0, q.vocab, [&](float v, int i) {
@@ -340,7 +362,7 @@ __device__ __forceinline__ SampleAt sample_settle(const SampleAsk &q, int b, boo
     unsigned long long first = (unsigned long long)sample_key(sample_most(q, b)) << 20, before = 0;
     const unsigned long long last = ((unsigned long long)sample_key(fmaxf(sample_least(q, b), -3.402823466e38f)) << 20) | 0xFFFFF;
     int bits = 64 - __builtin_clzll((last - first) | 1);
-    uint32_t left = listed ? n : q.by_k ? L.cupto[b + 1] - L.cupto[b] : ~0u;   // at most (bins are counted for a k)
+    uint32_t left = listed || far ? n : q.by_k ? L.cupto[b + 1] - L.cupto[b] : ~0u;   // at most (bins are counted for a k)
     while (left > SAMPLE_FEW) {
         const int drop = max(bits - 10, 0);
         sample_clear(L);
@@ -394,14 +416,15 @@ __device__ __forceinline__ SampleAt sample_settle(const SampleAsk &q, int b, boo
 }
 // The decisions, from the gathered tokens where they fit L.list: the k-th
 // token, the top-p border, the draw.
-__device__ __forceinline__ void sample_finish(const SampleArgs &a, int row, const SampleAsk &q, uint32_t n, SampleLds &L) {
+__device__ __forceinline__ void sample_finish(const SampleArgs &a, int row, const SampleAsk &q, uint32_t n, const SampleRow *far,
+                                              SampleLds &L) {
     unsigned long long kept = L.upto[SAMPLE_BINS], place = 0;
     for (int step = q.by_k ? 0 : q.by_p ? 1 : 2; step <= 2; step = step == 0 && q.by_p ? 1 : step == 2 ? 3 : 2) {
         if (step == 2 && kept > q.over_min) kept = q.over_min;
         const unsigned long long over = step == 0 ? (unsigned long long)q.k - 1
                                         : step == 1 ? sample_want(q.p, kept) - 1 : sample_over(q.u, kept);
         const int b = sample_seek(L.upto, L.cupto, step == 0, over);
-        const SampleAt r = sample_settle(q, b, step == 0, over - (step == 0 ? L.cupto[b] : L.upto[b]), n <= SAMPLE_CAP, n, L);
+        const SampleAt r = sample_settle(q, b, step == 0, over - (step == 0 ? L.cupto[b] : L.upto[b]), n, far, L);
         if (step == 2) place = r.place;
         else kept = L.upto[b] + r.cum;
     }
@@ -562,18 +585,16 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_pick(Sample
     }
     L.pow.fill();
     const float least = sample_bounds(q, L);
-    sample_gather(q, least, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), L);
+    SampleRow *r = a.rows + row;
+    sample_gather(q, least, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), L, r);
     // The gathered tokens cross workgroups as relaxed agent-scope atomics: the
     // wait and the barrier order them before the arrival, the last arriver's
     // loads come after its own (a fence would write back the whole L2).
-    SampleRow *r = a.rows + row;
-    const uint32_t n = L.n;
+    const uint32_t n = min(L.n, (uint32_t)SAMPLE_CAP);
     __shared__ uint32_t at;
     if (tid == 0) at = __hip_atomic_fetch_add(&r->n, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    if (at + n <= SAMPLE_CAP)
-        for (int i = tid; i < (int)n; i += SAMPLE_NT)
-            __hip_atomic_store(&r->list[at + i], L.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = tid; i < (int)n; i += SAMPLE_NT) sample_put(r, at + i, L.list[i]);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (tid == 0) at = __hip_atomic_fetch_add(&r->arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -583,7 +604,7 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_pick(Sample
     if (total <= SAMPLE_CAP)
         for (int i = tid; i < (int)total; i += SAMPLE_NT)
             L.list[i] = __hip_atomic_load(&r->list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    sample_finish(a, row, q, total, L);
+    sample_finish(a, row, q, total, total <= SAMPLE_MANY ? r : nullptr, L);
 }
 
 // Grid (1, rows): a row by one workgroup.
@@ -595,6 +616,6 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample(SampleArgs 
     if (sample_done(a, row, q, sample_best(q.x, 0, a.vocab, L.wave), true)) return;
     sample_bins(q, 0, a.vocab, L);
     const float least = sample_bounds(q, L);
-    sample_gather(q, least, 0, a.vocab, L);
-    sample_finish(a, row, q, L.n, L);
+    sample_gather(q, least, 0, a.vocab, L, nullptr);
+    sample_finish(a, row, q, L.n, nullptr, L);
 }

@@ -246,7 +246,7 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
 
 /* struct SampleArgs of kernels/sample.h, and the bytes of its SampleRow and
  * SampleChunk */
-#define SAMPLE_ROW_BYTES (4096 * 8 + 8)
+#define SAMPLE_ROW_BYTES (16384 * 8 + 8)
 #define SAMPLE_CHUNK_BYTES (1024 * 12 + 16)
 #define SAMPLE_CHUNKS 16    /* chunks of a row at most */
 #define SAMPLE_NT 512

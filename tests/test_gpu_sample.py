@@ -101,6 +101,18 @@ def test_far_below_the_largest(dev, vocab):
             check(dev, x, vocab, u, top_k=k, **params)
 
 
+@pytest.mark.parametrize("spread", [0.3, 0.05, 0.02, 0.002])
+@pytest.mark.parametrize("rows", [3, 40])
+def test_flat_rows(dev, rows, spread):
+    """Logits so close together that a bin holds hundreds, thousands or all of a row's tokens: more than a workgroup
+    gathers, more than the row's list takes."""
+    rng = np.random.default_rng(int(spread * 1000) + rows)
+    vocab = 60000 if rows == 3 else 30000
+    x = (rng.standard_normal((rows, vocab)) * spread).astype(np.float32)
+    for params in (dict(), dict(top_p=0.97), dict(top_k=25000), dict(top_k=20000, top_p=0.4, min_p=0.9), dict(temperature=4.0, top_p=0.6)):
+        check(dev, x, vocab, rng.random(rows).astype(np.float32), **params)
+
+
 def test_few_distinct_logits(dev):
     """Long runs of equal logits below a few others: the border falls inside a run."""
     rng = np.random.default_rng(4)
