@@ -515,7 +515,7 @@ __device__ __forceinline__ void sample_bins(SampleAsk &q, int i0, int i1, Sample
 }
 
 // Grid (chunks, rows): the chunk's first token of the order; the row's counters
-// cleared.
+// cleared. One row of 100003 4.6 us; 256 of 199999 38 us (5.4 TB/s).
 extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_max(SampleArgs a) {
     __shared__ unsigned long long wave[SAMPLE_WAVES];
     serve_args<64>();
@@ -527,7 +527,8 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_max(SampleA
     if (c == 0) a.rows[row].n = a.rows[row].arrived = 0;
 }
 
-// Grid (chunks, rows): the chunk's bins.
+// Grid (chunks, rows): the chunk's bins. 7.6 and 73 us for those, the latter
+// bound by the weights' doubles and the sums in shared memory.
 extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_bins(SampleArgs a) {
     __shared__ SampleLds L;
     serve_args<64>();
@@ -543,7 +544,8 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_bins(Sample
     if (tid == 0) o->over_min = q.over_min;
 }
 
-// Grid (chunks, rows): the decision, over the chunks' bins.
+// Grid (chunks, rows): the decision, over the chunks' bins. 12 and 76 us: the
+// row read again, then scans, barriers and the last workgroup's decisions.
 extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_pick(SampleArgs a) {
     __shared__ SampleLds L;
     serve_args<64>();
@@ -607,7 +609,8 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_pick(Sample
     sample_finish(a, row, q, total, total <= SAMPLE_MANY ? r : nullptr, L);
 }
 
-// Grid (1, rows): a row by one workgroup.
+// Grid (1, rows): a row by one workgroup (28 us a call of 11625 logits, its
+// batch included).
 extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample(SampleArgs a) {
     __shared__ SampleLds L;
     serve_args<64>();
