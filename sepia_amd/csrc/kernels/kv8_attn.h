@@ -634,10 +634,10 @@ KV8_KERNEL(sepia_kv8_attn_to64, kv8_attn_run, 64, false)
 
 // Many rows (prompts): a wave a unit, KV8_NW row tiles of one kv head side by
 // side in a workgroup, so that they find K and V in the caches; nothing is cut
-// or folded. Bound by its instructions: 2.6 us a step and pair of waves of a
-// SIMD at dim 128, 2.4 of them without any load; 500 rows behind 1500 (64 heads
-// on 8) 103 us. (K and V loaded once for the four and put in shared memory: 2.8
-// us a step.) Grid: (ids of KV8_NW row tiles, kv heads), kv heads fastest, so
+// or folded. 2.6 us a step and pair of waves of a SIMD at dim 128; the loads alone
+// take 2.2, all but the loads 2.4, all but the matrix products 2.5. 500 rows
+// behind 1500 (64 heads on 8) 103 us. (K and V loaded once for the four and put
+// in shared memory: 2.8 us a step; that in steps of 128 columns: spills.) Grid: (ids of KV8_NW row tiles, kv heads), kv heads fastest, so
 // that with 8 of them an XCD's L2 holds one head's K and V.
 template <int D, bool FULL>
 __device__ __forceinline__ void kv8_attn_rows(const Kv8Args &a, const Kv8Attn &b) {
