@@ -105,12 +105,16 @@ __device__ __forceinline__ int kv8_plan(const Kv8Args &a, const Kv8Attn &b, int 
         total += kv8_last(kv8_scan((float)rt * (float)steps));
     }
     const int chunk = b.budget > 0 ? max(KV8_NW, (int)ceilf(fminf(total * (float)a.Hkv / (float)b.budget, 1e9f))) : 0x7FFFFFFF;
+    // Folded by its last run, a unit of two steps a wave stays whole: the fold
+    // takes longer than the second step (32 sequences of up to 500 columns, 8 kv
+    // heads: 12.2 us against 9.8).
+    const int whole = b.arrived ? 2 * KV8_NW : 0;
     p.hk = id % a.Hkv;
     const int at = id / a.Hkv;
     int base = 0, slots = 0;
     for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
         if (a.n_seqs > 64) kv8_cost(a, b, s0 + lane, rt, steps, len, r0, r1);   // else they are still here
-        const int splits = (int)(((int64_t)steps + chunk - 1) / chunk);
+        const int splits = steps <= whole ? 1 : (int)(((int64_t)steps + chunk - 1) / chunk);
         const int mine = FOLD ? (splits > 1 ? rt : 0) : rt * splits;
         const int cut = splits > 1 ? rt * splits : 0;
         const int sum = kv8_scan(mine), csum = kv8_scan(cut);

@@ -156,6 +156,7 @@ int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *
 
 /* struct Kv8Attn of kernels/kv8_attn.h */
 #define KV8_ROWS 1024       /* units from which each has a wave of its own */
+#define KV8_NW 4            /* steps of a run at least, one for each wave */
 #define KV8_RUNS 16         /* runs of a unit, on average, above which a launch folds them */
 #define KV8_BUDGET 512      /* runs of a call whose units alone leave the chip idle: two workgroups a CU */
 typedef struct {
@@ -216,12 +217,19 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
     }
     const int64_t ids = n / b.TT + c->n_seqs;
     const size_t per = 16 * (size_t)c->head_dim * 4, limit = sepia_scratch_limit();
-    /* as many runs as places; half as many again where a run is long, since
-     * units of ragged lengths end unevenly (48 sequences of up to 12000
-     * columns: 122 us against 131; 32 of 512: 29 against 20) */
-    int64_t steps = c->max_pages * c->page / 64 + 1;   /* of a unit, at most */
+    /* No more runs than places: a unit's last run is short, so as many fewer as
+     * there are units (a whole round more for a few runs: 32 sequences in a
+     * window of 512, 16 kv heads, 18.4 us against 13.9; 4 of up to 8000 columns
+     * 24.2 against 20.4). Half as many again as places where a run is
+     * long, since units of ragged lengths end unevenly (48 sequences of up to
+     * 12000 columns: 122 us against 131; 32 of 512: 29 against 20). None where
+     * a run has every step that the table or the window leaves a unit. */
+    int64_t steps = (c->max_pages * c->page + 63) / 64;   /* of a unit, at most */
     if (window > 0 && window / 64 + 2 < steps) steps = window / 64 + 2;
-    int64_t budget = units * steps / KV8_BUDGET > 64 ? KV8_BUDGET * 3 / 2 : KV8_BUDGET, slots = 2 * budget + 64;
+    int64_t budget = KV8_BUDGET - (units < KV8_BUDGET / 2 ? units : KV8_BUDGET / 2);
+    if (units * steps / KV8_BUDGET > 64) budget = KV8_BUDGET * 3 / 2;
+    if (steps <= KV8_NW) budget = 0;
+    int64_t slots = 2 * budget + 64;
     while (budget && (size_t)slots * (per + 128) > limit) {
         budget /= 2;
         slots = 2 * budget + 64;
