@@ -157,7 +157,7 @@ int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *
 /* struct Kv8Attn of kernels/kv8_attn.h */
 #define KV8_ROWS 1024       /* units from which each has a wave of its own */
 #define KV8_NW 4            /* steps of a run at least, one for each wave */
-#define KV8_RUNS 16         /* runs of a unit, on average, above which a launch folds them */
+#define KV8_RUNS 16         /* runs of a unit above which a launch folds them */
 #define KV8_BUDGET 512      /* runs of a call whose units alone leave the chip idle: two workgroups a CU */
 typedef struct {
     const float *q, *rel, *tau;
@@ -235,8 +235,10 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
         slots = 2 * budget + 64;
     }
     /* Units of many runs are folded by a launch of their own, of few by the
-     * run that ends last. */
-    const int fold = units * KV8_RUNS < budget;
+     * run that ends last (one sequence, 8 kv heads: 2000 columns 9.6 us against
+     * 7.3 and 4.0 and a launch's gap, 4000 columns 12.1 against 8.0 and 4.2, 8000
+     * 15.6 against 7.9 and 4.9). */
+    const int fold = units * KV8_RUNS < budget && steps > KV8_RUNS * KV8_NW;
     if (budget) {
         uint8_t *s = (uint8_t *)sepia_scratch((size_t)slots * (per + 128), op);
         if (!s) return 0;
