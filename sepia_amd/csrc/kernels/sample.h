@@ -137,7 +137,7 @@ struct SampleLds {
     unsigned long long mass[SAMPLE_BINS + 1], upto[SAMPLE_BINS + 1];
     uint32_t count[SAMPLE_BINS + 1], cupto[SAMPLE_BINS + 1];
     unsigned long long list[SAMPLE_CAP], few[SAMPLE_FEW];
-    unsigned long long wave[SAMPLE_WAVES], set[SAMPLE_BINS / 64];
+    unsigned long long over_min, wave[SAMPLE_WAVES], set[SAMPLE_BINS / 64];
     uint32_t n;
     SamplePow pow;
 };
@@ -162,16 +162,36 @@ __device__ __forceinline__ unsigned long long sample_lane(unsigned long long v, 
     return (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)v, l) |
            (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32;
 }
+// f over the lanes up to each lane's own, by lane moves (by LDS permutes, and
+// with the bins' tail summed by three such scans, 48 rows took 57.8 us in the
+// place of 54.8): rows of 16, then a
+// row's last lane to the next row, then two rows' to the next two. `none`: f's
+// neutral value.
+template <class F>
+__device__ __forceinline__ unsigned long long sample_lanes(unsigned long long v, unsigned long long none, F f) {
+#define SAMPLE_DPP(ctrl, rows)                                                                                         \
+    {                                                                                                                  \
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, ctrl, rows, 0xF, false);          \
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp((int)(none >> 32), (int)(v >> 32), ctrl, rows, 0xF, false); \
+        v = f(v, (unsigned long long)hi << 32 | lo);                                                                   \
+    }
+    SAMPLE_DPP(0x111, 0xF)
+    SAMPLE_DPP(0x112, 0xF)
+    SAMPLE_DPP(0x114, 0xF)
+    SAMPLE_DPP(0x118, 0xF)
+    SAMPLE_DPP(0x142, 0xA)
+    SAMPLE_DPP(0x143, 0xC)
+#undef SAMPLE_DPP
+    return v;
+}
+__device__ __forceinline__ unsigned long long sample_sums(unsigned long long v) {
+    return sample_lanes(v, 0, [](unsigned long long a, unsigned long long b) { return a + b; });
+}
 // Exclusive prefix sums over the workgroup's threads; the total too.
 __device__ __forceinline__ unsigned long long sample_scan(unsigned long long v, unsigned long long *wave,
                                                           unsigned long long &total) {
     const int lane = (int)threadIdx.x & 63, w = (int)threadIdx.x >> 6;
-    unsigned long long s = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned long long u = __shfl_up(s, o, 64);
-        if (lane >= o) s += u;
-    }
+    const unsigned long long s = sample_sums(v);
     __syncthreads();
     if (lane == 63) wave[w] = s;
     __syncthreads();
@@ -186,14 +206,11 @@ __device__ __forceinline__ unsigned long long sample_scan(unsigned long long v, 
     return before + s - v;
 }
 __device__ __forceinline__ unsigned long long sample_min(unsigned long long v, unsigned long long *wave) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        const unsigned long long u = __shfl_xor(v, o, 64);
-        v = u < v ? u : v;
-    }
+    v = sample_lanes(v, ~0ull, [](unsigned long long a, unsigned long long b) { return b < a ? b : a; });
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) wave[threadIdx.x >> 6] = v;
     __syncthreads();
+    v = wave[0];
 #pragma unroll
     for (int i = 0; i < SAMPLE_WAVES; i++) v = wave[i] < v ? wave[i] : v;
     return v;
@@ -485,8 +502,9 @@ __device__ __forceinline__ void sample_bins(SampleAsk &q, int i0, int i1, Sample
     const int tid = (int)threadIdx.x;
     const unsigned long long floor_mass = q.f > 0.0f ? (unsigned long long)__builtin_ceil((double)q.f * SAMPLE_ONE) : 0;
     L.pow.fill();
+    if (tid == 0) L.over_min = 0;
     sample_clear(L);
-    unsigned long long tail = 0, over_min = 0, tails, ntails;
+    unsigned long long tail = 0, over_min = 0;
     uint32_t ntail = 0;
     const bool counted = q.k > 0;
     const auto add = [&](float v, bool floor) {
@@ -504,14 +522,17 @@ __device__ __forceinline__ void sample_bins(SampleAsk &q, int i0, int i1, Sample
     };
     if (floor_mass) sample_walk(q.x, i0, i1, [&](float v, int) { add(v, true); });
     else sample_walk(q.x, i0, i1, [&](float v, int) { add(v, false); });
-    sample_scan(tail, L.wave, tails);
-    sample_scan(ntail, L.wave, ntails);
-    if (floor_mass) sample_scan(over_min, L.wave, q.over_min);
-    if (tid == 0) {
-        L.mass[SAMPLE_BINS - 1] = tails;
-        L.count[SAMPLE_BINS - 1] = (uint32_t)ntails;
+    // the waves' sums, by each wave's last lane
+    tail = sample_sums(tail);
+    if (floor_mass) over_min = sample_sums(over_min);
+    if (counted) ntail = (uint32_t)sample_sums(ntail);
+    if ((tid & 63) == 63) {
+        atomicAdd(&L.mass[SAMPLE_BINS - 1], tail);
+        if (floor_mass) atomicAdd(&L.over_min, over_min);
+        if (counted) atomicAdd(&L.count[SAMPLE_BINS - 1], ntail);
     }
     __syncthreads();
+    if (floor_mass) q.over_min = L.over_min;
 }
 
 // Grid (chunks, rows): the chunk's first token of the order; the row's counters
@@ -527,7 +548,7 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_max(SampleA
     if (c == 0) a.rows[row].n = a.rows[row].arrived = 0;
 }
 
-// Grid (chunks, rows): the chunk's bins. 7.6 and 73 us for those, the latter
+// Grid (chunks, rows): the chunk's bins. 6.8 and 71 us for those, the latter
 // bound by the weights' doubles and the sums in shared memory.
 extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_bins(SampleArgs a) {
     __shared__ SampleLds L;
