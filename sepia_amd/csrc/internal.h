@@ -49,7 +49,7 @@ SEPIA_HIDDEN size_t sepia_scratch_limit(void);
 /* Kernels of the second code object (kernels/sepia_serve.hip), and a launch
  * of one on the library's stream, timed when the profiler is on. */
 enum { SK_KV8_APPEND, SK_KV8_READ, SK_KV8_ATTN, SK_KV8_ROWS = SK_KV8_ATTN + 4,   /* head dims 128, up to 128, 64, up to 64 */
-       SK_KV8_FOLD = SK_KV8_ROWS + 4, SK_SAMPLE_MAX, SK_SAMPLE_BINS, SK_SAMPLE_PICK, SK_SAMPLE, SK_COUNT };
+       SK_SAMPLE_MAX = SK_KV8_ROWS + 4, SK_SAMPLE_BINS, SK_SAMPLE_PICK, SK_SAMPLE, SK_COUNT };
 SEPIA_HIDDEN int sepia_serve_launch(int k, uint64_t gx, unsigned gy, unsigned gz, unsigned block, void **args,
                                     const char *op);
 

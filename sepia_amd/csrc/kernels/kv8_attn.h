@@ -34,7 +34,8 @@ struct Kv8Attn {
     const float *q, *rel, *tau;
     float *out;
     float *part, *ml;        // per run: O [16][Dh]; maxima [16], sums [16]
-    uint32_t *arrived;       // per unit (at its first run's place): runs done; NULL: sepia_kv8_fold folds
+    uint32_t *arrived;       // at a group's first run's place: its runs that are done; KV8_UNITS on, at a unit's
+                             // first run's place: its groups
     int32_t H, R, window, TT, budget;   // TT: tokens of a row tile
     float c;
 };
@@ -93,9 +94,7 @@ template <class T>
 __device__ __forceinline__ T kv8_last(T v) {
     return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
-// The id-th run (FOLD: the id-th unit that may be cut) in the order sequence,
-// row tile, split, kv head; 0 past the last.
-template <bool FOLD>
+// The id-th run in the order sequence, row tile, split, kv head; 0 past the last.
 __device__ __forceinline__ int kv8_plan(const Kv8Args &a, const Kv8Attn &b, int id, Kv8Plan &p) {
     const int lane = (int)(threadIdx.x & 63);
     float total = 0.0f;
@@ -105,17 +104,17 @@ __device__ __forceinline__ int kv8_plan(const Kv8Args &a, const Kv8Attn &b, int 
         total += kv8_last(kv8_scan((float)rt * (float)steps));
     }
     const int chunk = b.budget > 0 ? max(KV8_NW, (int)ceilf(fminf(total * (float)a.Hkv / (float)b.budget, 1e9f))) : 0x7FFFFFFF;
-    // Folded by its last run, a unit of two steps a wave stays whole: the fold
-    // takes longer than the second step (32 sequences of up to 500 columns, 8 kv
-    // heads: 12.2 us against 9.8).
-    const int whole = b.arrived ? 2 * KV8_NW : 0;
+    // A unit of two steps a wave stays whole: the fold takes longer than the
+    // second step (32 sequences of up to 500 columns, 8 kv heads: 12.2 us against
+    // 9.8).
+    const int whole = 2 * KV8_NW;
     p.hk = id % a.Hkv;
     const int at = id / a.Hkv;
     int base = 0, slots = 0;
     for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
         if (a.n_seqs > 64) kv8_cost(a, b, s0 + lane, rt, steps, len, r0, r1);   // else they are still here
         const int splits = steps <= whole ? 1 : (int)(((int64_t)steps + chunk - 1) / chunk);
-        const int mine = FOLD ? (splits > 1 ? rt : 0) : rt * splits;
+        const int mine = rt * splits;
         const int cut = splits > 1 ? rt * splits : 0;
         const int sum = kv8_scan(mine), csum = kv8_scan(cut);
         const uint64_t hit = __ballot(at >= base + sum - mine && at < base + sum);
@@ -124,8 +123,8 @@ __device__ __forceinline__ int kv8_plan(const Kv8Args &a, const Kv8Attn &b, int 
             p.s = s0 + l;
             p.splits = __builtin_amdgcn_readlane(splits, l);
             const int i = at - base - __builtin_amdgcn_readlane(sum - mine, l);
-            p.k = FOLD ? i : i / p.splits;
-            p.x = FOLD ? 0 : i - p.k * p.splits;
+            p.k = i / p.splits;
+            p.x = i - p.k * p.splits;
             p.slot = (slots + __builtin_amdgcn_readlane(csum - cut, l) + p.k * p.splits) * a.Hkv + p.hk;
             p.len = __builtin_amdgcn_readlane(len, l);
             p.r0 = __builtin_amdgcn_readlane(r0, l);
@@ -525,11 +524,63 @@ __device__ __forceinline__ float *kv8_out(const Kv8Args &a, const Kv8Attn &b, co
     return b.out + ((int64_t)(t.t0 + ti) * b.H + p.hk * G + (n - ti * G)) * a.Dh;
 }
 #define KV8_AHEAD 8   // partials whose loads are in flight at a time
+#define KV8_RUNS 16   // of a unit that are folded at once; more are folded in groups first
+#define KV8_UNITS 8192
+
+// Row `row`'s dims d .. d + 3 of n partials, `step` places apart from place `at`
+// on: the sums so far, relative to their maximum.
+struct Kv8Sum {
+    float top, sum;
+    kv8_f4 o;
+};
+__device__ __forceinline__ Kv8Sum kv8_fold(const Kv8Args &a, const Kv8Attn &b, int64_t at, int n, int step, int row, int d) {
+    Kv8Sum r = {-INFINITY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+    for (int x0 = 0; x0 < n; x0 += KV8_AHEAD) {
+        kv8_f4 v[KV8_AHEAD];
+        float vm[KV8_AHEAD], vl[KV8_AHEAD], mx = r.top;
+#pragma unroll
+        for (int j = 0; j < KV8_AHEAD; j++) {
+            const int64_t i = at + (int64_t)min(x0 + j, n - 1) * step;
+            v[j] = kv8_get(b.part + (i * 16 + row) * a.Dh + d);
+            vm[j] = __hip_atomic_load(&b.ml[i * 32 + row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            vl[j] = __hip_atomic_load(&b.ml[i * 32 + 16 + row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+#pragma unroll
+        for (int j = 0; j < KV8_AHEAD; j++) mx = fmaxf(mx, vm[j]);
+        const float from = mx == -INFINITY ? 0.0f : mx, al = __builtin_amdgcn_exp2f((r.top - from) * KV8_L2E);
+        r.sum *= al;
+        r.o *= al;
+        r.top = mx;
+#pragma unroll
+        for (int j = 0; j < KV8_AHEAD; j++) {
+            const float e = x0 + j < n ? __builtin_amdgcn_exp2f((vm[j] - from) * KV8_L2E) : 0.0f;
+            if (x0 + j < n) {
+                r.sum += vl[j] * e;
+                r.o += v[j] * e;
+            }
+        }
+    }
+    return r;
+}
+// Whether this workgroup is the last of n to arrive; the counter is zero again
+// then. What crosses workgroups are relaxed agent-scope atomics: the wait and
+// the barrier order the stores before the arrival, and the last arriver's loads
+// come after its own (a release fence would write back the whole L2).
+__device__ __forceinline__ bool kv8_arrive(uint32_t *counter, int n) {
+    __shared__ uint32_t before;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (before + 1 != (uint32_t)n) return false;
+    if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return true;
+}
 
 // Grid: the plan's runs, KV8_NW waves each. Bound by memory for long contexts
 // (48 sequences of 278000 columns in all, 8 kv heads of 128: 121 us, 4.8 TB/s),
 // else by the chain from the plan to the fold: one sequence of 20000 columns
-// 14 us, 32 in a window of 512 20 us (16 kv heads).
+// 17 us, 32 in a window of 512 20 us (16 kv heads).
 template <int D, bool FULL>
 __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b) {
     __shared__ kv8_f4 so[KV8_NW][Kv8Wave<D, FULL, false>::NC][64];
@@ -537,7 +588,7 @@ __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b)
     serve_args<128>();
     kv8_check(a);
     Kv8Plan p;
-    if (!kv8_plan<false>(a, b, (int)blockIdx.x, p)) return;
+    if (!kv8_plan(a, b, (int)blockIdx.x, p)) return;
     const Kv8Tile t = kv8_tile(b, p, p.splits);
     const int s0 = p.x * t.span, s1 = min(t.steps, s0 + t.span);
     if (s0 >= s1) return;
@@ -582,51 +633,40 @@ __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b)
         __hip_atomic_store(&b.ml[slot * 32 + n], M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __hip_atomic_store(&b.ml[slot * 32 + 16 + n], L, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    if (!b.arrived) return;
-    // The last of a unit's runs to arrive folds them, in their order. What
-    // crosses workgroups are relaxed agent-scope atomics: the wait and the
-    // barrier order the stores before the arrival, and the last arriver's loads
-    // come after its own (a release fence would write back the whole L2).
-    __shared__ uint32_t before;
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (threadIdx.x == 0)
-        before = __hip_atomic_fetch_add(&b.arrived[p.slot], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (before + 1 != (uint32_t)t.runs) return;
-    if (threadIdx.x == 0) __hip_atomic_store(&b.arrived[p.slot], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // The last of a unit's runs to arrive folds them, in their order. Of many
+    // the last of each group folds the group's to its first run's place, and the
+    // last of those the groups': two short chains of loads for a long one (one
+    // sequence of 20000 columns, 63 runs of a unit: 16.8 us against 18.3 and a
+    // gap with a fold by a launch, 25 by one workgroup; at 16 runs one is as fast).
     const int per = a.Dh / 4;
+    int n_part = t.runs, step = a.Hkv;
+    uint32_t *counter = b.arrived + p.slot;
+    if (t.runs > KV8_RUNS) {
+        int lg = 3;
+        while (t.runs > 1 << (2 * lg)) lg++;
+        const int x0 = p.x >> lg << lg, n = min(1 << lg, t.runs - x0);
+        const int64_t at = p.slot + (int64_t)x0 * a.Hkv;
+        if (!kv8_arrive(b.arrived + at, n)) return;
+        for (int i = (int)threadIdx.x; i < rows * per; i += 64 * KV8_NW) {
+            const int row = i / per, d = 4 * (i - row * per);
+            const Kv8Sum r = kv8_fold(a, b, at, n, a.Hkv, row, d);
+            kv8_put(b.part + (at * 16 + row) * a.Dh + d, r.o);
+            if (d == 0) sm[0][row] = r.top, sl[0][row] = r.sum;
+        }
+        __syncthreads();   // every thread has read the group's maxima and sums
+        if ((int)threadIdx.x < rows) {
+            __hip_atomic_store(&b.ml[at * 32 + threadIdx.x], sm[0][threadIdx.x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(&b.ml[at * 32 + 16 + threadIdx.x], sl[0][threadIdx.x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        n_part = (t.runs + (1 << lg) - 1) >> lg;
+        step = a.Hkv << lg;
+        counter += KV8_UNITS;
+    }
+    if (!kv8_arrive(counter, n_part)) return;
     for (int i = (int)threadIdx.x; i < rows * per; i += 64 * KV8_NW) {
         const int row = i / per, d = 4 * (i - row * per);
-        // the sums so far, relative to their maximum
-        float top = -INFINITY, sum = 0.0f;
-        kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int x0 = 0; x0 < t.runs; x0 += KV8_AHEAD) {
-            kv8_f4 v[KV8_AHEAD];
-            float vm[KV8_AHEAD], vl[KV8_AHEAD], mx = top;
-#pragma unroll
-            for (int j = 0; j < KV8_AHEAD; j++) {
-                const int64_t at = p.slot + (int64_t)min(x0 + j, t.runs - 1) * a.Hkv;
-                v[j] = kv8_get(b.part + (at * 16 + row) * a.Dh + d);
-                vm[j] = __hip_atomic_load(&b.ml[at * 32 + row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                vl[j] = __hip_atomic_load(&b.ml[at * 32 + 16 + row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-#pragma unroll
-            for (int j = 0; j < KV8_AHEAD; j++) mx = fmaxf(mx, vm[j]);
-            const float from = mx == -INFINITY ? 0.0f : mx, al = __builtin_amdgcn_exp2f((top - from) * KV8_L2E);
-            sum *= al;
-            o *= al;
-            top = mx;
-#pragma unroll
-            for (int j = 0; j < KV8_AHEAD; j++) {
-                const float e = x0 + j < t.runs ? __builtin_amdgcn_exp2f((vm[j] - from) * KV8_L2E) : 0.0f;
-                if (x0 + j < t.runs) {
-                    sum += vl[j] * e;
-                    o += v[j] * e;
-                }
-            }
-        }
-        *(kv8_f4 *)(kv8_out(a, b, p, t, row) + d) = o / sum;
+        const Kv8Sum r = kv8_fold(a, b, p.slot, n_part, step, row, d);
+        *(kv8_f4 *)(kv8_out(a, b, p, t, row) + d) = r.o / r.sum;
     }
 }
 #define KV8_KERNEL(name, run, D, FULL) \
@@ -673,55 +713,3 @@ KV8_KERNEL(sepia_kv8_rows_128, kv8_attn_rows, 128, true)
 KV8_KERNEL(sepia_kv8_rows_to128, kv8_attn_rows, 128, false)
 KV8_KERNEL(sepia_kv8_rows_64, kv8_attn_rows, 64, true)
 KV8_KERNEL(sepia_kv8_rows_to64, kv8_attn_rows, 64, false)
-
-// Folds the runs of the units that were cut, where those are few and of many
-// runs each (one user's token over a long context): a workgroup a unit's row,
-// eight groups of threads that take its runs in turn, a thread for 4 dims. Grid:
-// (units that may be cut, rows of a tile). 6 us for 8 units of 64 runs: a launch
-// and two rounds of loads.
-extern "C" __global__ __launch_bounds__(256) void sepia_kv8_fold(Kv8Args a, Kv8Attn b) {
-    __shared__ kv8_f4 so[8][32];
-    __shared__ float sl[8];
-    serve_args<128>();
-    Kv8Plan p;
-    if (!kv8_plan<true>(a, b, (int)blockIdx.x, p)) return;
-    const Kv8Tile t = kv8_tile(b, p, p.splits);
-    const int n = (int)blockIdx.y, j = (int)threadIdx.x >> 5, d = 4 * ((int)threadIdx.x & 31);
-    if (t.runs == 1 || n >= t.nt * (b.H / a.Hkv)) return;
-    float M = -INFINITY, L = 0.0f;
-    for (int x = (int)threadIdx.x & 63; x < t.runs; x += 64) M = fmaxf(M, b.ml[((int64_t)p.slot + (int64_t)x * a.Hkv) * 32 + n]);
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-    const float ref = M == -INFINITY ? 0.0f : M;
-    kv8_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int x0 = j; x0 < t.runs; x0 += 8 * KV8_AHEAD) {
-        kv8_f4 v[KV8_AHEAD];
-        float vm[KV8_AHEAD], vl[KV8_AHEAD];
-#pragma unroll
-        for (int i = 0; i < KV8_AHEAD; i++) {
-            const int64_t at = (int64_t)p.slot + (int64_t)min(x0 + 8 * i, t.runs - 1) * a.Hkv;
-            v[i] = *(const kv8_f4 *)(b.part + (at * 16 + n) * a.Dh + (d < a.Dh ? d : 0));
-            vm[i] = b.ml[at * 32 + n];
-            vl[i] = b.ml[at * 32 + 16 + n];
-        }
-#pragma unroll
-        for (int i = 0; i < KV8_AHEAD; i++) {
-            if (x0 + 8 * i >= t.runs) break;
-            const float f = __builtin_amdgcn_exp2f((vm[i] - ref) * KV8_L2E);
-            L += vl[i] * f;
-            o += v[i] * f;
-        }
-    }
-    so[j][d / 4] = o;
-    if (d == 0) sl[j] = L;
-    __syncthreads();
-    if (j > 0 || d >= a.Dh) return;
-    L = 0.0f;
-    o = kv8_f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        o += so[i][d / 4];
-        L += sl[i];
-    }
-    *(kv8_f4 *)(kv8_out(a, b, p, t, n) + d) = o / L;
-}

@@ -109,7 +109,7 @@ static const char *const k_names[K_COUNT] = {
 static const char *const serve_names[SK_COUNT] = {
     "sepia_kv8_append", "sepia_kv8_read",
     "sepia_kv8_attn_128", "sepia_kv8_attn_to128", "sepia_kv8_attn_64", "sepia_kv8_attn_to64",
-    "sepia_kv8_rows_128", "sepia_kv8_rows_to128", "sepia_kv8_rows_64", "sepia_kv8_rows_to64", "sepia_kv8_fold",
+    "sepia_kv8_rows_128", "sepia_kv8_rows_to128", "sepia_kv8_rows_64", "sepia_kv8_rows_to64",
     "sepia_sample_max", "sepia_sample_bins", "sepia_sample_pick", "sepia_sample",
 };
 #define K_ALL (K_COUNT + SK_COUNT)

@@ -157,8 +157,9 @@ int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *
 /* struct Kv8Attn of kernels/kv8_attn.h */
 #define KV8_ROWS 1024       /* units from which each has a wave of its own */
 #define KV8_NW 4            /* steps of a run at least, one for each wave */
-#define KV8_RUNS 16         /* runs of a unit above which a launch folds them */
+#define KV8_UNITS 8192
 #define KV8_BUDGET 512      /* runs of a call whose units alone leave the chip idle: two workgroups a CU */
+_Static_assert(2 * (KV8_BUDGET * 3 / 2) + 64 <= KV8_UNITS && 2 * KV8_UNITS <= SEPIA_COUNTERS, "a counter for each slot, twice");
 typedef struct {
     const float *q, *rel, *tau;
     float *out;
@@ -234,24 +235,16 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
         budget /= 2;
         slots = 2 * budget + 64;
     }
-    /* Units of many runs are folded by a launch of their own, of few by the
-     * run that ends last (one sequence, 8 kv heads: 2000 columns 9.6 us against
-     * 7.3 and 4.0 and a launch's gap, 4000 columns 12.1 against 8.0 and 4.2, 8000
-     * 15.6 against 7.9 and 4.9). */
-    const int fold = units * KV8_RUNS < budget && steps > KV8_RUNS * KV8_NW;
     if (budget) {
         uint8_t *s = (uint8_t *)sepia_scratch((size_t)slots * (per + 128), op);
         if (!s) return 0;
         b.part = (float *)s;
         b.ml = (float *)(s + (size_t)slots * per);
-        if (!fold) b.arrived = sepia_counters();   /* slots of them: fewer than there are */
+        b.arrived = sepia_counters();   /* two for each slot, the second KV8_UNITS behind the first */
     }
     b.budget = (int32_t)budget;
     void *args[] = { &a, &b };
-    if (!sepia_serve_launch(SK_KV8_ATTN + dim, (uint64_t)(budget + ids * c->n_kv_heads), 1, 1, 256, args, op)) return 0;
-    if (!fold) return 1;
-    const int64_t cut = ids * c->n_kv_heads < budget ? ids * c->n_kv_heads : budget;
-    return sepia_serve_launch(SK_KV8_FOLD, (uint64_t)cut, 16, 1, 256, args, op);
+    return sepia_serve_launch(SK_KV8_ATTN + dim, (uint64_t)(budget + ids * c->n_kv_heads), 1, 1, 256, args, op);
 }
 
 /* struct SampleArgs of kernels/sample.h, and the bytes of its SampleRow and

@@ -171,9 +171,9 @@ ATTNS = [
     # many rows: a wave a unit
     (128, 64, 128, 16, [200, 0, 3], [130, 0, 9], 0, 64), (96, 32, 128, 64, [64], [180], 90, 0),
     (48, 16, 64, 32, [70, 0], [200, 150], 100, 40), (112, 56, 80, 16, [17, 0], [100, 60], 0, 300),
-    # long: few units of many runs, whose partials a launch folds
+    # long: few units of many runs, whose partials are folded in groups first
     (16, 2, 128, 16, [5000], [1], 0, 1024), (14, 2, 80, 32, [9001, 100], [2, 0], 0, 50), (4, 4, 64, 64, [4500, 4400], [3, 1], 0, 0),
-    (8, 1, 16, 16, [6000], [9], 0, 7),
+    (8, 1, 16, 16, [6000], [9], 0, 7), (2, 1, 32, 32, [30000], [1], 0, 0), (8, 1, 16, 64, [70000], [1], 0, 33),
 ]
 
 

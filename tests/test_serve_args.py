@@ -11,7 +11,7 @@ import test_kernarg_warm as warm
 from sepia_amd import hip
 
 # the kernels that a file's warm-ups are compiled into, by the function that holds the call
-HOLDERS = {"sepia_kv8_append": "sepia_kv8_append", "sepia_kv8_read": "sepia_kv8_read", "sepia_kv8_fold": "sepia_kv8_fold",
+HOLDERS = {"sepia_kv8_append": "sepia_kv8_append", "sepia_kv8_read": "sepia_kv8_read",
            "kv8_attn_run": "sepia_kv8_attn_", "kv8_attn_rows": "sepia_kv8_rows_", "sepia_sample_max": "sepia_sample_max", "sepia_sample_bins": "sepia_sample_bins",
            "sepia_sample_pick": "sepia_sample_pick", "sepia_sample": "sepia_sample"}
 
@@ -20,7 +20,7 @@ HOLDERS = {"sepia_kv8_append": "sepia_kv8_append", "sepia_kv8_read": "sepia_kv8_
 def test_serve_args_within_segment(tmp_path, monkeypatch):
     monkeypatch.setattr(warm, "HSACO", hip.SERVE_HSACO_PATH)
     seg = warm.kernel_segments(tmp_path)
-    assert len(seg) == 15, sorted(seg)
+    assert len(seg) == 14, sorted(seg)
     seen = set()
     for name in ("kv8.h", "kv8_attn.h", "sample.h"):
         text = open(os.path.join(warm.KDIR, name)).read()
