@@ -97,12 +97,17 @@ __device__ __forceinline__ T kv8_last(T v) {
 // The id-th run in the order sequence, row tile, split, kv head; 0 past the last.
 __device__ __forceinline__ int kv8_plan(const Kv8Args &a, const Kv8Attn &b, int id, Kv8Plan &p) {
     const int lane = (int)(threadIdx.x & 63);
-    float total = 0.0f;
+    float total = 0.0f, tiles = 0.0f;
     int rt, steps, len, r0, r1;
     for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
         kv8_cost(a, b, s0 + lane, rt, steps, len, r0, r1);
         total += kv8_last(kv8_scan((float)rt * (float)steps));
+        tiles += kv8_last(kv8_scan((float)rt));
     }
+    // More tiles than the grid was made for: starts fall somewhere (an error,
+    // kv8_check). No run then, since a unit with some of its runs would leave its
+    // counter behind.
+    if (tiles > (float)(a.n / b.TT + a.n_seqs)) return 0;
     const int chunk = b.budget > 0 ? max(KV8_NW, (int)ceilf(fminf(total * (float)a.Hkv / (float)b.budget, 1e9f))) : 0x7FFFFFFF;
     // A unit of two steps a wave stays whole: the fold takes longer than the
     // second step (32 sequences of up to 500 columns, 8 kv heads: 12.2 us against

@@ -253,6 +253,30 @@ def test_graphs_outlive_their_scratch(dev):
         dev.free(b)
 
 
+def test_call_after_falling_starts(dev):
+    """Starts that fall give sequences more row tiles than the call has: an error, and the next calls are right (the runs
+    of a unit that is cut count themselves, and all of them or none have to be there)."""
+    L = dev.L
+    rng = np.random.default_rng(41)
+    H, heads, dim, page, lens = 32, 2, 64, 16, [2500, 2500, 2500, 2500, 2500]
+    c, starts, n = make(rng, heads, dim, page, lens, [7, 1, 0, 1, 1])
+    g = OnGpu(dev, c)
+    q = normal(rng, n, H, dim)
+    want, tol = c.attn(lens, starts, q, None, None, 0, 1 / dim)
+    lb, qb, ob = ints(dev, lens), dev.shared_from(q), dev.alloc(q.nbytes)
+    for bad in ([0, 7, 0, 7, 0, 7], [0, n, 0, n, 0, n], [3, n, 1, n, 0, n]):
+        sb = ints(dev, bad)
+        dev.begin()
+        assert L.sepia_hip_kv8_attn(B(g.desc), lb, sb, n, qb, None, None, ob, H, 0, 0, 1 / dim) == 1
+        assert L.sepia_gpu_end() == 0
+        dev.free(sb)
+        got = attn(dev, g, lens, starts, q, None, None, 0, 1 / dim)
+        assert np.all(np.abs(got - want) <= tol + np.abs(want) * 2.0 ** -23), bad
+    for b in (lb, qb, ob):
+        dev.free(b)
+    g.free()
+
+
 def test_grid_past_the_launch_limit(dev):
     """65536 sequences of 300 kv heads: more workgroups than a launch can have; refused, not cut short."""
     L = dev.L
