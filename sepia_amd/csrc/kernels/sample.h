@@ -38,6 +38,7 @@
 #pragma once
 #include "common.h"
 #include "serve.h"
+#include <stddef.h>
 
 #define SAMPLE_ONE 8796093022208.0    // 2^43: the largest weight
 #define SAMPLE_NT 512                 // two workgroups a CU (of 1024 threads one: 36 against 26 us at 48 rows)
@@ -375,11 +376,14 @@ __device__ __forceinline__ SampleAt sample_settle(const SampleAsk &q, int b, boo
             });
         }
     };
-    // the places from `first` on, 2^bits of them
-    unsigned long long first = (unsigned long long)sample_key(sample_most(q, b)) << 20, before = 0;
-    const unsigned long long last = ((unsigned long long)sample_key(fmaxf(sample_least(q, b), -3.402823466e38f)) << 20) | 0xFFFFF;
-    int bits = 64 - __builtin_clzll((last - first) | 1);
+    unsigned long long first = 0, before = 0;   // the places from `first` on, 2^bits of them
+    int bits = 0;
     uint32_t left = listed || far ? n : q.by_k ? L.cupto[b + 1] - L.cupto[b] : ~0u;   // at most (bins are counted for a k)
+    if (!(listed && n <= SAMPLE_FEW)) {
+        first = (unsigned long long)sample_key(sample_most(q, b)) << 20;
+        const unsigned long long last = ((unsigned long long)sample_key(fmaxf(sample_least(q, b), -3.402823466e38f)) << 20) | 0xFFFFF;
+        bits = 64 - __builtin_clzll((last - first) | 1);
+    }
     while (left > SAMPLE_FEW) {
         const int drop = max(bits - 10, 0);
         sample_clear(L);
@@ -565,6 +569,24 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_bins(Sample
     if (tid == 0) o->over_min = q.over_min;
 }
 
+// A thread's two bins of the row's chunks added up, eight chunks' loads in
+// flight (four: 3.0 us of 13 chunks, as each round of them is one of memory).
+template <class T>
+__device__ __forceinline__ void sample_add(const SampleChunk *o, int chunks, size_t field, T *to) {
+    typedef T Pair __attribute__((ext_vector_type(2)));
+    Pair sum = {0, 0};
+    for (int i = 0; i < chunks; i += 8) {
+        Pair v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = ((const Pair *)((const char *)(o + min(i + j, chunks - 1)) + field))[threadIdx.x];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (i + j < chunks) sum += v[j];
+    }
+    to[2 * threadIdx.x] = sum[0];
+    to[2 * threadIdx.x + 1] = sum[1];
+}
+
 // Grid (chunks, rows): the decision, over the chunks' bins. 12 and 76 us: the
 // row read again, then scans, barriers and the last workgroup's decisions.
 extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_pick(SampleArgs a) {
@@ -574,37 +596,11 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_pick(Sample
     SampleAsk q = sample_ask(a, row);
     if (sample_done(a, row, q, sample_first(a, row, L.wave), false)) return;
     const SampleChunk *o = a.bins + (int64_t)row * a.chunks;
-    unsigned long long mass[2] = {0, 0}, over_min = 0;
-    uint32_t count[2] = {0, 0};
-    for (int i = 0; i < a.chunks; i += 4) {   // four chunks' loads in flight
-        unsigned long long m[4][2], f[4];
-        uint32_t n[4][2];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const SampleChunk &h = o[min(i + j, a.chunks - 1)];
-            f[j] = h.over_min;
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                m[j][e] = h.mass[tid + e * SAMPLE_NT];
-                n[j][e] = q.k > 0 ? h.count[tid + e * SAMPLE_NT] : 0;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (i + j >= a.chunks) break;
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                mass[e] += m[j][e];
-                count[e] += n[j][e];
-            }
-            over_min = f[j] == ~0ull ? f[j] : over_min + f[j];
-        }
-    }
-    q.over_min = over_min;
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-        L.mass[tid + e * SAMPLE_NT] = mass[e];
-        L.count[tid + e * SAMPLE_NT] = count[e];
+    sample_add<unsigned long long>(o, a.chunks, offsetof(SampleChunk, mass), L.mass);
+    if (q.k > 0) sample_add<uint32_t>(o, a.chunks, offsetof(SampleChunk, count), L.count);
+    if (q.f > 0.0f) {   // a lane a chunk, every wave for itself
+        const unsigned long long sum = sample_sums((tid & 63) < a.chunks ? o[tid & 63].over_min : 0);
+        q.over_min = sample_lane(sum, 63);
     }
     L.pow.fill();
     const float least = sample_bounds(q, L);
