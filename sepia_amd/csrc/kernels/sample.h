@@ -587,7 +587,7 @@ __device__ __forceinline__ void sample_add(const SampleChunk *o, int chunks, siz
     to[2 * threadIdx.x + 1] = sum[1];
 }
 
-// Grid (chunks, rows): the decision, over the chunks' bins. 12 and 76 us: the
+// Grid (chunks, rows): the decision, over the chunks' bins. 10 and 75 us: the
 // row read again, then scans, barriers and the last workgroup's decisions.
 extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_pick(SampleArgs a) {
     __shared__ SampleLds L;
