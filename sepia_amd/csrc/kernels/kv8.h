@@ -52,10 +52,11 @@ __device__ __forceinline__ int kv8_seq(const Kv8Args &a, int s, int32_t &len, in
     return kv8_seq_ok(len, r0, r1, a.n, (int64_t)a.max_pages << a.lg);
 }
 
-// The sequence that owns `id`, its length and rows; -1 if there is none, or
-// one that cannot be used. 64 sequences a look: one round for up to 64 of
+// The sequence that owns `id`, which of its units that is, its length and rows;
+// -1 if there is none, or one that cannot be used. 64 sequences a look: one round for up to 64 of
 // them, with everything about the one found already loaded, two for 4096.
-__device__ __forceinline__ int kv8_find(const Kv8Args &a, int64_t id, int gran, int extra, int32_t &len, int32_t &r0, int32_t &r1) {
+__device__ __forceinline__ int kv8_find(const Kv8Args &a, int64_t id, int gran, int extra, int32_t &k, int32_t &len, int32_t &r0,
+                                        int32_t &r1) {
     const int lane = (int)(threadIdx.x & 63);
     int lo = 0, n = a.n_seqs;
     while (true) {
@@ -69,7 +70,8 @@ __device__ __forceinline__ int kv8_find(const Kv8Args &a, int64_t id, int gran, 
             r0 = __builtin_amdgcn_readlane(r0, c - 1);
             r1 = __builtin_amdgcn_readlane(r1, c - 1);
             len = __builtin_amdgcn_readlane(len, c - 1);
-            return kv8_seq_ok(len, r0, r1, a.n, (int64_t)a.max_pages << a.lg) ? lo + c - 1 : -1;
+            const int found = lo + c - 1;
+            return kv8_place(id, r0, found, gran, extra, &k) && kv8_seq_ok(len, r0, r1, a.n, (int64_t)a.max_pages << a.lg) ? found : -1;
         }
         lo += (c - 1) * step;
         n = min(step, n - (c - 1) * step);
@@ -181,11 +183,11 @@ extern "C" __global__ __launch_bounds__(256, 3) void sepia_kv8_append(Kv8Args a,
     const int hk = min(head, a.Hkv - 1);
     const bool mine = head < a.Hkv;   // else the wave only keeps the others company at the barrier
     kv8_check(a);
-    int32_t len, r0, r1;
-    const int s = kv8_find(a, blockIdx.x, a.gran, a.extra, len, r0, r1);
+    int32_t k_unit, len, r0, r1;
+    const int s = kv8_find(a, blockIdx.x, a.gran, a.extra, k_unit, len, r0, r1);
     Kv8Unit u;
     if (s < 0) return;
-    if (!kv8_unit(len, r0, r1, (int)(blockIdx.x - kv8_first_id(r0, s, a.gran, a.extra)), a.lg, &u)) return;
+    if (!kv8_unit(len, r0, r1, k_unit, a.lg, &u)) return;
     // The rows are asked for before the table's entry is waited for.
     const int page = kv8_page(a, s, u.page);
     const int64_t ld = (int64_t)a.Hkv * a.Dh;
@@ -341,11 +343,11 @@ extern "C" __global__ __launch_bounds__(256) void sepia_kv8_read(Kv8Args a, floa
     const int hk = head;
     kv8_check(a);
     if (head >= a.Hkv) return;
-    int32_t len, r0, r1;
-    const int s = kv8_find(a, blockIdx.x, a.gran, a.extra, len, r0, r1);
+    int32_t k_unit, len, r0, r1;
+    const int s = kv8_find(a, blockIdx.x, a.gran, a.extra, k_unit, len, r0, r1);
     Kv8Unit u;
     if (s < 0) return;
-    if (!kv8_unit(len, r0, r1, (int)(blockIdx.x - kv8_first_id(r0, s, a.gran, a.extra)), a.lg, &u)) return;
+    if (!kv8_unit(len, r0, r1, k_unit, a.lg, &u)) return;
     const int page = kv8_page(a, s, u.page);
     if (page < 0) {
         sepia_report_error(nullptr, KV8_ERR_PAGE, (int)threadIdx.x);

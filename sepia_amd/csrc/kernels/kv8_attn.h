@@ -696,9 +696,9 @@ __device__ __forceinline__ void kv8_attn_rows(const Kv8Args &a, const Kv8Attn &b
     Kv8Plan p;
     const int id = (int)blockIdx.x / a.Hkv, gran = KV8_NW * b.TT;
     p.hk = (int)blockIdx.x - id * a.Hkv;
-    p.s = kv8_find(a, id, gran, 1, p.len, p.r0, p.r1);
+    p.s = kv8_find(a, id, gran, 1, p.k, p.len, p.r0, p.r1);
     if (p.s < 0) return;
-    p.k = (id - (int)kv8_first_id(p.r0, p.s, gran, 1)) * KV8_NW + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    p.k = p.k * KV8_NW + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     if ((int64_t)p.k * b.TT >= p.r1 - p.r0) return;
     const Kv8Tile t = kv8_tile(b, p, 1);
     const int lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4;

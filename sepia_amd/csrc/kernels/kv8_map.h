@@ -24,6 +24,13 @@
 KV8_FN int64_t kv8_first_id(int32_t start, int32_t s, int32_t gran, int32_t extra) {
     return (int64_t)(start / gran) + (int64_t)extra * s;
 }
+// The unit of sequence s that `id` stands for; 0 where the sequence's ids begin
+// behind it, as they may for the one that a search finds where starts fall.
+KV8_FN int kv8_place(int64_t id, int32_t start, int32_t s, int32_t gran, int32_t extra, int32_t *k) {
+    const int64_t first = kv8_first_id(start, s, gran, extra);
+    *k = (int32_t)(id - first);
+    return id >= first;
+}
 // Ids of a call of n rows.
 KV8_FN int64_t kv8_ids(int64_t n, int32_t n_seqs, int32_t gran, int32_t extra) {
     return n / gran + (int64_t)extra * n_seqs;

@@ -1,0 +1,49 @@
+"""The serving operators at the edges of what a call may be handed."""
+import numpy as np
+import pytest
+
+from sepia_amd import hip
+from test_gpu_kv8 import B, OnGpu, ints, make, normal
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return hip.Device()
+
+
+@pytest.mark.parametrize("heads,H", [(2, 4), (64, 64)], ids=["few", "many"])
+def test_falling_starts(dev, heads, H):
+    """Starts that fall, so that the search finds a sequence whose ids begin behind the one that is looked for: an error,
+    and no page, row or output beside those of the sequences is touched. (As many units as take a wave each, too.)"""
+    rng = np.random.default_rng(heads)
+    dim, page, lens = 16, 16, [5, 5, 5]
+    c, _, _ = make(rng, heads, dim, page, lens, [40, 40, 40], spare=6)
+    n = 60
+    q, k = normal(rng, n, H, dim), normal(rng, n, heads * dim)
+    for starts in ([50, 60, 10, 20], [59, 60, 0, 1], [40, 41, 1, 2], [60, 0, 60, 0], [30, 60, 0, 30]):
+        g = OnGpu(dev, c)
+        before, scales = g.codes(), g.scales()
+        out = np.full((n, H, dim), 7.0, np.float32)
+        rows = np.full((n, heads * dim), 7.0, np.float32)
+        bufs = [ints(dev, lens), ints(dev, starts), dev.shared_from(q), dev.shared_from(out), dev.shared_from(k),
+                dev.shared_from(rows), dev.shared_from(rows)]
+        for call in (lambda: dev.L.sepia_hip_kv8_attn(B(g.desc), bufs[0], bufs[1], n, bufs[2], None, None, bufs[3], H, 0, 0, 1 / dim),
+                     lambda: dev.L.sepia_hip_kv8_read(B(g.desc), bufs[0], bufs[1], n, bufs[5], bufs[6]),
+                     lambda: dev.L.sepia_hip_kv8_append(B(g.desc), bufs[0], bufs[1], n, bufs[4], bufs[4], None, 0.0)):
+            dev.begin()
+            assert call() == 1
+            assert dev.L.sepia_gpu_end() == 0 and dev.L.sepia_hip_take_device_error() == 0
+        fits = [(s, a, b) for s, (a, b) in enumerate(zip(starts, starts[1:])) if a <= b and lens[s] + b - a <= page * c.max_pages]
+        inside = np.zeros(n, bool)
+        for _, a, b in fits:
+            inside[a:b] = True
+        for b, a in ((bufs[3], out), (bufs[5], rows), (bufs[6], rows)):
+            assert np.all(dev.download(b, a.size).reshape(a.shape)[~inside] == 7.0), starts
+        mine = {c.table[s, p // page] for s, a, b in fits for p in range(lens[s], lens[s] + b - a)}
+        rest = [p for p in range(c.n_pages) if p not in mine]
+        assert np.array_equal(g.codes()[rest], before[rest]) and np.array_equal(g.scales()[rest], scales[rest]), starts
+        for b in bufs:
+            dev.free(b)
+        g.free()
