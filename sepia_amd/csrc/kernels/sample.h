@@ -637,5 +637,7 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample(SampleArgs 
     sample_bins(q, 0, a.vocab, L);
     const float least = sample_bounds(q, L);
     sample_gather(q, least, 0, a.vocab, L, nullptr);
-    sample_finish(a, row, q, L.n, nullptr, L);
+    const uint32_t n = L.n;
+    __syncthreads();   // every wave has it: a decision among few tokens of many uses L.n at once
+    sample_finish(a, row, q, n, nullptr, L);
 }

@@ -4,6 +4,7 @@ import pytest
 
 from sepia_amd import hip
 from test_gpu_kv8 import B, OnGpu, ints, make, normal
+from test_gpu_sample import check
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +48,18 @@ def test_falling_starts(dev, heads, H):
         for b in bufs:
             dev.free(b)
         g.free()
+
+
+@pytest.mark.parametrize("vocab", [5000, 20000, 24575])
+def test_few_below_a_long_run(dev, vocab):
+    """A row of one workgroup, all but ten of whose logits are equal, more than a workgroup gathers, and whose k-th token
+    is among the ten in a bin below: they are decided at once, without a search by pieces before."""
+    rng = np.random.default_rng(vocab)
+    x = np.full((64, vocab), 2.0, np.float32)
+    for r in range(64):
+        x[r, rng.choice(vocab, 10, replace=False)] = 1.0 - 0.0005 * np.arange(10, dtype=np.float32)
+    # within the run, and at its end: one to ten tokens of weight 0.37 behind vocab - 10 of weight 1
+    u = np.where(np.arange(64) % 2, 1.0 - 10.0 ** -rng.uniform(3.5, 5.5, 64), rng.random(64)).astype(np.float32)
+    for below in (1, 5, 9):
+        check(dev, x, vocab, u, top_k=vocab - 10 + below)
+        check(dev, x, vocab, u, top_k=vocab - 10 + below, temperature=1.5, top_p=0.9999)
