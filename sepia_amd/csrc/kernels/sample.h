@@ -623,6 +623,7 @@ extern "C" __global__ __launch_bounds__(SAMPLE_NT) void sepia_sample_pick(Sample
     if (total <= SAMPLE_CAP)
         for (int i = tid; i < (int)total; i += SAMPLE_NT)
             L.list[i] = __hip_atomic_load(&r->list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();   // a few tokens are compared at once, by every wave
     sample_finish(a, row, q, total, total <= SAMPLE_MANY ? r : nullptr, L);
 }
 

@@ -63,3 +63,15 @@ def test_few_below_a_long_run(dev, vocab):
     for below in (1, 5, 9):
         check(dev, x, vocab, u, top_k=vocab - 10 + below)
         check(dev, x, vocab, u, top_k=vocab - 10 + below, temperature=1.5, top_p=0.9999)
+
+
+def test_few_gathered_of_chunks(dev):
+    """Rows in chunks whose decisions are among a handful of gathered tokens, three decisions in a row."""
+    rng = np.random.default_rng(5)
+    vocab, rows = 30000, 24
+    x = (rng.standard_normal((rows, vocab)) - 40).astype(np.float32)
+    for r in range(rows):
+        x[r, rng.choice(vocab, 12, replace=False)] = np.linspace(3, 0, 12).astype(np.float32)
+    u = rng.random(rows).astype(np.float32)
+    for params in (dict(), dict(top_k=7), dict(top_k=9, top_p=0.8), dict(top_k=10, top_p=0.95, min_p=0.2)):
+        check(dev, x, vocab, u, **params)
