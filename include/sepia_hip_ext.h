@@ -137,8 +137,9 @@ typedef struct {
  * x * k_norm / sqrt(mean(x^2) + eps) first. The scale of a (page, K or V,
  * head) covers the page's tokens so far: it grows to the largest new
  * magnitude / 127 (in f32, times 1 / 127) where that is larger, and the codes
- * that are there are rounded anew; a page's first token starts it afresh. A value that is not
- * finite makes that scale NaN, and with it what the page's head stands for.
+ * that are there are rounded anew (to 0 behind a scale of 0); a page's first
+ * token starts it afresh. A value that is not finite makes that scale NaN, and
+ * with it what the page's head stands for.
  * Two sequences of one call may not append to the same page. */
 int sepia_hip_kv8_append(const SepiaKv8Cache *cache, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n_tokens,
                          SepiaGpuBuf *k, SepiaGpuBuf *v, SepiaGpuBuf *k_norm, float eps);

@@ -162,7 +162,7 @@ __device__ __forceinline__ Kv8Scale kv8_rescale(float *scale, float old, float m
     if (mine && wave == w0 && (threadIdx.x & 63) == 0) *scale = s;
     Kv8Scale r;
     r.inv = s > 0.0f ? kv8_rcp((double)s) : 0.0;
-    r.ratio = s > old && old > 0.0f ? (double)old * r.inv : 1.0;
+    r.ratio = s > old ? (double)old * r.inv : 1.0;   // 0 behind a scale of 0, whose codes stand for 0
     return r;
 }
 

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from sepia_amd import hip
-from test_gpu_kv8 import B, OnGpu, ints, make, normal
+from test_gpu_kv8 import B, OnGpu, append, ints, make, normal
 from test_gpu_sample import check
 
 pytestmark = pytest.mark.gpu
@@ -75,3 +75,44 @@ def test_few_gathered_of_chunks(dev):
     u = rng.random(rows).astype(np.float32)
     for params in (dict(), dict(top_k=7), dict(top_k=9, top_p=0.8), dict(top_k=10, top_p=0.95, min_p=0.2)):
         check(dev, x, vocab, u, **params)
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (16, 64), (128, 32)])
+def test_append_behind_a_scale_of_zero(dev, dim, page):
+    """Codes whose scale is 0 stand for 0, and still do when a page's scale grows: they are rounded anew to 0. A scale that
+    stays 0 leaves them."""
+    rng = np.random.default_rng(dim)
+    heads, lens, news = 3, [page - 5, page + 7, 3], [2, page, 1]
+    c, starts, n = make(rng, heads, dim, page, lens, news)
+    firsts = [c.table[s, lens[s] // page] for s in range(3)]
+    for p in firsts:
+        c.scales[p, 0, :2] = 0.0   # K of heads 0 and 1, V of heads 1 and 2
+        c.scales[p, 1, 1:] = 0.0
+    k, v = normal(rng, n, heads * dim), normal(rng, n, heads * dim)
+    k[:, dim:2 * dim] = 0.0        # head 1: nothing but zeros comes, the scale stays 0
+    v[:, dim:2 * dim] = 0.0
+    g = OnGpu(dev, c)
+    append(dev, g, lens, starts, k, v)
+    codes, scales = g.codes(), g.scales()
+    c.append(lens, starts, k, v)   # its scales and new codes; of the old ones below
+    assert np.array_equal(scales, c.scales)
+    for s, p in enumerate(firsts):
+        at = lens[s] % page
+        for side, zero in ((0, 0), (1, 2)):
+            assert scales[p, side, zero] > 0
+            c.views(p)[side][:at, zero] = 0
+        assert scales[p, 0, 1] == 0 and scales[p, 1, 1] == 0
+    assert np.array_equal(codes, c.codes)
+    # what the pages stand for: the old positions of those heads are 0
+    rows = int(sum(lens))
+    back = np.concatenate([[0], np.cumsum(lens)])
+    bufs = [ints(dev, [0, 0, 0]), ints(dev, back), dev.alloc(rows * heads * dim * 4), dev.alloc(rows * heads * dim * 4)]
+    dev.run(dev.L.sepia_hip_kv8_read, B(g.desc), bufs[0], bufs[1], rows, bufs[2], bufs[3])
+    for side, zero in ((0, 0), (1, 2), (0, 1), (1, 1)):
+        got = dev.download(bufs[2 + side], rows * heads * dim).reshape(rows, heads, dim)
+        for s in range(3):
+            old = got[back[s]:back[s + 1]]
+            assert np.all(old[lens[s] // page * page:, zero] == 0.0)
+    for b in bufs:
+        dev.free(b)
+    g.free()
