@@ -211,8 +211,10 @@ int sepia_hip_set_iq2xxs_grid(const uint64_t *grid256);
  * run the call once, or reserve, before beginning a capture. (banded_attn and
  * kv8_attn take fewer splits first, sample a workgroup a row; moe_prefill may
  * run in parts, above.) A captured call's scratch stays until shutdown when a
- * later call grows the region, so its graph may still be replayed; graphs are
- * replayed on the library's stream, whose scratch they share. Needs init. */
+ * later call grows the region, so its graph may still be replayed; the new
+ * region is at least twice as large, where there is memory for that, so the
+ * ones that stay are together no larger than it. Graphs are replayed on the
+ * library's stream, whose scratch they share. Needs init. */
 int sepia_hip_reserve_scratch(size_t bytes);
 
 /* Bytes of the library's growable scratch region (0 before its first use).

@@ -385,8 +385,9 @@ static int prep_out(SepiaGpuBuf *b, const char *op) {
 static void *g_scratch;
 static size_t g_scratch_len;
 static int g_scratch_held;                  /* a captured call has its address */
-static void *g_scratch_old[64];             /* held regions that were outgrown */
+static void **g_scratch_old;                /* held regions that were outgrown */
 static int g_scratch_olds;
+static size_t g_scratch_min;                /* twice the largest of them */
 
 /* Data region of at least `need` bytes (the counters sit in front of it).
  * Growing waits for the stream, since queued kernels may still use the old
@@ -395,7 +396,9 @@ static int g_scratch_olds;
  * being captured a region that is too small is an error (run the same call
  * once before the capture, or reserve with sepia_hip_reserve_scratch). A region
  * that a captured call was given stays until the library shuts down, since its
- * graph may be replayed after a later call has grown the scratch. */
+ * graph may be replayed after a later call has grown the scratch. The one in
+ * its place has at least twice its size (where there is memory for that), so
+ * that all the ones kept are together no larger than the last. */
 static void *scratch(size_t need, const char *op) {
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
     const int capturing = hipStreamIsCapturing(g_stream, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone;
@@ -409,20 +412,30 @@ static void *scratch(size_t need, const char *op) {
             op, need, g_scratch ? g_scratch_len - CNT_BYTES : (size_t)0);
         return NULL;
     }
-    if (g_scratch_held && g_scratch_olds == (int)(sizeof g_scratch_old / sizeof *g_scratch_old)) {
-        LOG("%s: the scratch has been outgrown %d times with captured calls in it; reserve it before capturing", op,
-            g_scratch_olds);
-        return NULL;
+    if (g_scratch_held) {
+        void **olds = (void **)realloc(g_scratch_old, ((size_t)g_scratch_olds + 1) * sizeof *olds);
+        if (!olds) {
+            LOG("%s: out of host memory", op);
+            return NULL;
+        }
+        g_scratch_old = olds;
+        olds[g_scratch_olds++] = g_scratch;
+        if (g_scratch_min < 2 * g_scratch_len) g_scratch_min = 2 * g_scratch_len;
     }
     hipStreamSynchronize(g_stream);
-    if (g_scratch_held) g_scratch_old[g_scratch_olds++] = g_scratch;
-    else if (g_scratch) hipFree(g_scratch);
+    if (g_scratch && !g_scratch_held) hipFree(g_scratch);
     g_scratch = NULL;
     g_scratch_len = 0;
     g_scratch_held = 0;
-    size_t want = CNT_BYTES + (need < (4u << 20) ? (4u << 20) : need);
+    const size_t least = CNT_BYTES + (need < (4u << 20) ? (4u << 20) : need);
+    size_t want = least < g_scratch_min ? g_scratch_min : least;
     g_allocs++;
     hipError_t e = hipMalloc(&g_scratch, want);
+    if (e != hipSuccess && want > least) {
+        (void)hipGetLastError();   /* nothing of it is left for the caller's next call */
+        want = least;
+        e = hipMalloc(&g_scratch, want);
+    }
     if (e == hipSuccess) e = hipMemsetAsync(g_scratch, 0, want, g_stream);
     if (e == hipSuccess) e = hipStreamSynchronize(g_stream);
     if (e != hipSuccess) {
@@ -838,6 +851,9 @@ void sepia_gpu_shutdown(void) {
     pool_release_all();
     if (g_scratch) hipFree(g_scratch);
     while (g_scratch_olds > 0) hipFree(g_scratch_old[--g_scratch_olds]);
+    free(g_scratch_old);
+    g_scratch_old = NULL;
+    g_scratch_min = 0;
     g_scratch = NULL;
     g_scratch_len = 0;
     g_scratch_held = 0;

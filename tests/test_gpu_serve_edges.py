@@ -1,10 +1,14 @@
 """The serving operators at the edges of what a call may be handed."""
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
 from sepia_amd import hip
 from test_gpu_kv8 import B, OnGpu, append, ints, make, normal
 from test_gpu_sample import check
+from test_gpu_serve_run import ROOT
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +120,46 @@ def test_append_behind_a_scale_of_zero(dev, dim, page):
     for b in bufs:
         dev.free(b)
     g.free()
+
+
+GROWTH = r"""
+import sys
+sys.path[:0] = [sys.argv[1], sys.argv[1] + "/tests"]
+import numpy as np
+from np_serve import sample
+from sepia_amd import hip
+from test_gpu_serve_run import B, Hip, normal
+dev = hip.Device()
+L, h = dev.L, Hip(dev)
+rng = np.random.default_rng(2)
+rows, vocab = 3, 30000
+x, u = normal(rng, rows, vocab, scale=3.0), rng.random(rows).astype(np.float32)
+xb, ub, tb = h.private(x), h.private(u), dev.alloc(4 * rows, private=True)
+desc = hip.SampleDesc(u=ub)
+op = lambda: L.sepia_hip_sample(B(desc), xb, rows, vocab, vocab, tb, None)
+tokens = [sample(x[r], u[r])[0] for r in range(rows)]
+graphs, sizes = [], set()
+for i in range(90):   # the engine's way: a call of the next size, once, then its capture
+    assert L.sepia_hip_reserve_scratch((4 << 20) + (i << 18)) == 1, i
+    sizes.add(L.sepia_hip_scratch_bytes())
+    graphs.append(h.capture(op))
+    if i % 9 == 0:
+        for exe in graphs[::5] + graphs[-1:]:
+            h.put(tb, np.full(rows, -7, np.int32))
+            h.replay(exe)
+            assert list(h.get(tb, rows, np.int32)) == tokens, i
+assert L.sepia_hip_reserve_scratch(200 << 20) == 1
+assert len(sizes) < 12 and max(sizes) < 2 * ((4 << 20) + (90 << 18)) + (1 << 20), sorted(sizes)
+dev.begin()
+assert op() == 1
+dev.end()
+assert list(h.get(tb, rows, np.int32)) == tokens
+print("ok")
+"""
+
+
+def test_scratch_grows_among_many_captures():
+    """In a process of its own: 90 calls, each of a little more scratch and captured once it ran. The regions that graphs
+    hold are few, since each is at least twice the one before, and none of the calls is refused."""
+    r = subprocess.run([sys.executable, "-c", GROWTH, ROOT], capture_output=True, text=True, cwd=ROOT, timeout=100)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stdout + r.stderr
