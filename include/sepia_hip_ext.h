@@ -173,7 +173,7 @@ typedef struct {
 
 /* The next token of each row of logits (f32, up to 65535 rows, row r at element
  * r * stride, vocab values of it, 1 to 2^20). A token's weight is exp((logit - largest) /
- * temperature); -inf and NaN have none. In the order of falling logits, equal
+ * temperature); -inf and NaN have none, nor has a token beside one of +inf. In the order of falling logits, equal
  * ones by index: the first top_k tokens are kept, of these the shortest
  * beginning with at least top_p of their weight, of these the ones of weight
  * min_p or more. tokens[r] (int32) is the first whose cumulative weight

@@ -2,7 +2,8 @@
 // top-p, min-p, and a draw by a given uniform number.
 //
 // With x the row's logits, m their maximum and T the temperature, a token's
-// weight is w = e^((x - m) / T); -inf and NaN have none. The tokens are
+// weight is w = e^((x - m) / T); -inf and NaN have none, nor has a token below
+// one of +inf. The tokens are
 // ordered by falling logit, equal ones by index. Kept are the first k of them
 // (top-k), of these the shortest beginning whose weight reaches p of theirs
 // (top-p), and of these the ones with w >= min-p: a beginning of the order
@@ -492,7 +493,7 @@ __device__ __forceinline__ SampleAsk sample_ask(const SampleArgs &a, int row) {
 // all there is to decide (the workgroup of `write` says so).
 __device__ __forceinline__ bool sample_done(const SampleArgs &a, int row, SampleAsk &q, unsigned long long best, bool write) {
     q.m = sample_logit((uint32_t)(best >> 20));
-    q.scale = 256.0 * 1.4426950408889634074 / (double)q.t;
+    q.scale = 256.0 * 1.4426950408889634074 / (q.m < INFINITY ? (double)q.t : 1.0);   // below +inf nothing weighs, at any T
     if (best != SAMPLE_NONE && q.t > 0.0f && q.k != 1) return false;
     if (write && threadIdx.x == 0) {
         a.token[row] = best == SAMPLE_NONE ? -1 : (int32_t)(best & 0xFFFFF);

@@ -7,7 +7,7 @@ import pytest
 
 from sepia_amd import hip
 from test_gpu_kv8 import B, OnGpu, append, ints, make, normal
-from test_gpu_sample import check
+from test_gpu_sample import check, run
 from test_gpu_serve_run import ROOT
 
 pytestmark = pytest.mark.gpu
@@ -163,3 +163,22 @@ def test_scratch_grows_among_many_captures():
     hold are few, since each is at least twice the one before, and none of the calls is refused."""
     r = subprocess.run([sys.executable, "-c", GROWTH, ROOT], capture_output=True, text=True, cwd=ROOT, timeout=100)
     assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("rows,vocab", [(6, 3000), (3, 60000)], ids=["whole", "chunks"])
+def test_infinite_temperature_and_logits(dev, rows, vocab):
+    """A +inf logit leaves all others without weight at every temperature, an infinite one too."""
+    rng = np.random.default_rng(vocab)
+    for count in (1, 2, 40, 300):
+        x = normal(rng, rows, vocab)
+        at = [np.sort(rng.choice(vocab, count, replace=False)) for _ in range(rows)]
+        for r in range(rows):
+            x[r, at[r]] = np.inf
+        u = rng.random(rows).astype(np.float32)
+        for t in (np.inf, 3e38, 1.0, 1e-45):
+            for more in (dict(), dict(top_k=vocab - 1), dict(top_p=0.75), dict(min_p=0.5)):
+                token, prob = run(dev, x, vocab, u, temperature=t, **more)
+                kept = max(1, int(np.ceil(0.75 * count))) if "top_p" in more else count
+                for r in range(rows):
+                    assert token[r] == at[r][min(int(np.float64(u[r]) * kept), kept - 1)], (count, t, more, r)
+                    assert abs(prob[r] - 1 / kept) <= 2.0 ** -24 / kept * 2
