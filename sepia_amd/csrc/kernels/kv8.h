@@ -19,19 +19,13 @@
 #include "common.h"
 #include "kv8_map.h"
 #include "serve.h"
+#include "serve_layout.h"
 
 #define KV8_ERR_PAGE 6u   // device error: a page of the table outside the pool
 #define KV8_ERR_SEQ 7u    // device error: lens or starts that do not fit the call
 
-// What every kernel is given (the host's struct in serve.c mirrors it).
-struct Kv8Args {
-    int8_t *codes;
-    float *scales;
-    const int32_t *table, *lens, *starts;
-    int64_t n_pages;
-    int32_t n_seqs, max_pages, Hkv, Dh, lg, n;   // n: rows of the call
-    uint32_t head_bytes, page_bytes;             // of a head's K or V in a page, of a page
-    int32_t gran, extra;                         // the id space of the pages (kv8_map.h)
+// What every kernel is given.
+struct Kv8Args : Kv8Call {
     __device__ __forceinline__ int P() const { return 1 << lg; }
     __device__ __forceinline__ int8_t *k_codes(uint32_t page, int hk) const {
         return codes + (uint64_t)hk * head_bytes + (uint64_t)page * page_bytes;

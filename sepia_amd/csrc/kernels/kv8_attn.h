@@ -24,21 +24,12 @@
 #pragma once
 #include "kv8.h"
 
-#define KV8_NW 4             // waves of a workgroup: they take a unit's steps in turn
 #define KV8_C 8355711.0f     // 0x7F7F7F: the largest magnitude of three digits
 #define KV8_CP 4177855.0f    // half of it: a weight's place relative to a power of two
 #define KV8_L2E 1.44269504f
 #define KV8_LAZY 5.0f        // how far a maximum may rise before the sums are scaled anew
 
-struct Kv8Attn {
-    const float *q, *rel, *tau;
-    float *out;
-    float *part, *ml;        // per run: O [16][Dh]; maxima [16], sums [16]
-    uint32_t *arrived;       // at a group's first run's place: its runs that are done; KV8_UNITS on, at a unit's
-                             // first run's place: its groups
-    int32_t H, R, window, TT, budget;   // TT: tokens of a row tile
-    float c;
-};
+typedef Kv8AttnCall Kv8Attn;
 
 typedef int32_t kv8_i4 __attribute__((ext_vector_type(4)));
 typedef float kv8_f4 __attribute__((ext_vector_type(4)));
@@ -530,7 +521,6 @@ __device__ __forceinline__ float *kv8_out(const Kv8Args &a, const Kv8Attn &b, co
 }
 #define KV8_AHEAD 8   // partials whose loads are in flight at a time
 #define KV8_RUNS 16   // of a unit that are folded at once; more are folded in groups first
-#define KV8_UNITS 8192
 
 // Row `row`'s dims d .. d + 3 of n partials, `step` places apart from place `at`
 // on: the sums so far, relative to their maximum.

@@ -39,36 +39,13 @@
 #pragma once
 #include "common.h"
 #include "serve.h"
+#include "serve_layout.h"
 #include <stddef.h>
 
 #define SAMPLE_ONE 8796093022208.0    // 2^43: the largest weight
-#define SAMPLE_NT 512                 // two workgroups a CU (of 1024 threads one: 36 against 26 us at 48 rows)
 #define SAMPLE_WAVES (SAMPLE_NT / 64)
-#define SAMPLE_BINS 1024              // two a thread
 #define SAMPLE_CAP 4096               // gathered tokens in shared memory
-#define SAMPLE_MANY 16384             // and in scratch
 #define SAMPLE_FEW 16                 // tokens that are compared with each other (60 of them took 4 us)
-
-// In scratch where a row has several chunks: a chunk's bins, and what the
-// row's workgroups gather.
-struct SampleChunk {
-    unsigned long long mass[SAMPLE_BINS], over_min, best;
-    uint32_t count[SAMPLE_BINS];
-};
-struct SampleRow {
-    unsigned long long list[SAMPLE_MANY];
-    uint32_t n, arrived;
-};
-struct SampleArgs {
-    const float *logits, *u, *temperature, *top_p, *min_p;
-    const int32_t *top_k;
-    int32_t *token;
-    float *prob;
-    SampleRow *rows;
-    SampleChunk *bins;   // [row][chunk]
-    int64_t stride;
-    int32_t vocab, chunk, chunks;
-};
 
 // Keys fall as logits rise: 0 is the largest. -0 and +0 are equal.
 __device__ __forceinline__ uint32_t sample_key(float x) {

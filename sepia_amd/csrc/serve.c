@@ -7,26 +7,16 @@
 #include <string.h>
 
 #include "../../include/sepia_hip_ext.h"
+#include "kernels/serve_layout.h"
 
 #define LOG(...) sepia_log(__VA_ARGS__)
 #define MAX_ROWS ((int64_t)1 << 24)     /* rows of a call: grids of fewer than 2^32 threads */
 #define MAX_SAMPLES 65535              /* and of a sample call: the grid's second dimension */
 
-/* struct Kv8Args of kernels/kv8.h */
-typedef struct {
-    uint8_t *codes;
-    float *scales;
-    const int32_t *table, *lens, *starts;
-    int64_t n_pages;
-    int32_t n_seqs, max_pages, Hkv, Dh, lg, n;
-    uint32_t head_bytes, page_bytes;
-    int32_t gran, extra;
-} Kv8Args;
-
 /* Checks a cache and a call's rows, and fills the kernels' arguments; `write`:
  * the call writes to the pages. */
 static int kv8_args(const char *op, const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n,
-                    int write, Kv8Args *a) {
+                    int write, Kv8Call *a) {
     if (!c || c->n_pages < 1 || c->max_pages < 1 || c->n_seqs < 1 || c->n_seqs > 65536 || c->n_kv_heads < 1 ||
         c->n_kv_heads > 65535 || n < 0 || n > MAX_ROWS || c->n_pages > 0x7FFFFFFF) {
         LOG("%s: invalid arguments", op);
@@ -66,7 +56,7 @@ static int kv8_args(const char *op, const SepiaKv8Cache *c, SepiaGpuBuf *lens, S
               : !sepia_prep_in(c->codes, c->codes_off, cb, op) || !sepia_prep_in(c->scales, c->scales_off, sb, op))
         return 0;
     memset(a, 0, sizeof *a);
-    a->codes = sepia_buf_dev(c->codes) + c->codes_off;
+    a->codes = (int8_t *)sepia_buf_dev(c->codes) + c->codes_off;
     a->scales = (float *)(sepia_buf_dev(c->scales) + c->scales_off);
     a->table = (const int32_t *)(sepia_buf_dev(c->table) + c->table_off);
     a->lens = (const int32_t *)sepia_buf_dev(lens);
@@ -95,7 +85,7 @@ static int kv8_apart(const char *op, const SepiaKv8Cache *c, const SepiaGpuBuf *
 /* Units of pages, kv heads, K and V; a workgroup takes 64 tokens of the pages'
  * heads. A sequence of r > 0 rows touches at most r / page + 2 pages,
  * and at most r: the id space (kv8_map.h) that is the smaller for the call. */
-static int kv8_pages(int k, const SepiaKv8Cache *c, int64_t n, Kv8Args *a, void **args, const char *op) {
+static int kv8_pages(int k, const SepiaKv8Cache *c, int64_t n, Kv8Call *a, void **args, const char *op) {
     const int heads = 64 / c->page, few = n <= n / c->page + 2 * (int64_t)c->n_seqs;
     a->gran = few ? 1 : c->page;
     a->extra = few ? 0 : 2;
@@ -106,7 +96,7 @@ static int kv8_pages(int k, const SepiaKv8Cache *c, int64_t n, Kv8Args *a, void 
 int sepia_hip_kv8_append(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n, SepiaGpuBuf *k,
                          SepiaGpuBuf *v, SepiaGpuBuf *k_norm, float eps) {
     const char *op = "kv8_append";
-    Kv8Args a;
+    Kv8Call a;
     if (!c || !lens || !starts || !k || !v) {
         LOG("%s: invalid arguments", op);
         return 0;
@@ -138,7 +128,7 @@ int sepia_hip_kv8_append(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf 
 int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *starts, int64_t n, SepiaGpuBuf *k,
                        SepiaGpuBuf *v) {
     const char *op = "kv8_read";
-    Kv8Args a;
+    Kv8Call a;
     if (!c || !first || !starts || !k || !v || k == v || c->n_kv_heads < 1 || c->head_dim < 1) {
         LOG("%s: invalid arguments", op);
         return 0;
@@ -154,27 +144,16 @@ int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *
     return kv8_pages(SK_KV8_READ, c, n, &a, args, op);
 }
 
-/* struct Kv8Attn of kernels/kv8_attn.h */
 #define KV8_ROWS 1024       /* units from which each has a wave of its own */
-#define KV8_NW 4            /* steps of a run at least, one for each wave */
-#define KV8_UNITS 8192
 #define KV8_BUDGET 512      /* runs of a call whose units alone leave the chip idle: two workgroups a CU */
 _Static_assert(2 * (KV8_BUDGET * 3 / 2) + 64 <= KV8_UNITS && 2 * KV8_UNITS <= SEPIA_COUNTERS, "a counter for each slot, twice");
-typedef struct {
-    const float *q, *rel, *tau;
-    float *out;
-    float *part, *ml;
-    uint32_t *arrived;
-    int32_t H, R, window, TT, budget;
-    float c;
-} Kv8Attn;
 
 int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n, SepiaGpuBuf *q,
                        SepiaGpuBuf *rel_logits, SepiaGpuBuf *tau, SepiaGpuBuf *out, int64_t n_heads,
                        int64_t rel_extent, int64_t window, float inv_head_dim) {
     const char *op = "kv8_attn";
-    Kv8Args a;
-    Kv8Attn b;
+    Kv8Call a;
+    Kv8AttnCall b;
     if (!c || !lens || !starts || !q || !out || c->n_kv_heads < 1 || c->head_dim < 1 || n_heads < 1 ||
         n_heads > 65535 || n_heads % c->n_kv_heads || n_heads / c->n_kv_heads > 16 || window < 0 ||
         rel_extent < 0 || rel_extent > 0x7FFFFFFF || (rel_extent > 0) != (rel_logits != NULL) ||
@@ -247,24 +226,9 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
     return sepia_serve_launch(SK_KV8_ATTN + dim, (uint64_t)(budget + ids * c->n_kv_heads), 1, 1, 256, args, op);
 }
 
-/* struct SampleArgs of kernels/sample.h, and the bytes of its SampleRow and
- * SampleChunk */
-#define SAMPLE_ROW_BYTES (16384 * 8 + 8)
-#define SAMPLE_CHUNK_BYTES (1024 * 12 + 16)
 #define SAMPLE_CHUNKS 16    /* chunks of a row at most */
-#define SAMPLE_NT 512
 #define SAMPLE_CHUNK 8192   /* logits of a chunk at least */
 #define SAMPLE_PLACES 512   /* workgroups that the chip holds, two a CU */
-typedef struct {
-    const float *logits, *u, *temperature, *top_p, *min_p;
-    const int32_t *top_k;
-    int32_t *token;
-    float *prob;
-    uint8_t *rows, *bins;
-    int64_t stride;
-    int32_t vocab, chunk, chunks;
-} SampleArgs;
-
 int sepia_hip_sample(const SepiaSampleDesc *d, SepiaGpuBuf *logits, int64_t rows, int64_t vocab, int64_t stride,
                      SepiaGpuBuf *tokens, SepiaGpuBuf *prob) {
     const char *op = "sample";
@@ -320,15 +284,15 @@ int sepia_hip_sample(const SepiaSampleDesc *d, SepiaGpuBuf *logits, int64_t rows
     if (vocab < 3 * SAMPLE_CHUNK) chunks = 1;
     if (chunks > SAMPLE_PLACES / rows) chunks = SAMPLE_PLACES / rows;
     if (chunks > SAMPLE_CHUNKS) chunks = SAMPLE_CHUNKS;
-    const size_t per = SAMPLE_ROW_BYTES + SAMPLE_CHUNK_BYTES * (size_t)(chunks > 0 ? chunks : 1);
+    const size_t per = sizeof(SampleRow) + sizeof(SampleChunk) * (size_t)(chunks > 0 ? chunks : 1);
     if (chunks < 2 || (size_t)rows * per > sepia_scratch_limit()) chunks = 1;
     a.chunks = (int32_t)chunks;
     a.chunk = (int32_t)((vocab + chunks - 1) / chunks);
     void *args[] = { &a };
     if (chunks == 1) return sepia_serve_launch(SK_SAMPLE, 1, (unsigned)rows, 1, SAMPLE_NT, args, op);
-    a.rows = (uint8_t *)sepia_scratch((size_t)rows * per, op);
+    a.rows = (SampleRow *)sepia_scratch((size_t)rows * per, op);
     if (!a.rows) return 0;
-    a.bins = a.rows + (size_t)rows * SAMPLE_ROW_BYTES;
+    a.bins = (SampleChunk *)(a.rows + rows);
     for (int k = SK_SAMPLE_MAX; k <= SK_SAMPLE_PICK; k++)
         if (!sepia_serve_launch(k, (uint64_t)chunks, (unsigned)rows, 1, SAMPLE_NT, args, op)) return 0;
     return 1;
