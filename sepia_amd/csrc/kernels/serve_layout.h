@@ -39,7 +39,7 @@ typedef struct {
 } SampleChunk;
 typedef struct {
     unsigned long long list[SAMPLE_MANY];
-    uint32_t n, arrived;
+    uint32_t n, arrived, unused[2];   // a multiple of 16 bytes: the bins behind are read by pairs of masses
 } SampleRow;
 typedef struct {
     const float *logits, *u, *temperature, *top_p, *min_p;

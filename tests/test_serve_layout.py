@@ -35,6 +35,21 @@ def test_arguments_are_the_kernels(tmp_path, monkeypatch):
         assert seg[k] in (size, -(-size // 8) * 8 + 256), (k, seg[k], size)
 
 
+def test_bins_are_aligned(tmp_path):
+    """Pairs of 8-byte masses are one load of 16 bytes: the bins behind any number of rows begin at a multiple of that."""
+    r = build(tmp_path, r'''
+#include <stdio.h>
+#include <stddef.h>
+#include "serve_layout.h"
+int main(void) {
+    for (int rows = 1; rows < 40; rows++)
+        for (int chunk = 0; chunk < 3; chunk++)
+            if ((rows * sizeof(SampleRow) + chunk * sizeof(SampleChunk) + offsetof(SampleChunk, mass)) % 16) return rows;
+    return 0;
+}''')
+    assert r.returncode == 0
+
+
 def test_one_definition():
     csrc = os.path.join(ROOT, "sepia_amd", "csrc")
     shared = open(os.path.join(csrc, "kernels", "serve_layout.h")).read()
