@@ -389,6 +389,12 @@ static void **g_scratch_old;                /* held regions that were outgrown *
 static int g_scratch_olds;
 static size_t g_scratch_min;                /* twice the largest of them */
 
+/* Whether the library's stream is being captured (or cannot say). */
+static int capturing(void) {
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing(g_stream, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone;
+}
+
 /* Data region of at least `need` bytes (the counters sit in front of it).
  * Growing waits for the stream, since queued kernels may still use the old
  * region; the new allocation is cleared so every counter starts at zero.
@@ -400,13 +406,11 @@ static size_t g_scratch_min;                /* twice the largest of them */
  * its place has at least twice its size (where there is memory for that), so
  * that all the ones kept are together no larger than the last. */
 static void *scratch(size_t need, const char *op) {
-    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-    const int capturing = hipStreamIsCapturing(g_stream, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone;
     if (g_scratch && need <= g_scratch_len - CNT_BYTES) {
-        g_scratch_held |= capturing;
+        if (!g_scratch_held) g_scratch_held = capturing();   /* 67 ns */
         return (uint8_t *)g_scratch + CNT_BYTES;
     }
-    if (capturing) {
+    if (capturing()) {
         LOG("%s: needs %zu bytes of scratch but has %zu, and the stream is being captured (growing it would "
             "allocate); run the call once before the capture or call sepia_hip_reserve_scratch",
             op, need, g_scratch ? g_scratch_len - CNT_BYTES : (size_t)0);
@@ -541,8 +545,7 @@ static int pool_put(SepiaGpuBuf *b) {
  * become a node of the caller's graph (a fresh allocation fails there, at
  * its stream synchronisation, as before). */
 static SepiaGpuBuf *pool_take(size_t len, int kind) {
-    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(g_stream, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone) return NULL;
+    if (capturing()) return NULL;
     int i = g_pool_n - 1;
     while (i >= 0 && (g_pool[i].kind != kind || g_pool[i].len != len)) i--;
     if (i < 0) return NULL;
@@ -1370,8 +1373,7 @@ typedef struct {
 /* Bytes of scratch a call may use: what there is while the stream is being
  * captured, else any amount. */
 static size_t scratch_limit(void) {
-    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(g_stream, &cs) == hipSuccess && cs == hipStreamCaptureStatusNone) return SIZE_MAX;
+    if (!capturing()) return SIZE_MAX;
     return g_scratch ? g_scratch_len - CNT_BYTES : 0;
 }
 
