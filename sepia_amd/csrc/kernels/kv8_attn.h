@@ -62,9 +62,8 @@ __device__ __forceinline__ void kv8_cost(const Kv8Args &a, const Kv8Attn &b, int
                                          int &r1) {
     rt = steps = 0;
     if (s >= a.n_seqs || !kv8_seq(a, s, len, r0, r1) || r1 == r0) return;
-    const int end = len + (r1 - r0);
     rt = (r1 - r0 + b.TT - 1) / b.TT;
-    steps = (end + 63) / 64;
+    steps = kv8_steps(len + (r1 - r0));
     if (b.window > 0) steps = min(steps, (int)(((int64_t)b.window + b.TT + 61) / 64) + 1);
 }
 // Inclusive sums over the wave's lanes.

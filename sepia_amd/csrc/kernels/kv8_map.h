@@ -41,6 +41,9 @@ KV8_FN int kv8_seq_ok(int32_t len, int32_t r0, int32_t r1, int32_t n, int64_t ca
     return len >= 0 && r0 >= 0 && r1 >= r0 && r1 <= n && (int64_t)len + (r1 - r0) <= capacity;
 }
 
+// Steps of 64 columns that columns 0 .. end - 1 lie in, end > 0 (up to 2^31 - 1).
+KV8_FN int32_t kv8_steps(int32_t end) { return (end - 1) / 64 + 1; }
+
 // Slots [s0, s1) of page `page` of the sequence that the k-th touched page's
 // unit fills with the rows from r0 + (page << lg) + s0 - len on; 0 where there
 // is no such unit.

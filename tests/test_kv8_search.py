@@ -1,7 +1,9 @@
 """The search for the sequence that an id belongs to (kv8_find in kernels/kv8.h, a wave's lanes counted one by one here),
 in a CPU build of kernels/kv8_map.h: with starts that rise it finds the owner, and with starts that fall, which a call
 may be handed, no unit of what it finds lies outside the sequence's pages, rows and table."""
-from test_kv8_map import build
+import os
+
+from test_kv8_map import KDIR, build
 
 SEARCH = r'''
 #include <stdio.h>
@@ -79,3 +81,23 @@ int main(void) {
 def test_search_stays_inside(tmp_path):
     r = build(tmp_path, SEARCH, "-fsanitize=address,undefined")
     assert r.returncode == 0 and r.stdout.strip() == "1", (r.returncode, r.stdout, r.stderr[-500:])
+
+
+def test_steps_of_the_longest_sequences(tmp_path):
+    """The attention's steps of 64 columns, up to the last length that a table can hold (2^31 - 16 tokens): no sum on the
+    way passes 32 bits."""
+    r = build(tmp_path, r'''
+#include <stdio.h>
+#include "kv8_map.h"
+int main(void) {
+    const int32_t top = 2147483647;
+    for (int32_t end = 1; end < 5000; end++) {
+        if (kv8_steps(end) != (end + 63) / 64) return 1;
+        if (kv8_steps(top - end) != (int32_t)(((int64_t)top - end + 63) / 64)) return 2;
+    }
+    puts("ok");
+    return 0;
+}''', "-fsanitize=undefined", "-fno-sanitize-recover")
+    assert r.returncode == 0 and r.stdout.strip() == "ok", (r.returncode, r.stderr[-300:])
+    text = open(os.path.join(KDIR, "kv8_attn.h")).read()
+    assert "steps = kv8_steps(len + (r1 - r0));" in text
