@@ -104,6 +104,16 @@ int sepia_gpu_expert_ffn(const SepiaExpertTensor *gate, const SepiaExpertTensor 
  * No counterpart in the reference, whose cache is one sequence's f32 rows
  * (src/sepia.c:1203-1247) and whose next token is the host's arg-max. */
 
+/* A buffer over device memory that is the caller's ([dev, dev + len) within one
+ * allocation of device 0, dev a multiple of 16), without a copy: the serving
+ * calls below take it wherever they take a buffer, no others do (their kernels
+ * may read into the pad behind the library's own buffers). It has no host
+ * copy. sepia_gpu_free gives the handle back and leaves the memory, which has
+ * to stay until then, and for as long as a graph that was captured over it is
+ * replayed. The library's stream waits for the legacy default stream and the
+ * other way round; after work on any other stream the caller waits itself. */
+SepiaGpuBuf *sepia_hip_wrap_device(void *dev, size_t len);
+
 /* A layer's cache for n_seqs sequences. The pool holds n_pages pages of
  * `page` tokens (16, 32 or 64); page p is 2 * n_kv_heads * page * head_dim
  * bytes of codes at codes_off + p times that: K int8 [kv head][token][dim],

@@ -229,7 +229,7 @@ static const TypeInfo *type_info(int t) {
 }
 
 /* ------------------------------------------------------------ buffers --- */
-enum { BUF_SHARED = 0, BUF_PRIVATE = 1, BUF_WRAPPED = 2 };
+enum { BUF_SHARED = 0, BUF_PRIVATE = 1, BUF_WRAPPED = 2, BUF_FOREIGN = 3 /* the caller's device memory */ };
 
 /* Device allocations are padded by DEV_PAD bytes so a vectorised kernel may
  * read a full 16-byte line that straddles the logical end of a buffer. */
@@ -252,7 +252,7 @@ enum { BUF_SHARED = 0, BUF_PRIVATE = 1, BUF_WRAPPED = 2 };
 #define SHADOW_CHUNK ((size_t)1 << 16)
 struct SepiaGpuBuf {
     uint8_t *dev;
-    void *host;        /* pinned copy (shared), caller's base (wrapped), NULL (private) */
+    void *host;        /* pinned copy (shared), caller's base (wrapped), NULL (private, foreign) */
     size_t len;
     int kind;
     size_t ndirty;     /* chunks of the host copy that may be newer than the device copy */
@@ -307,7 +307,7 @@ int64_t sepia_row_bytes(int ggml_type, int64_t n) {
 }
 
 /* b holds [off, off + n) */
-static int chk(const SepiaGpuBuf *b, size_t off, size_t n, const char *op, const char *what) {
+static int chk_range(const SepiaGpuBuf *b, size_t off, size_t n, const char *op, const char *what) {
     if (!b || !b->dev) {
         LOG("%s: %s buffer is NULL", op, what);
         return 0;
@@ -317,6 +317,15 @@ static int chk(const SepiaGpuBuf *b, size_t off, size_t n, const char *op, const
         return 0;
     }
     return 1;
+}
+/* The same for a kernel that may read into the pad behind a buffer, which the
+ * caller's own memory does not have. */
+static int chk(const SepiaGpuBuf *b, size_t off, size_t n, const char *op, const char *what) {
+    if (b && b->kind == BUF_FOREIGN) {
+        LOG("%s: %s is not memory of the library's", op, what);
+        return 0;
+    }
+    return chk_range(b, off, n, op, what);
 }
 
 /* Bytes uploaded to shared buffers' device copies since init (tests read it
@@ -529,7 +538,7 @@ static PoolEnt pool_remove(int i) {
  * 0 if the pool does not take it (the caller frees it). The stream has
  * been synchronised: nothing queued uses b or the buffers released. */
 static int pool_put(SepiaGpuBuf *b) {
-    if (b->kind == BUF_WRAPPED || b->len > POOL_BUF_MAX) return 0;
+    if (b->kind == BUF_WRAPPED || b->kind == BUF_FOREIGN || b->len > POOL_BUF_MAX) return 0;
     const PoolEnt p = { b->dev, b->host, b->dirty, b->len, b->kind };
     while (g_pool_n > 0 && (g_pool_n == POOL_MAX || g_pool_bytes + pool_cost(&p) > POOL_BYTES_MAX)) {
         PoolEnt old = pool_remove(0);
@@ -643,6 +652,36 @@ SepiaGpuBuf *sepia_gpu_wrap_mmap(void *base, size_t len) {
     return b;
 }
 
+SepiaGpuBuf *sepia_hip_wrap_device(void *dev, size_t len) {
+    const char *op = "wrap_device";
+    if (!need_init(op)) return NULL;
+    if (!dev || len == 0 || (uintptr_t)dev % 16) {
+        LOG("%s: %p, %zu bytes: not an address that is a multiple of 16, and a length", op, dev, len);
+        return NULL;
+    }
+    hipPointerAttribute_t at;
+    void *base = NULL;
+    size_t size = 0;
+    hipError_t e = hipPointerGetAttributes(&at, dev);
+    if (e == hipSuccess && (at.type != hipMemoryTypeDevice || at.device != 0)) e = hipErrorInvalidDevicePointer;
+    if (e == hipSuccess) e = hipMemGetAddressRange((hipDeviceptr_t *)&base, &size, (hipDeviceptr_t)dev);
+    const size_t off = (size_t)((uintptr_t)dev - (uintptr_t)base);
+    if (e != hipSuccess || off > size || len > size - off) {
+        (void)hipGetLastError();   /* nothing of it is left for the caller's next call */
+        LOG("%s: [%p, +%zu) does not lie in one allocation of device 0", op, dev, len);
+        return NULL;
+    }
+    SepiaGpuBuf *b = (SepiaGpuBuf *)calloc(1, sizeof *b);
+    if (!b) {
+        LOG("%s: out of host memory", op);
+        return NULL;
+    }
+    b->dev = (uint8_t *)dev;
+    b->len = len;
+    b->kind = BUF_FOREIGN;
+    return b;
+}
+
 void sepia_gpu_free(SepiaGpuBuf *b) {
     if (!b) return;
     if (g_available) hipStreamSynchronize(g_stream);
@@ -659,13 +698,13 @@ void sepia_gpu_free(SepiaGpuBuf *b) {
         if (b->host) hipHostFree(b->host);
         free(b->dirty);
     }
-    if (b->dev) hipFree(b->dev);
+    if (b->dev && b->kind != BUF_FOREIGN) hipFree(b->dev);
     free(b);
 }
 
 void *sepia_gpu_host_ptr(SepiaGpuBuf *b) {
     if (!b) return NULL;
-    if (b->kind == BUF_PRIVATE) return NULL;
+    if (b->kind == BUF_PRIVATE || b->kind == BUF_FOREIGN) return NULL;
     if (b->kind == BUF_SHARED) {
         /* the caller may write anywhere in the copy from now on */
         memset(b->dirty, 0xFF, ((b->nchunks + 63) / 64) * sizeof(uint64_t));
@@ -974,7 +1013,7 @@ static int launch3(int k, unsigned gx, unsigned gy, unsigned gz, unsigned block,
 /* ---- more hooks for the other host files (internal.h) ---- */
 int sepia_need_batch(const char *op) { return need_batch(op); }
 int sepia_chk(const SepiaGpuBuf *b, size_t off, size_t n, const char *op, const char *what) {
-    return chk(b, off, n, op, what);
+    return chk_range(b, off, n, op, what);
 }
 int sepia_prep_in(SepiaGpuBuf *b, size_t off, size_t n, const char *op) { return prep_in_r(b, off, n, op); }
 int sepia_prep_out(SepiaGpuBuf *b, const char *op) { return prep_out(b, op); }

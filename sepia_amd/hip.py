@@ -102,6 +102,7 @@ PROTOTYPES = {
     "sepia_gpu_expert_ffn": (_I, [ctypes.POINTER(ExpertTensor), ctypes.POINTER(ExpertTensor),
                                   ctypes.POINTER(ExpertTensor), _I, _I, _I64, _I64, _P, _P]),
     # serving: the paged 8-bit key/value cache and sampling (serve.c)
+    "sepia_hip_wrap_device": (_P, [_P, _SZ]),
     "sepia_hip_kv8_append": (_I, [ctypes.POINTER(Kv8Cache), _P, _P, _I64, _P, _P, _P, _F]),
     "sepia_hip_kv8_read": (_I, [ctypes.POINTER(Kv8Cache), _P, _P, _I64, _P, _P]),
     "sepia_hip_kv8_attn": (_I, [ctypes.POINTER(Kv8Cache), _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _F]),
@@ -191,6 +192,12 @@ class Device:
     def alloc(self, nbytes, private=False):
         b = self.L.sepia_gpu_alloc(int(nbytes), 1 if private else 0)
         self.check(b, "alloc(%d)" % nbytes)
+        return b
+
+    def wrap(self, addr, nbytes):
+        """A buffer over device memory of another's (a tensor's data_ptr()), for the serving calls."""
+        b = self.L.sepia_hip_wrap_device(ctypes.c_void_p(int(addr)), int(nbytes))
+        self.check(b, "wrap_device(%d)" % nbytes)
         return b
 
     def free(self, b):
