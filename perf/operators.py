@@ -13,6 +13,7 @@ import math
 
 import torch
 
+# The library's buffers are handles over the tensors themselves (_Memory): both sides' state is made alike.
 own = False
 
 EPS = 1e-6
@@ -90,18 +91,16 @@ def _dev():
 
 
 class _Memory:
-    """A private device buffer of the library as torch takes it, given back when no tensor over it is left."""
+    """A buffer of the library's over a tensor's own memory: nothing is copied or laid out beforehand. Given back with
+    this object."""
 
-    def __init__(self, nbytes):
-        self.dev = _dev()
-        self.handle = self.dev.alloc(nbytes, private=True)
-        addr = self.dev.L.sepia_gpu_gpu_addr(self.handle)
-        self.__cuda_array_interface__ = dict(shape=(nbytes,), typestr="|u1", data=(addr, False), version=2)
+    def __init__(self, t):
+        dev = _dev()
+        self.free, self.handle = dev.free, dev.wrap(t.data_ptr(), t.numel() * t.element_size())
 
     def __del__(self):
         if getattr(self, "handle", None):
-            torch.cuda.synchronize()   # torch's work on it is done
-            self.dev.L.sepia_gpu_free(self.handle)
+            self.free(self.handle)
 
 
 class Buf:
@@ -110,10 +109,8 @@ class Buf:
     def __init__(self, t):
         t = t.contiguous()
         if own:
-            memory = _Memory(t.numel() * t.element_size())
-            self.handle = memory.handle
-            self.t = torch.as_tensor(memory, device="cuda").view(t.dtype).view(t.shape)
-            self.t.copy_(t)
+            self.memory = _Memory(t)
+            self.handle, self.t = self.memory.handle, t
         else:
             self.handle, self.t = None, t
 
