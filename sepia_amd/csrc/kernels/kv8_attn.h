@@ -97,7 +97,7 @@ __device__ __forceinline__ int kv8_plan(const Kv8Args &a, const Kv8Attn &b, int 
     // More tiles than the grid was made for: starts fall somewhere (an error,
     // kv8_check). No run then, since a unit with some of its runs would leave its
     // counter behind.
-    if (tiles > (float)(a.n / b.TT + a.n_seqs)) return 0;
+    if (tiles > (float)(a.n / b.TT + min(a.n, a.n_seqs))) return 0;
     const int chunk = b.budget > 0 ? max(KV8_NW, (int)ceilf(fminf(total * (float)a.Hkv / (float)b.budget, 1e9f))) : 0x7FFFFFFF;
     // A unit of two steps a wave stays whole: the fold takes longer than the
     // second step (32 sequences of up to 500 columns, 8 kv heads: 12.2 us against

@@ -195,7 +195,15 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
         return sepia_serve_launch(SK_KV8_ROWS + dim, (uint64_t)(n / (4 * b.TT) + c->n_seqs) * (uint64_t)c->n_kv_heads,
                                   1, 1, 256, args, op);
     }
-    const int64_t ids = n / b.TT + c->n_seqs;
+    /* Row tiles at most: sequences without rows have none. (4096 slots, a few in
+     * use: 2.6 ms with all counted.) A call past the grid of the kernel above is
+     * refused here too: whether it is does not go by the rows. */
+    if ((uint64_t)(n / b.TT + c->n_seqs) * (uint64_t)c->n_kv_heads * 256 > UINT32_MAX) {
+        LOG("%s: %lld row tiles and sequences of %d kv heads, more than a launch can have", op,
+            (long long)(n / b.TT + c->n_seqs), c->n_kv_heads);
+        return 0;
+    }
+    const int64_t ids = n / b.TT + (n < c->n_seqs ? n : c->n_seqs);
     const size_t per = 16 * (size_t)c->head_dim * 4, limit = sepia_scratch_limit();
     /* No more runs than places: a unit's last run is short, so as many fewer as
      * there are units (a whole round more for a few runs: 32 sequences in a
