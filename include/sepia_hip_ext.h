@@ -123,7 +123,9 @@ SepiaGpuBuf *sepia_hip_wrap_device(void *dev, size_t len);
  * of sequence s in order; entries behind its last token are not read. A page
  * may stand in several rows (a shared prefix) as long as no call appends to
  * it. head_dim: a multiple of 16 up to 128. codes_off a multiple of 16, the
- * others of 4; max_pages * page at most 2^31 - 1. */
+ * others of 4; max_pages * page at most 2^31 - 1. A scale is 0 or more, or NaN.
+ * The codes and scales belong in private buffers: a shared buffer that a batch
+ * appends to is downloaded whole at its sepia_gpu_end. */
 typedef struct {
     int64_t n_pages, max_pages;
     int n_seqs, n_kv_heads, head_dim, page;
@@ -167,7 +169,11 @@ int sepia_hip_kv8_read(const SepiaKv8Cache *cache, SepiaGpuBuf *first, SepiaGpuB
  * [head_dim] (out may be q); rel_logits f32 [n_tokens][n_heads][rel_extent],
  * NULL with rel_extent 0: no such term; tau f32 [n_tokens], NULL: 1. n_heads
  * is a multiple of n_kv_heads, up to 16 times. A row whose scores are all -inf
- * is NaN. */
+ * is NaN. The weighted sum is held in f32, weights of up to e^5: finite where a
+ * row's tokens times its largest cached |v| stay below 1e36. The launch counts
+ * n_seqs + n_tokens / (16 n_kv_heads / n_heads) workgroups and more for each kv
+ * head, of which HIP takes fewer than 2^24: past that the call is refused (65536
+ * sequences of 256 kv heads), also where few sequences have rows. */
 int sepia_hip_kv8_attn(const SepiaKv8Cache *cache, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n_tokens,
                        SepiaGpuBuf *q, SepiaGpuBuf *rel_logits, SepiaGpuBuf *tau, SepiaGpuBuf *out,
                        int64_t n_heads, int64_t rel_extent, int64_t window, float inv_head_dim);

@@ -69,8 +69,9 @@ __device__ __forceinline__ void sepia_kernarg_warm() {
 // Device error word and wait bound, set by the host when it loads the code
 // object (sepia_hip.c): sepia_err_word points at a host-visible word that
 // the host reads after each batch, sepia_wait_ticks bounds every spin wait
-// of a kernel in s_memrealtime ticks (100 MHz). The whole library is one
-// code object, so these are its only definitions.
+// of a kernel in s_memrealtime ticks (100 MHz). Both code
+// objects that the host loads define the error word; only sepia_kernels.hsaco
+// has spin waits, and their bound.
 // Both are constant memory: the kernels read them through the scalar cache.
 // (As plain device globals the bound was a vector load in every spin of a
 // wait, and under a launch's weight stream each such load took a loaded

@@ -164,8 +164,10 @@ __device__ __forceinline__ Kv8Scale kv8_rescale(float *scale, float old, float m
 // each 16 tokens of a page: four heads a workgroup with pages of 16, two of 32,
 // one of 64. What bounds it is the chain of dependent loads (arguments,
 // lengths, table entry, the old scale and codes) and the launch: 4.7 us for one
-// token (8 heads of 128), 8.6 for 61 sequences' tokens (16 heads), 19.9 for 5157
-// rows of prompts (8 heads; 53 MB, 2.7 TB/s). Twice as many waves of half the
+// token (8 heads of 128), 8.1 for 61 sequences' tokens (16 heads), 18.1 for 5157
+// rows of prompts (8 heads; 53 MB, 2.9 TB/s), in calls that append the rows over
+// themselves, so that no scale grows; 5.0, 9.7 and 18 where all of them do and the
+// codes before are rounded anew. Twice as many waves of half the
 // work took 11.3 us for the 61 and as long for the prompts; four waves a SIMD in
 // the place of three spilled and took 8.9 and 20.6.
 extern "C" __global__ __launch_bounds__(256, 3) void sepia_kv8_append(Kv8Args a, const float *__restrict__ k,

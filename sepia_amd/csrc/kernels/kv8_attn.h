@@ -572,9 +572,9 @@ __device__ __forceinline__ bool kv8_arrive(uint32_t *counter, int n) {
 }
 
 // Grid: the plan's runs, KV8_NW waves each. Bound by memory for long contexts
-// (48 sequences of 278000 columns in all, 8 kv heads of 128: 121 us, 4.8 TB/s),
+// (48 sequences of 278000 columns in all, 8 kv heads of 128: 118.5 us, 4.9 TB/s),
 // else by the chain from the plan to the fold: one sequence of 20000 columns
-// 17 us, 32 in a window of 512 20 us (16 kv heads).
+// 17.5 us, 32 in a window of 512 18.5 us (16 kv heads).
 template <int D, bool FULL>
 __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const Kv8Attn &b) {
     __shared__ kv8_f4 so[KV8_NW][Kv8Wave<D, FULL, false>::NC][64];
@@ -674,7 +674,7 @@ KV8_KERNEL(sepia_kv8_attn_to64, kv8_attn_run, 64, false)
 // side in a workgroup, so that they find K and V in the caches; nothing is cut
 // or folded. 2.6 us a step and pair of waves of a SIMD at dim 128; the loads alone
 // take 2.2, all but the loads 2.4, all but the matrix products 2.5. 500 rows
-// behind 1500 (64 heads on 8) 103 us. (K and V loaded once for the four and put
+// behind 1500 (64 heads on 8) 98 us. (K and V loaded once for the four and put
 // in shared memory: 2.8 us a step; that in steps of 128 columns: spills.) Grid: (ids of KV8_NW row tiles, kv heads), kv heads fastest, so
 // that with 8 of them an XCD's L2 holds one head's K and V.
 template <int D, bool FULL>

@@ -144,7 +144,16 @@ int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *
     return kv8_pages(SK_KV8_READ, c, n, &a, args, op);
 }
 
-#define KV8_ROWS 1024       /* units from which each has a wave of its own */
+/* Units from which each has a wave of its own (a whole chip of them at two
+ * workgroups a CU is 2048). Both kernels, wave a unit against cut into runs, us,
+ * dim 128, 64 heads on 8: a chunk of 192, 256, 384, 512 rows (768 to 2048 units)
+ * behind 200 columns 18, 23, 34, 40 against 20, 26, 38, 52, behind 1500 50, 53,
+ * 81, 89 against 40, 50, 74, 100. Sequences of single tokens, ragged up to the
+ * length: 128 (1024 units) of 500 columns 27 against 28, of 4000 138 against
+ * 104, of 16000 554 against 324; 256 of 500 44 against 59, of 16000 841 against
+ * 645; 1024 of 1000 227 against 480, since every run of a cut call looks through
+ * all lengths. So a number of units says too little where contexts are long. */
+#define KV8_ROWS 1024
 #define KV8_BUDGET 512      /* runs of a call whose units alone leave the chip idle: two workgroups a CU */
 _Static_assert(2 * (KV8_BUDGET * 3 / 2) + 64 <= KV8_UNITS && 2 * KV8_UNITS <= SEPIA_COUNTERS, "a counter for each slot, twice");
 
@@ -206,12 +215,15 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
     const int64_t ids = n / b.TT + (n < c->n_seqs ? n : c->n_seqs);
     const size_t per = 16 * (size_t)c->head_dim * 4, limit = sepia_scratch_limit();
     /* No more runs than places: a unit's last run is short, so as many fewer as
-     * there are units (a whole round more for a few runs: 32 sequences in a
-     * window of 512, 16 kv heads, 18.4 us against 13.9; 4 of up to 8000 columns
-     * 24.2 against 20.4). Half as many again as places where a run is
-     * long, since units of ragged lengths end unevenly (48 sequences of up to
-     * 12000 columns: 122 us against 131; 32 of 512: 29 against 20). None where
-     * a run has every step that the table or the window leaves a unit. */
+     * there are units (a whole round more for a few runs: 4 sequences of up to
+     * 8000 columns, 8 kv heads and a band of 1024, 16.4 us against 18.2 with 512
+     * runs). Half as many again as places where a run may be long, since units of
+     * ragged lengths end unevenly (48 sequences of up to 12000 columns: 118.5 us
+     * against 134.3 with 512; where runs are short they cost: 32 sequences in a
+     * window of 512, 16 kv heads, 18.5 us against 28.5). None, and no scratch,
+     * where a run has every step that the table or the window leaves a unit (as
+     * long either way). What a unit may have is taken from the table's width: the
+     * lengths are on the device. */
     int64_t steps = (c->max_pages * c->page + 63) / 64;   /* of a unit, at most */
     if (window > 0 && window / 64 + 2 < steps) steps = window / 64 + 2;
     int64_t budget = KV8_BUDGET - (units < KV8_BUDGET / 2 ? units : KV8_BUDGET / 2);
@@ -235,7 +247,7 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
 }
 
 #define SAMPLE_CHUNKS 16    /* chunks of a row at most */
-#define SAMPLE_CHUNK 8192   /* logits of a chunk at least */
+#define SAMPLE_CHUNK 8192   /* logits of a chunk: at most, and 6145 at least, unless the chunks have to be fewer */
 #define SAMPLE_PLACES 512   /* workgroups that the chip holds, two a CU */
 int sepia_hip_sample(const SepiaSampleDesc *d, SepiaGpuBuf *logits, int64_t rows, int64_t vocab, int64_t stride,
                      SepiaGpuBuf *tokens, SepiaGpuBuf *prob) {
