@@ -110,7 +110,8 @@ int sepia_gpu_expert_ffn(const SepiaExpertTensor *gate, const SepiaExpertTensor 
  * may read into the pad behind the library's own buffers). It has no host
  * copy. sepia_gpu_free gives the handle back and leaves the memory, which has
  * to stay until then, and for as long as a graph that was captured over it is
- * replayed. The library's stream waits for the legacy default stream and the
+ * replayed. What a call writes may not overlap what else it takes, in two
+ * handles over the same memory as in one buffer (kv8_attn's out may be q). The library's stream waits for the legacy default stream and the
  * other way round; after work on any other stream the caller waits itself. */
 SepiaGpuBuf *sepia_hip_wrap_device(void *dev, size_t len);
 

@@ -13,10 +13,36 @@
 #define MAX_ROWS ((int64_t)1 << 24)     /* rows of a call: grids of fewer than 2^32 threads */
 #define MAX_SAMPLES 65535              /* and of a sample call: the grid's second dimension */
 
+/* What a call reads or writes of a buffer. */
+typedef struct {
+    SepiaGpuBuf *b;
+    size_t off, n;
+    const char *what;
+} Part;
+/* What a call writes (bit i of `written`: part i) while other workgroups read
+ * the rest has to lie apart from all else, in one buffer or in two handles over
+ * the same memory. */
+static int apart(const char *op, const Part *p, int parts, unsigned written) {
+    for (int i = 0; i < parts; i++) {
+        if (!(written >> i & 1) || !p[i].b || !p[i].n) continue;
+        const uintptr_t at = (uintptr_t)sepia_buf_dev(p[i].b) + p[i].off;
+        for (int j = 0; j < parts; j++) {
+            if (j == i || !p[j].b || !p[j].n) continue;
+            const uintptr_t other = (uintptr_t)sepia_buf_dev(p[j].b) + p[j].off;
+            if (at + p[i].n <= other || other + p[j].n <= at) continue;
+            LOG("%s: %s overlaps %s", op, p[i].what, p[j].what);
+            return 0;
+        }
+    }
+    return 1;
+}
+
 /* Checks a cache and a call's rows, and fills the kernels' arguments; `write`:
- * the call writes to the pages. */
+ * the call writes to the pages. p: places for the cache's KV8_PARTS parts, then
+ * the call's own (`parts` in all). */
+enum { KV8_CODES, KV8_SCALES, KV8_TABLE, KV8_LENS, KV8_STARTS, KV8_PARTS };
 static int kv8_args(const char *op, const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n,
-                    int write, Kv8Call *a) {
+                    int write, Part *p, int parts, unsigned written, Kv8Call *a) {
     if (!c || c->n_pages < 1 || c->max_pages < 1 || c->n_seqs < 1 || c->n_seqs > 65536 || c->n_kv_heads < 1 ||
         c->n_kv_heads > 65535 || n < 0 || n > MAX_ROWS || c->n_pages > 0x7FFFFFFF) {
         LOG("%s: invalid arguments", op);
@@ -49,6 +75,12 @@ static int kv8_args(const char *op, const SepiaKv8Cache *c, SepiaGpuBuf *lens, S
         !sepia_chk(c->table, c->table_off, tb, op, "table") || !sepia_chk(lens, 0, lb, op, "lens") ||
         !sepia_chk(starts, 0, lb + 4, op, "starts"))
         return 0;
+    p[KV8_CODES] = (Part){ c->codes, c->codes_off, cb, "codes" };
+    p[KV8_SCALES] = (Part){ c->scales, c->scales_off, sb, "scales" };
+    p[KV8_TABLE] = (Part){ c->table, c->table_off, tb, "table" };
+    p[KV8_LENS] = (Part){ lens, 0, lb, "lens" };
+    p[KV8_STARTS] = (Part){ starts, 0, lb + 4, "starts" };
+    if (!apart(op, p, parts, written | (write ? 1u << KV8_CODES | 1u << KV8_SCALES : 0))) return 0;
     if (!sepia_need_batch(op) || !sepia_prep_in(c->table, c->table_off, tb, op) || !sepia_prep_in(lens, 0, lb, op) ||
         !sepia_prep_in(starts, 0, lb + 4, op))
         return 0;
@@ -71,15 +103,6 @@ static int kv8_args(const char *op, const SepiaKv8Cache *c, SepiaGpuBuf *lens, S
     a->head_bytes = (uint32_t)(c->page * c->head_dim);
     a->page_bytes = (uint32_t)page;
     return 1;
-}
-
-/* `out` is written while the inputs are read: it may be none of the cache's
- * buffers, nor one of the call's tables. */
-static int kv8_apart(const char *op, const SepiaKv8Cache *c, const SepiaGpuBuf *lens, const SepiaGpuBuf *starts,
-                     const SepiaGpuBuf *out, const char *what) {
-    if (out != c->codes && out != c->scales && out != c->table && out != lens && out != starts) return 1;
-    LOG("%s: %s is also an input", op, what);
-    return 0;
 }
 
 /* Units of pages, kv heads, K and V; a workgroup takes 64 tokens of the pages'
@@ -112,10 +135,8 @@ int sepia_hip_kv8_append(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf 
         if (c->n_kv_heads < 1 || c->head_dim < 1) LOG("%s: invalid arguments", op);
         return 0;
     }
-    if (!kv8_apart(op, c, lens, starts, k, "k") || !kv8_apart(op, c, lens, starts, v, "v") ||
-        (k_norm && !kv8_apart(op, c, lens, starts, k_norm, "k_norm")))
-        return 0;
-    if (!kv8_args(op, c, lens, starts, n, 1, &a) || !sepia_prep_in(k, 0, rows, op) || !sepia_prep_in(v, 0, rows, op) ||
+    Part p[KV8_PARTS + 3] = { [KV8_PARTS] = { k, 0, rows, "k" }, { v, 0, rows, "v" }, { k_norm, 0, nb, "k_norm" } };
+    if (!kv8_args(op, c, lens, starts, n, 1, p, KV8_PARTS + 3, 0, &a) || !sepia_prep_in(k, 0, rows, op) || !sepia_prep_in(v, 0, rows, op) ||
         (k_norm && !sepia_prep_in(k_norm, 0, nb, op)))
         return 0;
     if (n == 0) return 1;
@@ -134,10 +155,9 @@ int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *
         return 0;
     }
     const size_t rows = n < 0 || n > MAX_ROWS ? 0 : (size_t)n * (size_t)c->n_kv_heads * (size_t)c->head_dim * 4;
-    if (!sepia_chk(k, 0, rows, op, "k") || !sepia_chk(v, 0, rows, op, "v") ||
-        !kv8_apart(op, c, first, starts, k, "k") || !kv8_apart(op, c, first, starts, v, "v"))
-        return 0;
-    if (!kv8_args(op, c, first, starts, n, 0, &a) || !sepia_prep_out(k, op) || !sepia_prep_out(v, op)) return 0;
+    if (!sepia_chk(k, 0, rows, op, "k") || !sepia_chk(v, 0, rows, op, "v")) return 0;
+    Part p[KV8_PARTS + 2] = { [KV8_PARTS] = { k, 0, rows, "k" }, { v, 0, rows, "v" } };
+    if (!kv8_args(op, c, first, starts, n, 0, p, KV8_PARTS + 2, 3u << KV8_PARTS, &a) || !sepia_prep_out(k, op) || !sepia_prep_out(v, op)) return 0;
     if (n == 0) return 1;
     float *kp = (float *)sepia_buf_dev(k), *vp = (float *)sepia_buf_dev(v);
     void *args[] = { &a, &kp, &vp };
@@ -173,14 +193,13 @@ int sepia_hip_kv8_attn(const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *s
     const size_t rows = n < 0 || n > MAX_ROWS ? 0 : (size_t)n;
     const size_t qb = rows * (size_t)n_heads * (size_t)c->head_dim * 4, rb = rows * (size_t)n_heads * (size_t)rel_extent * 4;
     if (!sepia_chk(q, 0, qb, op, "q") || !sepia_chk(out, 0, qb, op, "out") ||
-        (rel_logits && !sepia_chk(rel_logits, 0, rb, op, "rel_logits")) || (tau && !sepia_chk(tau, 0, rows * 4, op, "tau")) ||
-        !kv8_apart(op, c, lens, starts, out, "out"))
+        (rel_logits && !sepia_chk(rel_logits, 0, rb, op, "rel_logits")) || (tau && !sepia_chk(tau, 0, rows * 4, op, "tau")))
         return 0;
-    if (out == rel_logits || out == tau) {
-        LOG("%s: out is also an input", op);
-        return 0;
-    }
-    if (!kv8_args(op, c, lens, starts, n, 0, &a) || !sepia_prep_in(q, 0, qb, op) ||
+    /* out may be q: a row of q is read by the workgroups whose last one writes it */
+    const int same = sepia_buf_dev(q) == sepia_buf_dev(out);
+    Part p[KV8_PARTS + 4] = { [KV8_PARTS] = { out, 0, qb, "out" }, { same ? NULL : q, 0, qb, "q" },
+                              { rel_logits, 0, rb, "rel_logits" }, { tau, 0, rows * 4, "tau" } };
+    if (!kv8_args(op, c, lens, starts, n, 0, p, KV8_PARTS + 4, 1u << KV8_PARTS, &a) || !sepia_prep_in(q, 0, qb, op) ||
         (rel_logits && !sepia_prep_in(rel_logits, 0, rb, op)) || (tau && !sepia_prep_in(tau, 0, rows * 4, op)) ||
         !sepia_prep_out(out, op))
         return 0;
@@ -267,17 +286,12 @@ int sepia_hip_sample(const SepiaSampleDesc *d, SepiaGpuBuf *logits, int64_t rows
     if (!sepia_chk(logits, 0, lb, op, "logits") || !sepia_chk(tokens, 0, rb, op, "tokens") ||
         (prob && !sepia_chk(prob, 0, rb, op, "prob")))
         return 0;
+    Part p[8] = { { tokens, 0, rb, "tokens" }, { prob, 0, rb, "prob" }, { logits, 0, lb, "logits" } };
     for (int i = 0; i < 5; i++) {
         if (in[i] && !sepia_chk(in[i], 0, rb, op, names[i])) return 0;
-        if (in[i] && (in[i] == tokens || in[i] == prob)) {
-            LOG("%s: %s is also an output", op, names[i]);
-            return 0;
-        }
+        p[3 + i] = (Part){ in[i], 0, rb, names[i] };
     }
-    if (tokens == prob || logits == tokens || logits == prob) {
-        LOG("%s: logits, tokens and prob are not three buffers", op);
-        return 0;
-    }
+    if (!apart(op, p, 8, 3)) return 0;
     if (!sepia_need_batch(op) || !sepia_prep_in(logits, 0, lb, op)) return 0;
     for (int i = 0; i < 5; i++)
         if (in[i] && !sepia_prep_in(in[i], 0, rb, op)) return 0;

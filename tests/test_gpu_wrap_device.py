@@ -112,10 +112,75 @@ def test_refusals(dev):
     for args in ((b, own, own), (own, b, own), (own, own, b)):
         assert L.sepia_gpu_add(*args, 16) == 0
     assert L.sepia_gpu_copy(b, 0, own, 0, 4) == 0 and L.sepia_gpu_matvec_q(8, b, 0, own, own, 1, 32) == 0
-    assert L.sepia_hip_sample(B(hip.SampleDesc(u=b)), own, 1, 16, 16, whole, None) == 1
+    head = wrap(at, 16)
+    assert L.sepia_hip_sample(B(hip.SampleDesc(u=b)), own, 1, 16, 16, head, None) == 1
     assert L.sepia_hip_sample(B(hip.SampleDesc(u=b)), own, 17, 1, 1, whole, None) == 0   # u past its 64 bytes
     dev.end()
     assert L.sepia_gpu_selftest_touch(b, 4) == 0
-    for x in (b, whole, own):
+    for x in (b, whole, own, head):
+        dev.free(x)
+    pool.free()
+
+
+def test_overlapping_handles(dev):
+    """Two handles over the same memory are refused where one buffer is: what a call writes lies apart from what else it
+    takes, by a byte's overlap; side by side, in one allocation or in one buffer, is taken."""
+    L, h = dev.L, Hip(dev)
+    pool = Pool(h, 1 << 20)
+    pool.put(0, np.zeros(1 << 20, np.uint8))
+    base, handles = pool.base.value, []
+
+    def at(off, n):
+        handles.append(dev.wrap(base + off, n))
+        return handles[-1]
+
+    heads, dim, page, n_pages, n, H, R, rows, vocab = 2, 16, 16, 4, 3, 4, 5, 4, 8
+    size = dict(codes=n_pages * 2 * heads * page * dim, scales=n_pages * 2 * heads * 4, table=16, lens=4, starts=8, k=n * heads * dim * 4,
+                v=n * heads * dim * 4, norm=dim * 4, q=n * H * dim * 4, out=n * H * dim * 4, rel=n * H * R * 4, tau=n * 4,
+                logits=rows * vocab * 4, u=rows * 4, p=rows * 4, tokens=rows * 4, prob=rows * 4)
+    off, place = {}, 0
+    for name, b in size.items():
+        off[name], place = place, place + (b + 15) // 16 * 16
+    pool.put(off["starts"], np.array([0, n], np.int32))
+
+    def calls(which, **moved):
+        o = dict(off, **moved)
+        b = {name: at(o[name], size[name]) for name in size}
+        d = hip.Kv8Cache(n_pages=n_pages, max_pages=4, n_seqs=1, n_kv_heads=heads, head_dim=dim, page=page, codes=b["codes"],
+                         scales=b["scales"], table=b["table"])
+        s = hip.SampleDesc(u=b["u"], top_p=b["p"])
+        return dict(append=lambda: L.sepia_hip_kv8_append(B(d), b["lens"], b["starts"], n, b["k"], b["v"], b["norm"], 1e-5),
+                    read=lambda: L.sepia_hip_kv8_read(B(d), b["lens"], b["starts"], n, b["k"], b["v"]),
+                    attn=lambda: L.sepia_hip_kv8_attn(B(d), b["lens"], b["starts"], n, b["q"], b["rel"], b["tau"], b["out"], H, R, 0, 1.0),
+                    sample=lambda: L.sepia_hip_sample(B(s), b["logits"], rows, vocab, vocab, b["tokens"], b["prob"]))[which]()
+
+    dev.begin()
+    assert [calls(w) for w in ("append", "read", "attn", "sample")] == [1, 1, 1, 1]   # side by side
+    assert calls("attn", q=off["out"]) == 1
+    writes = dict(append=("codes", "scales"), read=("k", "v"), attn=("out",), sample=("tokens", "prob"))
+    takes = dict(append=("codes", "scales", "table", "lens", "starts", "k", "v", "norm"), read=("codes", "scales", "table", "lens", "starts", "k", "v"),
+                 attn=("codes", "scales", "table", "lens", "starts", "q", "rel", "tau"), sample=("logits", "u", "p", "tokens", "prob"))
+    for which in writes:
+        for w in writes[which]:
+            for t in takes[which]:
+                if t == w:
+                    continue
+                last = off[w] + (size[w] - 1) // 16 * 16   # the 16 bytes with w's last
+                assert calls(which, **{t: last}) == 0, (which, w, t)
+                if (which, t) != ("attn", "q"):
+                    assert calls(which, **{t: off[w]}) == 0, (which, w, t)
+    assert calls("attn", q=off["out"] + 16) == 0
+    assert calls("append", k=off["v"]) == 1   # both are read
+    dev.end()
+    # in one buffer of the library's, at offsets
+    own = dev.alloc(1 << 16)
+    lens, starts, k = dev.shared_from(np.zeros(1, np.int32)), dev.shared_from(np.array([0, n], np.int32)), dev.alloc(size["k"])
+    dev.begin()
+    for scales_off, want in ((size["codes"], 1), (size["codes"] - 4, 0), (0, 0)):
+        d = hip.Kv8Cache(n_pages=n_pages, max_pages=4, n_seqs=1, n_kv_heads=heads, head_dim=dim, page=page, codes=own, scales=own,
+                         table=own, scales_off=scales_off, table_off=size["codes"] + size["scales"])
+        assert L.sepia_hip_kv8_append(B(d), lens, starts, n, k, k, None, 0.0) == want
+    dev.end()
+    for x in handles + [own, lens, starts, k]:
         dev.free(x)
     pool.free()
