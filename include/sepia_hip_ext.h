@@ -111,8 +111,9 @@ int sepia_gpu_expert_ffn(const SepiaExpertTensor *gate, const SepiaExpertTensor 
  * copy. sepia_gpu_free gives the handle back and leaves the memory, which has
  * to stay until then, and for as long as a graph that was captured over it is
  * replayed. What a call writes may not overlap what else it takes, in two
- * handles over the same memory as in one buffer (kv8_attn's out may be q). The library's stream waits for the legacy default stream and the
- * other way round; after work on any other stream the caller waits itself. */
+ * handles over the same memory as in one buffer (kv8_attn's out may be q). The
+ * library's stream waits for the legacy default stream and the other way round;
+ * after work on any other stream the caller waits itself. */
 SepiaGpuBuf *sepia_hip_wrap_device(void *dev, size_t len);
 
 /* A layer's cache for n_seqs sequences. The pool holds n_pages pages of
@@ -189,10 +190,10 @@ typedef struct {
 } SepiaSampleDesc;
 
 /* The next token of each row of logits (f32, up to 65535 rows, row r at element
- * r * stride, vocab values of it, 1 to 2^20). A token's weight is exp((logit - largest) /
- * temperature); -inf and NaN have none, nor has a token beside one of +inf. In the order of falling logits, equal
- * ones by index: the first top_k tokens are kept, of these the shortest
- * beginning with at least top_p of their weight, of these the ones of weight
+ * r * stride, vocab values of it, 1 to 2^20). A token's weight is exp((logit -
+ * largest) / temperature); -inf and NaN have none, nor has a token beside one
+ * of +inf. In the order of falling logits, equal ones by index: the first top_k
+ * tokens are kept, of these the shortest beginning with at least top_p of their weight, of these the ones of weight
  * min_p or more. tokens[r] (int32) is the first whose cumulative weight
  * exceeds u times the kept weight, -1 for a row without any finite or +inf
  * logit; prob[r] (f32, NULL: not wanted) its share of the kept weight. Sums of
