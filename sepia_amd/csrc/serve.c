@@ -9,6 +9,7 @@
 
 #include "../../include/sepia_hip_ext.h"
 #include "kernels/serve_layout.h"
+#include "kv8_route.h"
 
 #define LOG(...) sepia_log(__VA_ARGS__)
 #define MAX_ROWS ((int64_t)1 << 24)     /* rows of a call: grids of fewer than 2^32 threads */
@@ -165,39 +166,15 @@ int sepia_hip_kv8_read(const SepiaKv8Cache *c, SepiaGpuBuf *first, SepiaGpuBuf *
     return kv8_pages(SK_KV8_READ, c, n, &a, args, op);
 }
 
-/* Units from which each has a wave of its own (a whole chip of them at two
- * workgroups a CU is 2048). Both kernels, wave a unit against cut into runs, us,
- * dim 128, 64 heads on 8: a chunk of 192, 256, 384, 512 rows (768 to 2048 units)
- * behind 200 columns 18, 23, 34, 40 against 20, 26, 38, 52, behind 1500 50, 53,
- * 81, 89 against 40, 50, 74, 100. Sequences of single tokens, ragged up to the
- * length: 128 (1024 units) of 500 columns 27 against 28, of 4000 138 against
- * 104, of 16000 554 against 324; 256 of 500 44 against 59, of 16000 841 against
- * 645; 1024 of 1000 227 against 480, since every run of a cut call looks through
- * all lengths. So a number of units says too little where contexts are long. */
-#define KV8_ROWS 1024
-#define KV8_BUDGET 512      /* runs of a call whose units alone leave the chip idle: two workgroups a CU */
-_Static_assert(2 * (KV8_BUDGET * 3 / 2) + 64 <= KV8_UNITS && 2 * KV8_UNITS <= SEPIA_COUNTERS, "a counter for each slot, twice");
-
 /* What a call's rows see, and its kernels (kv8_attn.h): by runs, by rows. */
 typedef struct {
     const char *op;
     int tree, runs, rows, pair;
 } Kv8Kind;
+_Static_assert(2 * (KV8_BUDGET * 3 / 2) + 64 <= KV8_UNITS && 2 * KV8_UNITS <= SEPIA_COUNTERS, "a counter for each slot, twice");
 static const Kv8Kind kv8_window = { "kv8_attn", 0, SK_KV8_ATTN, SK_KV8_ROWS, 0 },
                      kv8_sinks = { "kv8_attn_sinks", 0, SD_SINKS_ATTN, SD_SINKS_ROWS, SD_SINKS_PAIR },
                      kv8_tree = { "kv8_attn_tree", 1, SD_TREE_ATTN, SD_TREE_ROWS, SD_TREE_PAIR };
-/* Steps of 64 columns up to which a unit is short. Short units that are more than
- * the chip holds workgroups go two to a workgroup, one round for two (40 single
- * tokens, 16 kv heads, window 512: 25.5 us against 27.5 with one; 9 trees of 64
- * rows, dim 64, window 300: 17.9 against 22.2). Trees' units that are not short
- * are cut into runs up to KV8_TREES of them: a wave alone with the longest takes
- * that long (24 trees of up to 33 rows behind up to 6000 columns: 183 us against
- * 233 a wave a unit; 50 behind 4000 238 against 269; 100 behind 3000, 13000 units,
- * 448 against 444; 200 behind 2500 780 against 671), and of up to KV8_TREES / 32
- * sequences, which every workgroup walks through (300 of 9 rows 424 against 429,
- * 600 of 5 542 against 485). */
-#define KV8_LONG 32
-#define KV8_TREES 8192
 static int kv8_attn(const Kv8Kind *kind, const SepiaKv8Cache *c, SepiaGpuBuf *lens, SepiaGpuBuf *starts,
                     SepiaGpuBuf *tree, int64_t n, SepiaGpuBuf *q, SepiaGpuBuf *rel_logits, SepiaGpuBuf *tau,
                     SepiaGpuBuf *out, int64_t n_heads, int64_t rel_extent, int64_t window, int64_t sinks,
@@ -235,20 +212,17 @@ static int kv8_attn(const Kv8Kind *kind, const SepiaKv8Cache *c, SepiaGpuBuf *le
     b->out = (float *)sepia_buf_dev(out);
     b->H = (int32_t)n_heads;
     b->R = (int32_t)rel_extent;
-    b->window = window > 0x7FFFFFFF ? 0 : (int32_t)window;
     b->c = inv_head_dim;
     m.tree = (const uint64_t *)sepia_buf_dev(tree);
-    m.sinks = !b->window ? 0 : sinks > 0x7FFFFFFF ? 0x7FFFFFFF : (int32_t)sinks;   /* without a window all is seen */
     /* 16 rows a wave. Many units (row tile, kv head): a wave each. Few: cut
      * into runs of steps, whose partials are folded. */
     b->TT = (int32_t)(16 / (n_heads / c->n_kv_heads));
     const int dim = 2 * (c->head_dim <= 64) + (c->head_dim % 64 != 0);   /* which of the four kernels */
-    const int64_t units = (n / b->TT > c->n_seqs ? n / b->TT : n < c->n_seqs ? n : c->n_seqs) * c->n_kv_heads;
-    int64_t steps = (c->max_pages * c->page + 63) / 64;   /* of a unit, at most: the lengths are on the device */
-    const int64_t wide = window / 64 + 2 + (m.sinks + 63) / 64 + kind->tree;   /* a tree's rows end 63 columns apart */
-    if (window > 0 && wide < steps) steps = wide;
-    const int cut = kind->tree && steps > KV8_LONG && units < KV8_TREES && c->n_seqs <= KV8_TREES / 32;
-    if (units >= KV8_ROWS && !cut) {
+    const Kv8Route to = kv8_route(n, c->n_seqs, c->n_kv_heads, b->TT, c->max_pages, c->page, window, sinks, kind->tree,
+                                  kind->pair != 0);
+    b->window = to.window;
+    m.sinks = to.sinks;
+    if (to.form == KV8_ROWS_FORM) {
         void *args[] = { &a, &m };
         return sepia_serve_launch(kind->rows + dim, (uint64_t)(n / (4 * b->TT) + c->n_seqs) * (uint64_t)c->n_kv_heads,
                                   1, 1, 256, args, op);
@@ -262,27 +236,12 @@ static int kv8_attn(const Kv8Kind *kind, const SepiaKv8Cache *c, SepiaGpuBuf *le
         return 0;
     }
     const int64_t ids = n / b->TT + (n < c->n_seqs ? n : c->n_seqs);
-    if (kind->pair && units > KV8_BUDGET && steps <= KV8_LONG) {
+    if (to.form == KV8_PAIR_FORM) {
         void *args[] = { &a, &m };
         return sepia_serve_launch(kind->pair + dim, (uint64_t)(ids * c->n_kv_heads + 1) / 2, 1, 1, 256, args, op);
     }
     const size_t per = 16 * (size_t)c->head_dim * 4, limit = sepia_scratch_limit();
-    /* No more runs than places: a unit's last run is short, so as many fewer as
-     * there are units (a whole round more for a few runs: 4 sequences of up to
-     * 8000 columns, 8 kv heads and a band of 1024, 16.4 us against 18.2 with 512
-     * runs). Half as many again as places where a run may be long, since units of
-     * ragged lengths end unevenly (48 sequences of up to 12000 columns: 118.5 us
-     * against 134.3 with 512; where runs are short they cost: 32 sequences in a
-     * window of 512, 16 kv heads, 18.5 us against 28.5). Not for trees whose units
-     * are mostly as long as their neighbours (one tree of 60 rows behind 20001
-     * columns 125.5 us against 144, 12 of up to 33 behind 6000 104.5 against 110;
-     * 12 of up to 9 behind 20000 106 against 90, so they keep it). None, and no scratch,
-     * where a run has every step that the table or the window leaves a unit (as
-     * long either way). */
-    int64_t budget = KV8_BUDGET - (units < KV8_BUDGET / 2 ? units : KV8_BUDGET / 2);
-    const int even = kind->tree && (c->n_seqs == 1 || n / b->TT >= 8 * c->n_seqs);
-    if (units * steps / KV8_BUDGET > 64 && !even) budget = KV8_BUDGET * 3 / 2;
-    if (steps <= KV8_NW) budget = 0;
+    int64_t budget = to.budget;
     int64_t slots = 2 * budget + 64;
     while (budget && (size_t)slots * (per + 128) > limit) {
         budget /= 2;
