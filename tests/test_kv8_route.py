@@ -73,3 +73,21 @@ def test_routes(tmp_path):
         ((200, 9, 8, 2, 600, 16, 300, 5, 1, 1), "pair"),
     ]
     assert [r[0] for r in route(tmp_path, [c for c, _ in want])] == [f for _, f in want]
+
+
+def test_every_kernel_has_a_case(tmp_path):
+    """The GPU tests' cases that are compared with the restatement reach all kernels of attention with sinks and over
+    trees, and each of test_gpu_kv8_routes the one that it is meant for."""
+    from test_gpu_kv8_masked import SINKS, TREES
+    from test_gpu_kv8_routes import CASES, KERNELS
+    cases = [("sinks",) + c for c in SINKS] + [("tree",) + c for c in TREES] + CASES
+    calls, names = [], []
+    for sees, H, heads, dim, page, lens, news, window, sinks, _ in cases:
+        sees = sees.split("_")[0]
+        n = H % 2 + sum(news) + H % 3
+        pages = 1 + max(1, max(-(-(a + b) // page) for a, b in zip(lens, news)))   # test_gpu_kv8.make's table
+        calls.append((n, len(lens), heads, 16 // (H // heads), pages, page, window, sinks, sees == "tree", 1))
+        names.append((sees, ("" if dim % 64 == 0 else "to") + ("64" if dim <= 64 else "128")))
+    reached = ["sepia_kv8_%s_%s_%s" % (sees, "attn" if r[0] == "runs" else r[0], dim) for (sees, dim), r in zip(names, route(tmp_path, calls))]
+    assert set(reached) == set(KERNELS)
+    assert reached[-len(CASES):] == ["sepia_kv8_" + c[0] for c in CASES]
