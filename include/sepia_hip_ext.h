@@ -235,7 +235,8 @@ int sepia_hip_kv8_keep(const SepiaKv8Cache *cache, SepiaGpuBuf *lens, SepiaGpuBu
  * tokens, s being r's sequence: rows row_starts[s] .. row_starts[s + 1] - 1 belong
  * to it, or (row_starts NULL) row s alone. Rows of a tree have besides the drafted
  * tokens of the rows on their path, themselves included (tree as in kv8_attn_tree,
- * the sequence's rows counted from row_starts[s], up to 64). With n the number of
+ * the sequence's rows counted from row_starts[s], up to 64); a list ends before the
+ * token of row 0, which row 0's own bit counts. With n the number of
  * times that a token occurs there, the first prompt[s] tokens of the list not
  * counted, a logit x of a token that occurs at all becomes x / repetition (x > 0) or
  * x * repetition; then x - frequency * n - presence where n > 0. Then the row's
