@@ -224,7 +224,10 @@ int sepia_hip_tree_accept(SepiaGpuBuf *tree, SepiaGpuBuf *starts, int64_t n_seqs
  * within a sequence. A page that a row moves to gets the largest of its tokens'
  * scales (NaN if one is), and its codes are rounded anew where that is larger (to 0
  * behind a scale of 0); where nothing moves nothing changes. What lies behind the
- * last kept row is not defined. Up to 64 rows a sequence; more, and entries that do
+ * last kept row is not defined. No scale becomes smaller: append has rounded a
+ * page's tokens for the largest of all drafts in it, also those that are dropped, and
+ * a dropped draft that is not finite leaves its page's head NaN (pages that end at
+ * lens[s] have no drafts). Up to 64 rows a sequence; more, and entries that do
  * not rise or lie outside its rows, are device error 7 and move nothing of it. The
  * pages moved to belong to one sequence alone. */
 int sepia_hip_kv8_keep(const SepiaKv8Cache *cache, SepiaGpuBuf *lens, SepiaGpuBuf *starts, int64_t n_tokens,

@@ -1,10 +1,14 @@
-"""What a drafting engine has to know of the calls around drafted trees: where a request's list ends."""
+"""What a drafting engine has to know of the calls around drafted trees: where a request's list ends, and what a draft
+that is not accepted leaves behind in the pages of accepted tokens."""
 import numpy as np
 import pytest
 
+import np_draft
+from np_serve import Cache
 from sepia_amd import hip
-from test_gpu_draft import adjust
-from test_gpu_kv8 import normal
+from test_gpu_draft import accept, adjust, keep
+from test_gpu_kv8 import B, OnGpu, append, ints, normal
+from test_gpu_kv8_masked import close, masked
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +33,71 @@ def test_list_ends_before_row_0(dev, vocab):
     twice = adjust(dev, x, vocab, [0, 4], lists=[old + drafted[:1]], words=words, drafted=drafted, out_stride=vocab, **rates)
     counted = adjust(dev, x, vocab, lists=[old + drafted[:1] + drafted[:i + 1] for i in range(4)], out_stride=vocab, **rates)
     assert np.array_equal(twice.view(np.uint32), counted.view(np.uint32)) and np.all(twice[:, 7] < got[:, 7])
+
+
+def read(dev, g, n_seqs, tokens):
+    """Keys and values of each sequence's positions from 0 on."""
+    starts = np.concatenate([[0], np.cumsum(tokens)])
+    n, kv = int(starts[-1]), g.c.heads * g.c.dim
+    bufs = [ints(dev, [0] * n_seqs), ints(dev, starts), dev.alloc(n * kv * 4), dev.alloc(n * kv * 4)]
+    dev.run(dev.L.sepia_hip_kv8_read, B(g.desc), bufs[0], bufs[1], n, bufs[2], bufs[3])
+    got = [dev.download(b, n * kv).reshape(n, g.c.heads, g.c.dim) for b in bufs[2:]]
+    for b in bufs:
+        dev.free(b)
+    return [[x[starts[s]:starts[s + 1]] for x in got] for s in range(n_seqs)]
+
+
+@pytest.mark.parametrize("value", [1000.0, np.nan])
+@pytest.mark.parametrize("sampled", [[50, 0, 0, 0, 0], [11, 0, 0, 0, 0], [12, 0, 0, 0, 0]], ids=["none", "stays", "moves"])
+def test_rejected_draft_stays_in_its_pages_scales(dev, value, sampled):
+    """A draft of one large value, or of a NaN, that is not accepted: the tokens of its page (those that were there, and
+    the accepted ones) keep that value's scale, also when rows move; other pages have nothing of it. A sequence whose
+    tokens end with a page keeps all that it had as it was."""
+    rng = np.random.default_rng(3)
+    heads, dim, page, lens, news = 2, 32, 16, [20, 16], [5, 5]
+    c = Cache(8, 2, 3, heads, dim, page, rng)
+    for s in range(2):
+        c.reserve(s, lens[s] + news[s])
+    g = OnGpu(dev, c)
+    k, v = normal(rng, 36, heads * dim), normal(rng, 36, heads * dim)
+    append(dev, g, [0, 0], [0, 20, 36], k, v)
+    c.append([0, 0], [0, 20, 36], k, v)
+    before = read(dev, g, 2, lens)
+    # rows 1 and 2 are row 0's children, row 3 row 1's, row 4 row 2's; row 3 has the value and is never accepted
+    words = np.array([1, 3, 5, 11, 21] * 2, np.uint64)
+    drafted, chosen = np.array([10, 11, 12, 13, 14] * 2), np.array(sampled * 2)
+    k, v = normal(rng, 10, heads * dim), normal(rng, 10, heads * dim)
+    for x in (k, v):
+        x[[3, 8], 5] = value   # of the first head
+    starts = [0, 5, 10]
+    append(dev, g, lens, starts, k, v)
+    c.append(lens, starts, k, v)
+    (kept, counts, _), _ = accept(dev, words, starts, drafted, chosen, 2)
+    assert list(counts) == ([1, 1] if sampled[0] == 50 else [2, 2]) and 3 not in kept
+    codes, scales, known = np_draft.keep(c, lens, starts, kept)
+    keep(dev, g, lens, starts, kept)
+    got = g.scales()
+    assert np.array_equal(np.isnan(got), np.isnan(scales)) and np.array_equal(got[~np.isnan(scales)], scales[~np.isnan(scales)])
+    known &= ~np.isnan(scales)[..., None]
+    assert np.array_equal(g.codes()[known], codes[known])
+    after = read(dev, g, 2, [a + int(b) for a, b in zip(lens, counts)])
+    step = np.float32(value) * np.float32(1 / 127)
+    for s in range(2):
+        hit = c.table[s, 1]   # the page of the drafts
+        assert np.all(np.isnan(got[hit, :, 0])) if np.isnan(value) else np.all(got[hit, :, 0] == step)
+        for was, now in zip(before[s], after[s]):
+            assert np.array_equal(now[:16], was[:16])                       # the first page, and the second head's drafts
+            assert np.all(np.abs(now[:, 1]) < 10)
+            if np.isnan(value):
+                assert np.isnan(now[16:, 0]).all()
+            else:   # half a step of the page's scale, and the product's own rounding
+                assert np.all(np.abs(now[16:lens[s], 0] - was[16:, 0]) <= step * np.float32(0.5001))
+                assert not np.array_equal(now[16:lens[s], 0], was[16:, 0]) or lens[s] == 16
+    # the next row sees the page as it is: NaN for the first head's queries
+    c.codes[:], c.scales[:] = g.codes(), got
+    lens = [a + int(b) for a, b in zip(lens, counts)]
+    q = normal(rng, 2, 4, dim)
+    want, tol = np_draft.attn(c, [a - 1 for a in lens], [0, 1, 2], q, scale=np.float32(1 / dim))
+    assert np.isnan(want[:, :2]).all() == np.isnan(value) and np.isfinite(want[:, 2:]).all()
+    close(masked(dev, g, [a - 1 for a in lens], [0, 1, 2], q, c=1 / dim), want, tol)
+    g.free()
