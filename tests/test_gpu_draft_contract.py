@@ -1,5 +1,5 @@
-"""What a drafting engine has to know of the calls around drafted trees: where a request's list ends, and what a draft
-that is not accepted leaves behind in the pages of accepted tokens."""
+"""What a drafting engine has to know of the calls around drafted trees: where a request's list ends, what a draft that is
+not accepted leaves behind in the pages of accepted tokens, and rows whose sequences' starts fall."""
 import numpy as np
 import pytest
 
@@ -101,3 +101,22 @@ def test_rejected_draft_stays_in_its_pages_scales(dev, value, sampled):
     assert np.isnan(want[:, :2]).all() == np.isnan(value) and np.isfinite(want[:, 2:]).all()
     close(masked(dev, g, [a - 1 for a in lens], [0, 1, 2], q, c=1 / dim), want, tol)
     g.free()
+
+
+def test_logits_rows_where_starts_fall(dev):
+    """Starts that fall: error 7, and each row is as it was or as a sequence that holds it has it."""
+    rng = np.random.default_rng(5)
+    vocab = 300
+    x = normal(rng, 6, vocab)
+    words, rates = np_draft.trees(rng, [0, 6], 6), np.full(6, 1.0, np.float32)
+    for starts in ([0, 2, 1, 6], [3, 6, 0, 3], [0, 6, 5, 2], [2, 0, 6, 6]):
+        got = adjust(dev, x, vocab, starts, lists=[[1], [2], [3]], words=words, drafted=[4] * 6, frequency=rates, ok=0)
+        for r in range(6):
+            right = [s for s in range(3) if starts[s] <= r < starts[s + 1] and not np.array_equal(got[r], x[r])]
+            if not np.array_equal(got[r].view(np.uint32), x[r].view(np.uint32)):
+                fits = []
+                for s in right:
+                    want, tol = np_draft.logits(x, starts[s:s + 2], vocab, lists=[[s + 1]], words=words, drafted=[4] * 6, frequency=rates)
+                    fits.append(bool(np.all(np.abs(got[r] - want[r]) <= tol[r])))
+                assert any(fits), (starts, r)
+    assert dev.L.sepia_hip_take_device_error() == 0
