@@ -9,7 +9,8 @@
 // Workgroup: (chunk of the vocabulary, row). It goes through the row's whole
 // list and counts what falls into its chunk in shared memory (whole numbers, so
 // the order does not matter), a word a token: the count, and in the highest bit
-// that it was seen. In place only logits that change are touched.
+// that it was seen. In place only logits that change are written, by masks alone of
+// many rows whole lines of memory with such a logit (sepia_logits_lines).
 //
 // Bound by memory where rows are many: 196 rows of 100003 with lists of up to 8000
 // tokens, masks and biases (157 MB) 43 us with three states in turn, 35 with one,
