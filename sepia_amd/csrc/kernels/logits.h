@@ -73,7 +73,7 @@ __device__ __forceinline__ logits_f4 logits_four(const float *x, uint32_t t, uin
     return v;
 }
 // A logit whose token's word is n. The quotient is the product with 1 / repetition in
-// double, off by 2^-53 before it is rounded.
+// double: two roundings of 2^-53, so off by up to 2^-52 before it is rounded to f32.
 __device__ __forceinline__ float logits_penal(float v, uint32_t n, float rep, double inv, float freq, float pres) {
     if (n == 0) return v;
     const float times = (float)(n & ~LOGITS_SEEN);
