@@ -264,9 +264,10 @@ typedef struct {
 /* Adjusted logits: row r of `logits` (f32, element r * stride, vocab values; up to
  * 65535 rows, vocab 1 to 2^20) to row r of out (element r * out_stride). out may be
  * logits, with the same stride: then all that is not to change keeps its bits, though
- * masks alone may write the lines of memory that they change whole, within a row. Lists, rows,
- * biases and masks are read on the device; rows outside all sequences, and rows whose
- * lists, biases or mask do not fit (device error 7), are left as they are. */
+ * masks alone may write the lines of memory that they change whole, within a row.
+ * Lists, rows, biases and masks are read on the device; rows outside all sequences,
+ * and rows whose lists, biases or mask do not fit (device error 7), are left as they
+ * are. */
 int sepia_hip_logits_adjust(const SepiaLogitsDesc *desc, SepiaGpuBuf *logits, int64_t rows, int64_t vocab,
                             int64_t stride, SepiaGpuBuf *out, int64_t out_stride);
 

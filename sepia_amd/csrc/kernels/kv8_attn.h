@@ -716,8 +716,12 @@ __device__ __forceinline__ bool kv8_arrive(uint32_t *counter, int n) {
 // 20001 columns (64 heads on 8) 70 us, of 13 row tiles a kv head; 24 trees of 502
 // rows behind 58900 columns 183 us. Two units a workgroup: 9 trees of 377 rows in a
 // window of 300 17.9 us (dim 64, 32 heads on 8), 40 sequences in a window of 512
-// behind 4 sinks 25.4 us (64 heads on 16). Those are bound by VALU and matrix
-// instructions that a wave issues in turn, two waves a SIMD.
+// behind 4 sinks 25.4 us (64 heads on 16). The trees behind long contexts are bound by
+// VALU and matrix instructions that a wave issues in turn (54 and 18% of SIMD cycles),
+// at two waves a SIMD; the pairs by latency: VALU 27-42%, 40% of wave cycles waiting,
+// 1.0-1.3 waves a SIMD on average. Registers: 224 and more above dim 64, where two waves
+// a SIMD fit; up to 64 the ones of sinks in pairs 165 and 167, where a third fits (168),
+// cut into runs 169 and 170, trees' 170 to 174.
 template <int D, bool FULL, int U, class B>
 __device__ __forceinline__ void kv8_attn_run(const Kv8Args &a, const B &b) {
     constexpr int NW = KV8_NW / U;   // waves of a unit

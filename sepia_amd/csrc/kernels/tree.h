@@ -8,7 +8,8 @@
 // was drafted with the row's sampled token; a child of row p is a row whose
 // path's rows before it are p's and p. One wave a sequence, lane i its row i:
 // a level is a ballot, at most 63 of them. Bound by the launch and two dependent
-// loads: 4.2 us for one sequence as for 250 of 7072 rows.
+// loads: 4.0-4.3 us by events around the launch, for one sequence as for 250 of 7072
+// rows (2.5 in a trace, which leaves the launch out).
 extern "C" __global__ __launch_bounds__(64) void sepia_tree_accept(TreeCall a) {
     serve_args<64>();
     const int s = (int)blockIdx.x, i = (int)threadIdx.x;

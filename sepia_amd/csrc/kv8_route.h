@@ -30,7 +30,12 @@
  * 233 a wave a unit; 50 behind 4000 238 against 269; 100 behind 3000, 13000 units,
  * 448 against 444; 200 behind 2500 780 against 671), and of up to KV8_TREES / 32
  * sequences, which every workgroup walks through (300 of 9 rows 424 against 429,
- * 600 of 5 542 against 485). */
+ * 600 of 5 542 against 485). Where this rule goes wrong, for all that it does not know:
+ * one tree of 25 rows behind 20001 columns, in a call of 1800 rows and 256 slots 116
+ * us, of 257 slots 493 (a wave a unit); 250 of 9 rows ragged up to 12000 columns 930 and
+ * 1094. And trees of 9 or 33 rows behind 200 columns whose table has room for 32768,
+ * so that they look long: 40 of 9 21.5 us against 19.6 with a table of their width, 40
+ * of 33 63.7 against 38.6 (dim 64: 29.7 against 22.5), 100 of 9 54 against 35. */
 #define KV8_LONG 32
 #define KV8_TREES 8192
 
@@ -68,7 +73,8 @@ static inline Kv8Route kv8_route(int64_t n, int64_t n_seqs, int64_t kv_heads, in
      * ragged lengths end unevenly (48 sequences of up to 12000 columns: 118.5 us
      * against 134.3 with 512; where runs are short they cost: 32 sequences in a
      * window of 512, 16 kv heads, 18.5 us against 28.5). Not for trees whose units
-     * are mostly as long as their neighbours (one tree of 60 rows behind 20001
+     * are likely to be as long as their neighbours, which 8 row tiles a sequence on
+     * average are taken for (one tree of 60 rows behind 20001
      * columns 125.5 us against 144, 12 of up to 33 behind 6000 104.5 against 110;
      * 12 of up to 9 behind 20000 106 against 90, so they keep it). None, and no scratch,
      * where a run has every step that the table or the window leaves a unit (as
