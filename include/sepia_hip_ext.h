@@ -347,8 +347,8 @@ uint64_t sepia_hip_uploaded_bytes(void);
 /* The first device error a kernel recorded since the last call, 0 if none,
  * and clears it. A kernel records one when a bounded spin wait expires (code
  * 5), a cache's table names a page outside its pool (6) or a sequence's
- * length or rows do not fit the call (7): its launch's outputs are then
- * invalid. sepia_gpu_end checks and
+ * length or rows, a list, biases or a mask do not fit the call (7): its
+ * launch's outputs are then invalid. sepia_gpu_end checks and
  * clears it itself and fails the batch (logging the code); callers that run
  * the library's launches without ending a batch (a captured graph replayed
  * on the library's stream) call this after synchronizing. No counterpart in

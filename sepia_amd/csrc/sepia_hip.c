@@ -955,7 +955,7 @@ int sepia_gpu_flush(void) {
 /* What a device error's code stands for. */
 static const char *device_error(unsigned code) {
     if (code == 6) return "a page of a cache's table lies outside its pool";
-    if (code == 7) return "a sequence's length or rows do not fit the call";
+    if (code == 7) return "a sequence's length or rows, a list, biases or a mask do not fit the call";
     return "a kernel's bounded wait expired";
 }
 

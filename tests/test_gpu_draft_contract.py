@@ -120,3 +120,12 @@ def test_logits_rows_where_starts_fall(dev):
                     fits.append(bool(np.all(np.abs(got[r] - want[r]) <= tol[r])))
                 assert any(fits), (starts, r)
     assert dev.L.sepia_hip_take_device_error() == 0
+
+
+def test_error_names_what_does_not_fit(dev, capfd):
+    """A mask that is not there: the batch fails, and the log line does not speak of lengths and rows alone."""
+    x = normal(np.random.default_rng(1), 2, 40)
+    got = adjust(dev, x, 40, masks=np.zeros((1, 2), np.uint32), mask_row=[0, 1], ok=0)
+    assert np.all(got[0] == -np.inf) and np.array_equal(got[1], x[1])
+    assert "rows, a list, biases or a mask do not fit the call (device error 7)" in capfd.readouterr().err
+    assert dev.L.sepia_hip_take_device_error() == 0
